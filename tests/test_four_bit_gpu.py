@@ -1,0 +1,360 @@
+"""Writing a cache in 4 bits, reading it back and attention over it, against plain numpy in 64 bits."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import four_bit as F
+from xyntetik_runner_amd.engine.batch import Chunked, StepContext, StepEntry, first_key
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+DT = {"float32": torch.float32, "bfloat16": torch.bfloat16}
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from xyntetik_runner_amd.csrc.ops import load_ops
+    return load_ops()
+
+
+def scattered(rng, lens, page):
+    """A block table a request, pages in any order, page 0 and two more nobody's."""
+    counts = [-(-n // page) for n in lens]
+    ids = rng.permutation(np.arange(1, sum(counts) + 3)).tolist()
+    return [[ids.pop() for _ in range(c)] for c in counts], sum(counts) + 3
+
+
+def step(starts, q_lens, tables):
+    from xyntetik_runner_amd.cache.manager import RequestCache
+    held = [RequestCache(b, b, s, [list(t)], False) for b, (s, t) in enumerate(zip(starts, tables))]
+    return StepContext(None, torch.device(DEV), [StepEntry(b, [0] * n) for b, n in enumerate(q_lens)], held, 1)
+
+
+class Recorded:
+    """The same step to a part that must not go by its lengths."""
+    knows_lengths = False
+
+    def __init__(self, ctx):
+        self.positions, self.req_of_token, self.block_table = ctx.positions, ctx.req_of_token, ctx.block_table
+        self.shared = {}
+
+
+def on_gpu(codes, scales, dim):
+    from xyntetik_runner_amd.csrc.ops import FourBitPages
+    return FourBitPages(torch.tensor(codes, device=DEV), torch.tensor(scales, device=DEV), dim)
+
+
+def host(pages):
+    return pages.codes.cpu().numpy(), pages.scales.cpu().numpy()
+
+
+def rotated(x, positions, inv_freq, rot, interleaved, mscale=1.0):
+    """64-bit rotation of [T, heads, D]; and the size of what every number was made of."""
+    y, size = x.copy(), np.abs(x)
+    if rot:
+        angle = positions[:, None].astype(np.float64) * inv_freq.astype(np.float64)
+        c, s = (np.cos(angle) * mscale)[:, None], (np.sin(angle) * mscale)[:, None]
+        i0 = np.arange(0, rot, 2) if interleaved else np.arange(rot // 2)
+        i1 = i0 + 1 if interleaved else i0 + rot // 2
+        a, b = x[..., i0], x[..., i1]
+        y[..., i0], y[..., i1] = a * c - b * s, a * s + b * c
+        size[..., i0] = size[..., i1] = (np.abs(a) + np.abs(b)) * abs(mscale)
+    return y, size
+
+
+WRITES = [
+    # H, Hk, D, Dv, rot, interleaved, paired, page, starts, q_lens
+    (4, 2, 128, 128, 128, False, True, 64, [0, 63, 64, 1000], [1, 1, 1, 1]),
+    (8, 2, 64, 64, 64, False, False, 32, [0, 31, 5], [70, 3, 8]),
+    (2, 2, 128, 128, 64, False, True, 64, [131000], [40]),                    # half of a head rotated; far positions
+    (3, 1, 80, 80, 80, True, False, 16, [3, 7], [9, 1]),                      # pairs side by side; a last block of 16
+    (6, 3, 96, 96, 20, False, False, 128, [250, 0], [5, 200]),                # a rotary width whose half is no multiple of 8
+    (4, 4, 16, 32, 16, False, False, 8, [0], [33]),                           # values of another size; pages of 8
+    (2, 1, 256, 192, 256, False, True, 64, [62], [4]),
+    (5, 5, 8, 8, 0, False, False, 16, [15, 16], [2, 1]),                      # no rotation; a block of 8
+    (0, 2, 64, 64, 64, False, False, 64, [9], [3]),                           # no queries
+]
+
+
+@pytest.mark.parametrize("case", WRITES)
+@pytest.mark.parametrize("dt", ["bfloat16", "float32"])
+def test_write(ops, case, dt):
+    from xyntetik_runner_amd.csrc.ops import paired_order
+    H, Hk, D, Dv, rot, interleaved, paired, page, starts, q_lens = case
+    rng = np.random.default_rng(D + rot + len(starts))
+    lens = [s + n for s, n in zip(starts, q_lens)]
+    tables, n_pages = scattered(rng, lens, page)
+    ctx = step(starts, q_lens, tables)
+    T = sum(q_lens)
+    inv = (1.0 / 10000.0 ** (np.arange(0, max(rot, 2), 2) / max(rot, 2))).astype(np.float32)[:max(rot // 2, 1)]
+    x = (rng.normal(size=(T, (H + Hk) * D + Hk * Dv + 3)) * np.exp(rng.normal(size=(T, 1)))).astype(np.float32)
+    empty = [([np.zeros((0, Hk, d), dtype=np.uint8)] * 3) for d in (D, Dv)]
+    k0, v0 = (F.fill_pages([e] * len(lens), tables, n_pages, page, values, junk=rng) for e, values in zip(empty, (False, True)))
+    kp, vp = on_gpu(*k0, D), on_gpu(*v0, Dv)
+    proj = torch.tensor(x, device=DEV)          # rows of an odd stride: nothing is 16-byte aligned
+    q_in, k_in, v_in = proj[:, :H * D], proj[:, H * D:(H + Hk) * D], proj[:, (H + Hk) * D:(H + Hk) * D + Hk * Dv]
+    q = torch.full((T, H * D), 7.0, dtype=DT[dt], device=DEV)
+    ops.rope_kv_write(q_in if H else None, k_in, v_in, q if H else None, kp, vp, ctx.positions, ctx.req_of_token, ctx.block_table(0),
+                      torch.tensor(inv, device=DEV) if rot else None, H, Hk, D, rot, interleaved, 1.25, page, paired=paired)
+    pos = ctx.positions.cpu().numpy()
+    x64 = x.astype(np.float64)
+    qk = x64[:, :(H + Hk) * D].reshape(T, H + Hk, D)
+    if paired:                                   # column c of the input holds channel order[c]
+        ckpt = np.empty_like(qk)
+        ckpt[..., paired_order(D, rot)] = qk
+        qk = ckpt
+    want, size = rotated(qk, pos, inv, rot, interleaved, 1.25)
+    if H:
+        got = q.cpu().double().numpy().reshape(T, H, D)
+        # half a step of the type, and of 32 bits: cosine, sine (2 steps each from the angle on), two products and a sum
+        eps = 2.0 ** -8 if dt == "bfloat16" else 0.0
+        assert (np.abs(got - want[:, :H]) <= eps * np.abs(want[:, :H]) + 8 * 2.0 ** -24 * size[:, :H]).all()
+    v64 = x64[:, (H + Hk) * D:(H + Hk) * D + Hk * Dv].reshape(T, Hk, Dv)
+    (kc, ks), (vc, vs) = host(kp), host(vp)
+    row = 0
+    for b, n in enumerate(q_lens):
+        places = [starts[b] + i for i in range(n)]
+        for codes, scales, values, ref, off_by in ((kc, ks, False, want[row:row + n, H:], size[row:row + n, H:]), (vc, vs, True, v64[row:row + n], 0.0 * np.abs(v64[row:row + n]))):
+            got = F.pages_rows(codes, scales, tables[b], places, page, values)
+            pb = np.array([[tables[b][p // page], p % page] for p in places])
+            byte = scales[pb[:, 0], :, pb[:, 1] // 8, :, pb[:, 1] % 8].astype(np.float64)
+            unit = np.repeat(2.0 ** (byte - 127), 32, axis=-1)[..., :ref.shape[-1]]
+            a = np.abs(ref) / unit
+            gap = np.where(a >= 4, 2.0, np.where(a >= 2, 1.0, 0.5)) * unit
+            slack = 8 * 2.0 ** -24 * off_by
+            # half a step, and as much more as the rotated number itself is off by 32-bit arithmetic
+            assert (np.abs(got - ref) <= gap / 2 + slack + 1e-12 * np.abs(ref)).all()
+            lo, hi = (np.vectorize(lambda t: t)(np.abs(ref) - slack), np.abs(ref) + slack)
+            for block in range(scales.shape[3]):
+                at = slice(32 * block, 32 * block + 32)
+                least, most = (np.array([[F.scale_byte(r[at]) for r in tok] for tok in t]) for t in (np.maximum(lo, 0), hi))
+                assert ((least <= byte[..., block]) & (byte[..., block] <= most)).all()
+            if values:                            # (no rotation: the codes are exactly the oracle's)
+                assert np.array_equal(got, F.rounded(ref)[2])
+        row += n
+    # what the step does not own is as it was
+    mine = {(tables[b][p // page], p % page) for b, n in enumerate(q_lens) for p in range(starts[b], starts[b] + n)}
+    for (c0, s0), (c1, s1), values in ((k0, (kc, ks), False), (v0, (vc, vs), True)):
+        for p in range(n_pages):
+            for off in range(page):
+                if (p, off) not in mine:
+                    assert np.array_equal(s0[p, :, off // 8, :, off % 8], s1[p, :, off // 8, :, off % 8])
+                    if values:
+                        assert np.array_equal(c0[p, :, off // 8, :, off % 8], c1[p, :, off // 8, :, off % 8])
+                    else:
+                        assert np.array_equal(c0[p, :, off], c1[p, :, off])
+
+
+def test_write_of_special_numbers(ops):
+    """Blocks of zeros, of one sign, with ties, at both ends of the scales, with a NaN or an infinity: the oracle's bytes."""
+    rng = np.random.default_rng(5)
+    rows = np.zeros((16, 1, 64), dtype=np.float32)
+    rows[1] = -0.0
+    rows[2, 0, :9] = [0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 7.0, -5.0]
+    rows[3] = rng.normal(size=64) * 1e-39          # subnormal
+    rows[4] = rng.normal(size=64) * 1e-36
+    rows[5] = rng.choice([3.4e38, -3.3e38, 2.6e38, 1e38], size=64)
+    rows[6, 0, 3] = np.nan
+    rows[7, 0, 40] = np.inf
+    rows[8, 0, 63] = -np.inf
+    rows[9] = rng.normal(size=64)
+    rows[9, 0, 33] = np.float32(1.75) * 4
+    rows[10] = np.nextafter(np.float32(7.0), np.float32(8.0))
+    rows[11] = 6.999
+    rows[12:] = rng.normal(size=(4, 1, 64)) * 10.0 ** rng.integers(-30, 30, size=(4, 1, 1))
+    T = len(rows)
+    ctx = step([0], [T], [[1]])
+    from xyntetik_runner_amd.csrc.ops import FourBitPages
+    kp, vp = (FourBitPages.zeros(2, 1, 16, 64, values, DEV) for values in (False, True))
+    x = torch.tensor(rows.reshape(T, 64), device=DEV)
+    ops.rope_kv_write(None, x, x, None, kp, vp, ctx.positions, ctx.req_of_token, ctx.block_table(0), None, 0, 1, 64, 0, False, 1.0, 16)
+    codes, scales, numbers = F.rounded(rows.astype(np.float64))
+    for pages, values in ((kp, False), (vp, True)):
+        c, s = F.fill_pages([(codes, scales, numbers)], [[1]], 2, 16, values)
+        gc, gs = host(pages)
+        assert np.array_equal(gs, s) and np.array_equal(gc, c)
+    for dt in DT.values():
+        for got in ops.read_rows(kp, vp, ctx.positions, ctx.req_of_token, ctx.block_table(0), dt):
+            assert np.array_equal(got.double().cpu().numpy().reshape(rows.shape), numbers, equal_nan=True)
+
+
+READS = [(2, 128, 128, 64, [1, 63, 64, 65, 200]), (1, 256, 192, 32, [33]), (3, 80, 48, 16, [100, 5]), (4, 64, 64, 128, [129, 1000]), (1, 8, 16, 8, [9]), (2, 32, 32, 64, [70])]
+
+
+@pytest.mark.parametrize("Hk,D,Dv,page,lens", READS)
+@pytest.mark.parametrize("dt", ["bfloat16", "float32"])
+def test_reading_back(ops, Hk, D, Dv, page, lens, dt):
+    """Rows in any order, some twice, one without a page; whole pages with zeros behind a request's end.  Exact: every number is one of the type's."""
+    rng = np.random.default_rng(D + page)
+    tables, n_pages = scattered(rng, lens, page)
+    ks, vs = ([F.random_sequence(rng, n, Hk, d) for n in lens] for d in (D, Dv))
+    kp = on_gpu(*F.fill_pages(ks, tables, n_pages, page, False, junk=rng), D)
+    vp = on_gpu(*F.fill_pages(vs, tables, n_pages, page, True, junk=rng), Dv)
+    ctx = step([n - 1 for n in lens], [1] * len(lens), tables)
+    places = [(b, p) for b, n in enumerate(lens) for p in rng.integers(0, n, size=min(n, 40)).tolist()] + [(0, 0), (0, 0)]
+    places = [places[i] for i in rng.permutation(len(places))]
+    req, pos = (torch.tensor([x[i] for x in places] + [0], dtype=torch.int32, device=DEV) for i in (0, 1))
+    pos[-1] = page * ctx.block_table(0).shape[1] + 5          # past the table
+    k, v = ops.read_rows(kp, vp, pos, req, ctx.block_table(0), DT[dt])
+    for got, seqs, d in ((k, ks, D), (v, vs, Dv)):
+        want = np.stack([seqs[b][2][p] for b, p in places] + [np.zeros((Hk, d))])
+        assert np.array_equal(got.double().cpu().numpy().reshape(want.shape), want)
+    k, v, table = ops.read_pages(kp, vp, ctx, 0, DT[dt])
+    assert k.dtype == v.dtype == DT[dt] and len(k) == len(v) == sum(-(-n // page) for n in lens)
+    k, v, table = k.double().cpu().numpy(), v.double().cpu().numpy(), table.cpu().numpy()
+    seen = []
+    for b, n in enumerate(lens):
+        for i in range(table.shape[1]):
+            if i * page >= n:
+                assert table[b, i] == -1
+                continue
+            m = min(page, n - i * page)
+            seen.append(table[b, i])
+            pk, pv = k[table[b, i]].transpose(1, 0, 2), v[table[b, i]].transpose(2, 0, 1)
+            assert np.array_equal(pk[:m], ks[b][2][i * page:i * page + m]) and not pk[m:].any()
+            assert np.array_equal(pv[:m], vs[b][2][i * page:i * page + m]) and not pv[m:].any()
+    assert seen == list(range(len(k)))
+    some = ops.read_pages(kp, vp, ctx, 0, DT[dt], requests=(len(lens) - 1,))
+    last = -(-lens[-1] // page)
+    assert len(some[0]) == last and torch.equal(some[0].cpu().double(), torch.tensor(k[len(k) - last:])) and int(some[2].max()) == last - 1
+
+
+def ref(qs, ks, vs, starts, Hk, scale, mask=None, keep=0, sinks=None, slopes=None, cap=0.0, gate=None, out_scale=1.0):
+    out, r = [], 0
+    for b, q in enumerate(qs):
+        for i in range(len(q)):
+            p = starts[b] + i
+            js = np.array(sorted(set(range(min(keep, p + 1) if mask else 0)) | set(range(first_key(mask, p), p + 1))))
+            H = q.shape[1]
+            row = []
+            for h in range(H):
+                g = h // (H // Hk)
+                s = ks[b][js, g] @ q[i, h] * scale
+                if cap:
+                    s = cap * np.tanh(s / cap)
+                if slopes is not None:
+                    s = s - slopes[h] * (p - js)
+                top = max(s.max(), sinks[h]) if sinks is not None else s.max()
+                e = np.exp(s - top)
+                o = e / (e.sum() + (np.exp(sinks[h] - top) if sinks is not None else 0.0)) @ vs[b][js, g]
+                row.append(o * (1 / (1 + np.exp(-gate[r, h])) if gate is not None else 1.0) * out_scale)
+            out.append(np.stack(row))
+            r += 1
+    return np.stack(out)
+
+
+ATTEND = [
+    # H, Hk, D, Dv, page, mask, starts, q_lens
+    (8, 2, 128, 128, 64, None, [0, 63, 64, 127, 500, 1900], [1] * 6),
+    (4, 1, 32, 32, 32, None, [0, 31, 32, 33], [1, 1, 1, 1]),
+    (8, 2, 64, 64, 64, None, [1000, 5, 191, 192, 193], [1, 4, 3, 2, 1]),
+    (16, 1, 64, 32, 32, None, [300, 2], [1, 1]),
+    (5, 5, 128, 128, 128, 100, [0, 99, 100, 101, 700], [16, 9, 3, 1, 2]),
+    (6, 2, 256, 256, 32, None, [400, 2], [5, 1]),
+    (4, 2, 256, 128, 64, Chunked(64), [63, 64, 200], [2, 1, 3]),
+    (4, 2, 128, 128, 64, None, [5000], [1]),
+    (3, 3, 96, 96, 32, 33, [3000, 40], [1, 1]),
+    (4, 2, 64, 64, 64, None, [0, 300, 10], [130, 1, 33]),                  # a portion beside a decoded token
+    (24, 1, 128, 128, 64, None, [333, 64], [1, 3]),                        # more heads than 16 over one
+    (4, 2, 80, 48, 16, 50, [10, 130], [40, 1]),
+    (2, 2, 16, 16, 16, None, [0, 200], [1, 20]),
+    (2, 1, 8, 8, 8, None, [11], [3]),
+]
+
+
+def attend(ops, case, dt, seed, recorded=False, **opt):
+    H, Hk, D, Dv, page, mask, starts, q_lens = case
+    rng = np.random.default_rng(seed)
+    lens = [s + n for s, n in zip(starts, q_lens)]
+    tables, n_pages = scattered(rng, lens, page)
+    ks, vs = ([F.random_sequence(rng, n, Hk, d) for n in lens] for d in (D, Dv))
+    kp = on_gpu(*F.fill_pages(ks, tables, n_pages, page, False, junk=rng), D)
+    vp = on_gpu(*F.fill_pages(vs, tables, n_pages, page, True, junk=rng), Dv)
+    keep = opt.get("keep", 0)
+    if mask:                                     # what the mask has passed was given back
+        for b, s in enumerate(starts):
+            for i in range(-(-keep // page), first_key(mask, s) // page):
+                tables[b][i] = -1
+    ctx = step(starts, q_lens, tables)
+    T, scale = sum(q_lens), 1.1 / math.sqrt(D)
+    qt = [torch.tensor(rng.normal(size=(n, H, D)) * 1.5).to(DT[dt]) for n in q_lens]
+    sinks = np.concatenate([[30.0], rng.normal(size=H - 1) * 2]).astype(np.float32) if opt.get("sinks") else None
+    slopes = (2.0 ** -np.linspace(2, 7, H)).astype(np.float32) if opt.get("slopes") else None
+    gate = rng.normal(size=(T, H + 2)).astype(np.float32) if opt.get("gate") else None
+    dev = lambda a: torch.tensor(a, device=DEV)
+    want = ref([t.double().numpy() for t in qt], [k[2] for k in ks], [v[2] for v in vs], starts, Hk, scale, mask, keep,
+               sinks, slopes, opt.get("cap", 0.0), gate, opt.get("out_scale", 1.0))
+    q = torch.cat(qt).reshape(T, H * D).contiguous().to(DEV)
+    room = torch.full((T, H * Dv + 8), 3.0, dtype=DT[dt], device=DEV)
+    for _ in range(2):
+        got = ops.attention(q, kp, vp, Recorded(ctx) if recorded else ctx, 0, H, Hk, D, page, scale, mask if isinstance(mask, int) else None,
+                            slopes=dev(slopes) if slopes is not None else None, chunk=mask.size if isinstance(mask, Chunked) else None,
+                            keep_first=keep, sinks=dev(sinks) if sinks is not None else None, v_head_dim=Dv, softcap=opt.get("cap", 0.0),
+                            gate=dev(gate)[:, :H] if gate is not None else None, out_scale=opt.get("out_scale", 1.0), out=room[:, :H * Dv])
+        assert (room[:, H * Dv:] == 3.0).all()
+        got = got.cpu().double().numpy().reshape(T, H, Dv)
+        assert np.isfinite(got).all()
+        # probabilities and the result in bfloat16 (2^-9 each of a value) against the largest output, as over 16-bit pages; 32 bits: sums of
+        # up to 5,000 products, exponentials of scores up to 30 that are off by 2^-22
+        assert np.abs(got - want).max() <= (1.2e-2 if dt == "bfloat16" else 2e-5) * np.abs(want).max()
+    return got
+
+
+@pytest.mark.parametrize("case", ATTEND)
+@pytest.mark.parametrize("dt", ["bfloat16", "float32"])
+@pytest.mark.parametrize("recorded", [False, True])
+def test_attention(ops, case, dt, recorded):
+    attend(ops, case, dt, 11 + case[2], recorded)
+
+
+OPTIONS = {"sinks": dict(sinks=True), "slopes": dict(slopes=True), "cap and sinks": dict(cap=1.3, sinks=True),
+           "gate": dict(gate=True, out_scale=0.75), "slopes, sinks, gate": dict(slopes=True, sinks=True, gate=True, out_scale=1.5),
+           "kept keys": dict(keep=5), "kept keys, sinks, cap": dict(keep=70, sinks=True, cap=1.3)}
+
+
+@pytest.mark.parametrize("what", OPTIONS)
+@pytest.mark.parametrize("shape", [(8, 2, 64, 64), (4, 1, 128, 64), (2, 2, 48, 32)])
+@pytest.mark.parametrize("recorded", [False, True])
+@pytest.mark.parametrize("dt", ["bfloat16", "float32"])
+def test_attention_with(ops, what, shape, recorded, dt):
+    H, Hk, D, page = shape
+    opt = OPTIONS[what]
+    mask = 70 if opt.get("keep") or what == "sinks" else Chunked(64) if what.startswith("cap") else None
+    attend(ops, (H, Hk, D, D, page, mask, [0, 37, 129, 300, 1500, 64], [1, 2, 1, 40, 1, 1]), dt, 100 + len(what), recorded, **opt)
+
+
+def test_refusals(ops):
+    from xyntetik_runner_amd.csrc.ops import FourBitPages, KernelError
+    kp, vp = (FourBitPages.zeros(4, 2, 16, 64, values, DEV) for values in (False, True))
+    ctx = step([3], [1], [[1]])
+    q = torch.zeros((1, 4 * 64), dtype=torch.bfloat16, device=DEV)
+    x = torch.zeros((1, 2 * 64), device=DEV)
+    bad = [lambda: ops.attention(q, kp, kp, ctx, 0, 4, 2, 64, 16, 1.0),
+           lambda: ops.attention(q, kp, torch.zeros((4, 2, 64, 16), dtype=torch.bfloat16, device=DEV), ctx, 0, 4, 2, 64, 16, 1.0),
+           lambda: ops.attention(q, kp, vp, ctx, 0, 4, 2, 64, 32, 1.0),
+           lambda: ops.attention(q[:, :128], kp, vp, ctx, 0, 4, 2, 64, 16, 1.0),
+           lambda: ops.attention(q.half(), kp, vp, ctx, 0, 4, 2, 64, 16, 1.0),
+           lambda: ops.attention(q, kp, vp, ctx, 0, 4, 2, 64, 16, 1.0, v_head_dim=32),
+           lambda: ops.attention(q, kp, vp, ctx, 0, 4, 2, 64, 16, 1.0, window=3, chunk=3),
+           lambda: ops.read_pages(kp, vp, Recorded(ctx), 0, torch.bfloat16),
+           lambda: ops.read_pages(kp, vp, ctx, 0, torch.float16),
+           lambda: ops.read_rows(kp, vp, ctx.positions.long(), ctx.req_of_token, ctx.block_table(0), torch.bfloat16),
+           lambda: ops.read_rows(kp, vp, ctx.positions, ctx.req_of_token[:0], ctx.block_table(0), torch.bfloat16),
+           lambda: ops.read_rows(kp, vp, ctx.positions, ctx.req_of_token, ctx.block_table(0)[0], torch.bfloat16),
+           lambda: ops.rope_kv_write(None, x, None, None, kp, vp, ctx.positions, ctx.req_of_token, ctx.block_table(0), None, 0, 2, 64, 0, False, 1.0, 16),
+           lambda: ops.rope_kv_write(None, x[:, :64], x, None, kp, vp, ctx.positions, ctx.req_of_token, ctx.block_table(0), None, 0, 2, 64, 0, False, 1.0, 16),
+           lambda: ops.rope_kv_write(None, x, x, None, kp, vp, ctx.positions, ctx.req_of_token, ctx.block_table(0), None, 0, 2, 64, 64, False, 1.0, 16),
+           lambda: ops.rope_kv_write(None, x, x, None, kp, vp, ctx.positions, ctx.req_of_token, ctx.block_table(0), torch.ones(31, device=DEV), 0, 2, 64, 63, False, 1.0, 16),
+           lambda: ops.rope_kv_write(None, x.bfloat16(), x, None, kp, vp, ctx.positions, ctx.req_of_token, ctx.block_table(0), None, 0, 2, 64, 0, False, 1.0, 16),
+           lambda: ops.rope_kv_write(q.float()[:, :256], x, x, q[:, :128], kp, vp, ctx.positions, ctx.req_of_token, ctx.block_table(0), None, 4, 2, 64, 0, False, 1.0, 16)]
+    for i, call in enumerate(bad):
+        with pytest.raises(KernelError):
+            call()
+            pytest.fail(f"call {i} was not refused")
+    # and the smallest calls that are allowed
+    none = torch.zeros((0,), dtype=torch.int32, device=DEV)
+    assert [t.shape for t in ops.read_rows(kp, vp, none, none, ctx.block_table(0), torch.bfloat16)] == [(0, 128), (0, 128)]
+    ops.rope_kv_write(None, x[:0], x[:0], None, kp, vp, none, none, ctx.block_table(0), None, 0, 2, 64, 0, False, 1.0, 16)
+    assert not kp.codes.any()

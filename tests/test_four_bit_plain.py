@@ -1,0 +1,108 @@
+"""The 4-bit format itself, on the CPU: what a block rounds to, the page layouts' refusals, and a step's list of pages."""
+import numpy as np
+import pytest
+import torch
+
+import four_bit as F
+
+
+def test_every_code_is_itself():
+    for byte in (8, 100, 127, 252):
+        codes = np.concatenate([np.arange(16), np.arange(16)]).astype(np.uint8)
+        x = F.numbers(codes[None], np.array([[byte]], dtype=np.uint8))
+        c, s, y = F.rounded(x)
+        assert s[0, 0] == byte and np.array_equal(y, x) and np.array_equal(c[0], codes)
+
+
+@pytest.mark.parametrize("top,e", [(4.0, 0), (6.0, 0), (7.0, 0), (7.0001, 1), (7.99, 1), (8.0, 1), (1.0, -2), (0.875, -3), (0.876, -2),
+                                   (1e-37, -119), (3.3e38, 125)])
+def test_scales(top, e):
+    assert F.scale_byte(np.array([0.1 * top, -top])) == e + 127
+
+
+def test_ties_and_the_largest():
+    #  halfway between neighbours: to the even code, that is 0, 1, 1 (not 1.5), 2, 2 (not 3), 4, 4 (not 6); over 6: 6
+    x = np.array([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 7.0, -0.25, -0.0])
+    c, s, y = F.rounded(x[None])
+    assert s[0, 0] == 127
+    assert y[0].tolist() == [0.0, 1.0, 1.0, 2.0, 2.0, 4.0, 4.0, 6.0, 0.0, 0.0] and c[0, 8] == 8
+
+
+def test_off_by_half_a_step_at_most():
+    rng = np.random.default_rng(3)
+    x = rng.normal(size=(400, 64)) * 10.0 ** rng.uniform(-6, 6, size=(400, 1))
+    _, s, y = F.rounded(x)
+    unit = np.repeat(2.0 ** (s.astype(float) - 127), 32, axis=1)
+    # steps of 2 from 4 on, 1 from 2 on, 0.5 below; what lies from 6 to 7 is cut
+    a = np.abs(x) / unit
+    step = np.where(a >= 4, 2.0, np.where(a >= 2, 1.0, 0.5))
+    assert (np.abs(x - y) <= step / 2 * unit * (1 + 1e-12)).all()
+    assert np.array_equal(F.fast_rounded(x)[2], y)
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+def test_a_block_with_no_numbers_reads_as_nan(bad):
+    x = np.ones((1, 64))
+    x[0, 40] = bad
+    _, s, y = F.rounded(x)
+    assert s[0].tolist() == [125, 255] and np.isnan(y[0, 32:]).all() and (y[0, :32] == 1).all()
+
+
+@pytest.mark.parametrize("dim,page,ok", [(64, 64, True), (8, 8, True), (256, 128, True), (80, 32, True), (12, 64, False), (264, 64, False), (64, 48, False), (64, 4, False)])
+def test_page_shapes(dim, page, ok):
+    from xyntetik_runner_amd.csrc.ops import FourBitPages, KernelError
+    if not ok:
+        with pytest.raises(KernelError):
+            FourBitPages.zeros(3, 2, page, dim, False, "cpu")
+        return
+    k, v = (FourBitPages.zeros(3, 2, page, dim, values, "cpu") for values in (False, True))
+    assert (k.values, v.values, k.page_size, v.page_size, k.heads, k.num_pages) == (False, True, page, page, 2, 3)
+    nb = -(-dim // 32)
+    assert k.nbytes == v.nbytes == 3 * 2 * page * (dim // 2 + nb)
+
+
+def test_refused_pages():
+    from xyntetik_runner_amd.csrc.ops import FourBitPages, KernelError, Ops
+    k, v = (FourBitPages.zeros(3, 2, 64, 64, values, "cpu") for values in (False, True))
+    with pytest.raises(KernelError, match="do not fit"):
+        FourBitPages(k.codes, k.scales, 96)
+    with pytest.raises(KernelError, match="uint8"):
+        FourBitPages(k.codes.to(torch.int8), k.scales, 64)
+    with pytest.raises(KernelError, match="contiguous"):
+        FourBitPages(torch.zeros((3, 2, 64, 64), dtype=torch.uint8)[..., ::2], k.scales, 64)
+    assert Ops._pages4("x", k, v, 2, 64, 64)[4] == 3
+    for pair, sizes in (((v, k), ()), ((k, k), ()), ((k, torch.zeros(3)), ()), ((k, FourBitPages.zeros(4, 2, 64, 64, True, "cpu")), ()),
+                        ((k, v), (4, 64, 64)), ((k, v), (2, 32, 64)), ((k, v), (2, 64, 32))):
+        with pytest.raises(KernelError):
+            Ops._pages4("x", *pair, *sizes)
+
+
+@pytest.mark.parametrize("mask,keep", [(None, 0), (40, 0), (40, 33), ("chunk", 0)])
+@pytest.mark.parametrize("requests", [None, (2, 0)])
+def test_page_list(mask, keep, requests, monkeypatch):
+    from xyntetik_runner_amd.cache.manager import RequestCache
+    from xyntetik_runner_amd.engine import batch
+    monkeypatch.setattr(torch.Tensor, "pin_memory", lambda self: self)      # (there is no GPU to pin for)
+    real = torch.empty
+    monkeypatch.setattr(torch, "empty", lambda *a, pin_memory=False, **k: real(*a, **k))
+    mask = batch.Chunked(64) if mask == "chunk" else mask
+    page, starts, lens = 16, [100, 0, 37], [9, 1, 30]
+    tables = [[7, 3, 9, 2, 11, 1, 4], [5], [6, 8, 10, 12, 13]]
+    held = [RequestCache(b, b, s, [t], False) for b, (s, t) in enumerate(zip(starts, tables))]
+    ctx = batch.StepContext(None, "cpu", [batch.StepEntry(b, [0] * n) for b, n in enumerate(lens)], held, 1)
+    ctx._held[0][0, 0] = -1 if mask and not keep else ctx._held[0][0, 0]      # (given back)
+    slots, table, n = ctx.page_list(0, page, requests, mask, keep)
+    slots, table = slots.view(n, 3).tolist(), table.tolist()
+    seen = set()
+    for b in range(3):
+        for i in range(len(table[0])):
+            positions = set(range(i * page, min((i + 1) * page, starts[b] + lens[b])))
+            wanted = set()
+            for p in range(starts[b], starts[b] + lens[b]):
+                wanted |= set(range(batch.first_key(mask, p), p + 1)) | (set(range(min(keep, p + 1))) if mask else set())
+            if (requests is None or b in requests) and positions & wanted:
+                assert slots[table[b][i]] == [b, i, len(positions)]
+                seen.add(table[b][i])
+            elif not positions or (requests is not None and b not in requests):
+                assert table[b][i] == -1
+    assert seen == set(range(n))

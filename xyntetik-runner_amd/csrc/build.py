@@ -37,12 +37,12 @@ UNITS: Dict[str, dict] = {
         "sources": ["errors.hip", "basic_kernels.hip", "gemm_ref.hip", "gemm_f32_parts.hip", "attention_ref.hip",
                     "sampling.hip", "gemm_mfma.hip", "sequence_kernels.hip", "recurrent_kernels.hip", "recurrent_chunks.hip", "recurrent_step.hip",
                     "attention_pooled.hip", "stream_kernels.hip", "latent_kernels.hip", "moe_kernels.hip", "grouped_mfma.hip", "mixer_kernels.hip",
-                    "ssd_kernels.hip"],
+                    "ssd_kernels.hip", "pages4_kernels.hip"],
         "defines": [],
     },
 }
 ATTN_SOURCES = ["errors.hip", "attention_mfma.hip"]
-HEADERS = ["common.h", "async_copy.h", "no_alloc.h"]
+HEADERS = ["common.h", "async_copy.h", "no_alloc.h", "pages4.h"]
 
 
 class BuildError(RuntimeError):

@@ -120,6 +120,10 @@ _PROTOS = {
     "xr_qkv_store": [_p, _p, _p, _p, _p, _p, _i, _p, _p, _p, _i, _i, _i, _i, _i, _i, _i, _i, _p],
     "xr_pool_blocks": [_p, _p, _p, _p, _p, _p, _p, _i, _p, _i, _i, _i, _i, _i, _i, _i, _i, _i, _p],
     "xr_attention_pool_partial": [_p, _p, _p, _p, _p, _p, _i, _p, _i, _i, _i, _i, _i, _i, _f, _i, _i, _i, _p],
+    "xr_rope_kv_write4": [_p, _p, _p, _i, _p] + [_p] * 4 + [_i] + [_p] * 3 + [_i, _p] + [_i] * 7 + [_f, _i, _i, _i, _p],
+    "xr_read_rows4": [_p, _p] + [_p] * 4 + [_i] + [_p] * 3 + [_i] * 7 + [_p],
+    "xr_read_pages4": [_p, _p] + [_p] * 4 + [_i, _p, _i, _p] + [_i] * 6 + [_p],
+    "xr_attention_any4": [_p, _p] + [_p] * 4 + [_i] + [_p] * 3 + [_i] * 7 + [_f] + [_i] * 4 + [_p, _p, _f, _p, _i, _f, _i, _p],
     "xr_attention_pooled": [_p, _p, _p, _p, _p, _p, _p, _p, _p, _i, _p, _i, _i, _i, _i, _i, _i, _i, _f, _i, _i, _i, _p],
 }
 
@@ -165,6 +169,60 @@ class PackedWeight:
     @property
     def device(self):
         return self.data.device
+
+
+class FourBitPages:
+    """The pages of a layer's keys, or of its values, held in 4 bits: in place of a cache tensor for ``Ops.rope_kv_write``, which
+    rounds what it writes, ``Ops.attention``, ``Ops.read_rows`` and ``Ops.read_pages``.
+
+    Every 32 channels of a head at one position are a block with one scale, a power of two; a number is one of 0, 0.5, 1, 1.5, 2, 3, 4
+    or 6 with a sign, times the scale: 4.25 bits a number.  The scale is the largest under which no magnitude of the block is over 7
+    (up to 7 rounds to 6), within 2^-119 .. 2^125; ties go to the even code.  A block with a NaN or an infinity reads back as NaN.
+
+    ``codes``: keys ``[pages, heads, page_size, dim / 2]``, values ``[pages, heads, page_size / 8, dim / 2, 8]`` (the bytes of 8 positions
+    side by side), ``scales [pages, heads, page_size / 8, ceil(dim / 32), 8]``, uint8.  Heads of 8 to 256 channels in steps of 8,
+    pages of a power of two of at least 8 positions."""
+
+    BLOCK = 32
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, dim: int):
+        self.codes, self.scales, self.dim = codes, scales, int(dim)
+        self.values = codes.dim() == 5
+        self.num_pages, self.heads = int(codes.shape[0]), int(codes.shape[1])
+        self.page_size = int(codes.shape[2]) * (8 if self.values else 1)
+        if self.shapes(self.num_pages, self.heads, self.page_size, self.dim, self.values) != (tuple(codes.shape), tuple(scales.shape)):
+            raise KernelError(f"4-bit pages of {self.dim} channels: codes {tuple(codes.shape)} and scales {tuple(scales.shape)} do not fit")
+        if codes.dtype != torch.uint8 or scales.dtype != torch.uint8 or codes.device != scales.device:
+            raise KernelError("4-bit pages: codes and scales must be uint8 on one device")
+        if not codes.is_contiguous() or not scales.is_contiguous() or codes.data_ptr() % 16 or scales.data_ptr() % 8:
+            raise KernelError("4-bit pages: codes and scales must be contiguous, 16 and 8 bytes aligned")
+
+    @staticmethod
+    def shapes(pages: int, heads: int, page_size: int, dim: int, values: bool):
+        """The shapes of ``codes`` and ``scales``."""
+        if not (8 <= dim <= 256 and dim % 8 == 0):
+            raise KernelError(f"4-bit pages hold heads of 8 to 256 channels in steps of 8, not {dim}")
+        if page_size < 8 or page_size & (page_size - 1):
+            raise KernelError(f"4-bit pages have a power of two of at least 8 positions, not {page_size}")
+        codes = (pages, heads, page_size // 8, dim // 2, 8) if values else (pages, heads, page_size, dim // 2)
+        return codes, (pages, heads, page_size // 8, -(-dim // FourBitPages.BLOCK), 8)
+
+    @classmethod
+    def zeros(cls, pages: int, heads: int, page_size: int, dim: int, values: bool, device) -> "FourBitPages":
+        codes, scales = cls.shapes(pages, heads, page_size, dim, values)
+        return cls(torch.zeros(codes, dtype=torch.uint8, device=device), torch.zeros(scales, dtype=torch.uint8, device=device), dim)
+
+    @property
+    def device(self):
+        return self.codes.device
+
+    @property
+    def is_cuda(self):
+        return self.codes.is_cuda
+
+    @property
+    def nbytes(self) -> int:
+        return self.codes.numel() + self.scales.numel()
 
 
 class F32Weight(torch.Tensor):
@@ -712,9 +770,13 @@ class Ops:
         """Rotate queries (into ``q_out``) and keys, and write keys and values to their pages.
 
         ``q_in``/``k_in``/``v_in`` are 32-bit views with one common row stride.  ``paired``: the
-        channels of every query and key head come in ``paired_order``.
+        channels of every query and key head come in ``paired_order``.  Caches that are ``FourBitPages`` take their
+        blocks' codes and scales (values may have another size than keys there: as the cache says).
         """
         self._dev(q_in, k_in, v_in, q_out, k_cache, v_cache, positions, req_of_token, block_table, inv_freq)
+        if isinstance(k_cache, FourBitPages) or isinstance(v_cache, FourBitPages):
+            return self._rope_kv_write4(q_in, k_in, v_in, q_out, k_cache, v_cache, positions, req_of_token, block_table, inv_freq, H, Hk, D, rot,
+                                        interleaved, mscale, page_size, paired)
         T = positions.numel()
         ins = [t for t in (q_in, k_in, v_in) if t is not None]
         if any(t.dtype != torch.float32 or t.stride(-1) != 1 for t in ins):
@@ -732,6 +794,98 @@ class Ops:
             block_table.stride(0) if block_table is not None else 0, _ptr(inv_freq), T, H, Hk, D, rot,
             1 if interleaved else 0, float(mscale), page_size, dtype_code(store.dtype), 1 if paired else 0,
             _stream()))
+
+    @staticmethod
+    def _pages4(what: str, k_pages, v_pages, Hk: Optional[int] = None, D: Optional[int] = None, page_size: Optional[int] = None):
+        """The operands of a pair of 4-bit caches for the library."""
+        if not (isinstance(k_pages, FourBitPages) and isinstance(v_pages, FourBitPages)) or k_pages.values or not v_pages.values:
+            raise KernelError(f"{what}: keys and values must both be in 4-bit pages, keys in a key's and values in a value's")
+        if (k_pages.num_pages, k_pages.heads, k_pages.page_size) != (v_pages.num_pages, v_pages.heads, v_pages.page_size) or k_pages.device != v_pages.device:
+            raise KernelError(f"{what}: keys and values differ in pages, heads or device")
+        if ((Hk is not None and Hk != k_pages.heads) or (D is not None and D != k_pages.dim)
+                or (page_size is not None and page_size != k_pages.page_size)):
+            raise KernelError(f"{what}: 4-bit pages of {k_pages.heads} heads of {k_pages.dim} channels in pages of {k_pages.page_size} do not fit "
+                              f"{Hk} heads of {D} in pages of {page_size}")
+        return (k_pages.codes.data_ptr(), k_pages.scales.data_ptr(), v_pages.codes.data_ptr(), v_pages.scales.data_ptr(), k_pages.num_pages)
+
+    @staticmethod
+    def _ints(what: str, n: Optional[int], *ts: torch.Tensor) -> None:
+        for t in ts:
+            if t.dtype != torch.int32 or t.dim() != 1 or (t.numel() > 1 and t.stride(0) != 1) or (n is not None and t.numel() != n):
+                raise KernelError(f"{what}: positions and requests must be int32, contiguous and of one length")
+
+    @staticmethod
+    def _table(what: str, table: torch.Tensor) -> None:
+        if table is None or table.dtype != torch.int32 or table.dim() != 2 or table.shape[1] < 1 or table.stride(1) != 1:
+            raise KernelError(f"{what}: the block table must be int32 [requests, pages] with unit column stride")
+
+    def _rope_kv_write4(self, q_in, k_in, v_in, q_out, k_pages, v_pages, positions, req_of_token, block_table, inv_freq, H: int, Hk: int,
+                        D: int, rot: int, interleaved: bool, mscale: float, page_size: int, paired: bool) -> None:
+        pages = self._pages4("rope_kv_write", k_pages, v_pages, Hk, D, page_size)
+        T, Dv = positions.numel(), v_pages.dim
+        if k_in is None or v_in is None or req_of_token is None or (q_in is None) != (q_out is None):
+            raise KernelError("rope_kv_write: 4-bit pages take keys and values (queries come with the place they go to)")
+        self._ints("rope_kv_write", T, positions, req_of_token)
+        self._table("rope_kv_write", block_table)
+        H = H if q_in is not None else 0
+        for t, width in ((q_in, H * D), (k_in, Hk * D), (v_in, Hk * Dv)):
+            if t is not None and (t.dtype != torch.float32 or tuple(t.shape) != (T, width) or (width > 1 and t.stride(1) != 1)):
+                raise KernelError(f"rope_kv_write: inputs must be float32 [{T}, heads x channels] with unit column stride")
+        if T > 1 and len({t.stride(0) for t in (q_in, k_in, v_in) if t is not None}) > 1:
+            raise KernelError("rope_kv_write: q, k and v inputs must share a row stride")
+        if q_out is not None and (tuple(q_out.shape) != (T, H * D) or not q_out.is_contiguous() or q_out.data_ptr() % 16):
+            raise KernelError(f"rope_kv_write: the queries' place must be contiguous [{T}, {H * D}] and 16-byte aligned")
+        if rot and (inv_freq is None or inv_freq.dtype != torch.float32 or inv_freq.numel() != rot // 2 or not inv_freq.is_contiguous()):
+            raise KernelError(f"rope_kv_write: {rot // 2} 32-bit frequencies are needed")
+        self.lib.check(self.lib.xr_rope_kv_write4(
+            _ptr(q_in), k_in.data_ptr(), v_in.data_ptr(), k_in.stride(0), _ptr(q_out), *pages, positions.data_ptr(), req_of_token.data_ptr(),
+            block_table.data_ptr(), block_table.stride(0), _ptr(inv_freq) if rot else None, T, H, Hk, D, Dv, rot, 1 if interleaved else 0,
+            float(mscale), page_size, dtype_code(q_out.dtype) if q_out is not None else XR_F32, 1 if paired else 0, _stream()))
+
+    def read_rows(self, k_pages: "FourBitPages", v_pages: "FourBitPages", positions: torch.Tensor, req_of_row: torch.Tensor,
+                  block_table: torch.Tensor, dtype: torch.dtype):
+        """Cached keys ``[n, heads * dim]`` and values of any list of (request, position), as ``dtype`` numbers; a row whose position
+        has no page in ``block_table`` reads as zeros."""
+        pages = self._pages4("read_rows", k_pages, v_pages)
+        self._dev(k_pages, positions, req_of_row, block_table)
+        n = positions.numel()
+        self._ints("read_rows", n, positions, req_of_row)
+        self._table("read_rows", block_table)
+        Hk, D, Dv = k_pages.heads, k_pages.dim, v_pages.dim
+        k = torch.empty((n, Hk * D), dtype=dtype, device=k_pages.device)
+        v = torch.empty((n, Hk * Dv), dtype=dtype, device=k_pages.device)
+        self.lib.check(self.lib.xr_read_rows4(k.data_ptr(), v.data_ptr(), *pages, positions.data_ptr(), req_of_row.data_ptr(),
+                                              block_table.data_ptr(), block_table.stride(0), n, Hk, D, Dv, k_pages.page_size, dtype_code(dtype),
+                                              _stream()))
+        return k, v
+
+    def read_pages(self, k_pages: "FourBitPages", v_pages: "FourBitPages", ctx, group: int, dtype: torch.dtype, requests=None, window: Optional[int] = None,
+                   chunk: Optional[int] = None, keep_first: int = 0):
+        """The step's cached keys and values as pages of ``dtype`` in the layout of 16- and 32-bit caches, numbered from 0 in the requests'
+        order, and the block table that names them: ``(k [n, heads, page_size, dim], v [n, heads, dim, page_size], table)``.  Positions behind a request's end
+        are zeros.  ``requests``: the places in the step of those that are read (None: all); with a ``window`` or ``chunk`` the
+        pages that none of the step's rows reads are left out (``keep_first``: except those of the first so many positions), as are
+        pages that were given back: -1 in the table.  A step that is being recorded has no lengths to go by and is refused."""
+        pages = self._pages4("read_pages", k_pages, v_pages)
+        if not getattr(ctx, "knows_lengths", False):
+            raise KernelError("read_pages: the lengths of a recorded step's requests change from replay to replay")
+        if window and chunk:
+            raise KernelError("read_pages: a layer reads a window or its chunk, not both")
+        block_table = ctx.block_table(group)
+        self._dev(k_pages, block_table)
+        self._table("read_pages", block_table)
+        Hk, D, Dv, P = k_pages.heads, k_pages.dim, v_pages.dim, k_pages.page_size
+        mask = Chunked(int(chunk)) if chunk else window
+        key = ("read_pages", group, P, None if requests is None else tuple(requests), mask, keep_first if mask else 0)
+        made = ctx.shared.get(key)
+        if made is None:
+            made = ctx.shared[key] = ctx.page_list(group, P, requests, mask, keep_first)
+        slots, table, n = made
+        k = torch.empty((n, Hk, P, D), dtype=dtype, device=k_pages.device)
+        v = torch.empty((n, Hk, Dv, P), dtype=dtype, device=k_pages.device)
+        self.lib.check(self.lib.xr_read_pages4(k.data_ptr(), v.data_ptr(), *pages, slots.data_ptr(), n, block_table.data_ptr(),
+                                               block_table.stride(0), Hk, D, Dv, P, dtype_code(dtype), _stream()))
+        return k, v, table
 
     def row_norm_rope_write(self, q_in, k_in, v_in, w_q, w_k, eps: float, k_cache, v_cache, ctx, group: int, inv_freq, H: int,
                             Hk: int, D: int, rot: int, interleaved: bool, mscale: float, page_size: int, out_dtype) -> torch.Tensor:
@@ -887,12 +1041,20 @@ class Ops:
 
         bfloat16 runs on the matrix cores (head and value sizes in steps of 16 up to 256, pages of at least
         16 positions, a cap or slopes; kept first keys only where values have the keys' size); float32, and what the MFMA kernel does not take, runs the 32-bit kernel.
+        Caches that are ``FourBitPages`` are read back first (``read_pages``), but for steps that are being recorded, which a
+        32-bit kernel serves from the codes themselves.
         """
         positions, req_of_token, block_table = ctx.positions, ctx.req_of_token, ctx.block_table(group)
         self._dev(q, k_cache, v_cache, positions, req_of_token, block_table)
         T = positions.numel()
         self._contig(q, "attention queries")
-        if q.dtype != k_cache.dtype or q.dtype != v_cache.dtype:
+        four = isinstance(k_cache, FourBitPages) or isinstance(v_cache, FourBitPages)
+        if four:
+            pages = self._pages4("attention", k_cache, v_cache, Hk, D, page_size)
+            if tuple(q.shape) != (T, H * D) or v_cache.dim != (int(v_head_dim) if v_head_dim is not None else D):
+                raise KernelError(f"attention: queries {tuple(q.shape)} or values of {v_cache.dim} do not fit {T} rows of {H} heads of {D}")
+            dtype_code(q.dtype)
+        elif q.dtype != k_cache.dtype or q.dtype != v_cache.dtype:
             raise KernelError("attention: queries and cache differ in dtype")
         if H % Hk:
             raise KernelError(f"attention: {H} query heads are not a multiple of {Hk} key/value heads")
@@ -912,6 +1074,14 @@ class Ops:
                     raise KernelError(f"attention: the {name} must be float32 [{H}]")
         if chunk and window:
             raise KernelError("attention: a layer reads a window or its chunk, not both")
+        if four:
+            if not getattr(ctx, "knows_lengths", False):
+                self.lib.check(self.lib.xr_attention_any4(
+                    out.data_ptr(), q.data_ptr(), *pages, positions.data_ptr(), req_of_token.data_ptr(), block_table.data_ptr(), block_table.stride(0),
+                    T, H, Hk, D, Dv, page_size, float(scale), int(window or 0), int(chunk or 0), int(keep_first), dtype_code(q.dtype), _ptr(slopes),
+                    _ptr(sinks), float(softcap), *gating, _stream()))
+                return out
+            k_cache, v_cache, block_table = self.read_pages(k_cache, v_cache, ctx, group, q.dtype, window=window, chunk=chunk, keep_first=keep_first)
         if (self.attention_on_matrix_cores(q.dtype, D, Dv, page_size) and not (softcap and slopes is not None)
                 and (D == Dv or not keep_first) and out.stride(0) % 4 == 0 and out.data_ptr() % 8 == 0):
             # The first keys that a window has passed enter the same softmax as a partial result of its own, which

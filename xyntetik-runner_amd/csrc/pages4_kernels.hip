@@ -1,0 +1,408 @@
+// Cache pages held in 4 bits (pages4.h has the format): rotating and writing a step's keys and values, reading rows and whole pages
+// back, and attention over them for any head size in plain 32-bit arithmetic.
+#include "pages4.h"
+
+// ---------------------------------------------------------------- rotary + cache write
+// Rotation as in k_rope_kv_write, of the angle pos * inv_freq itself: it is reduced to turns in 64 bits, so that far positions
+// lose nothing (a 32-bit product is off by 0.004 at 131,071).
+//
+// A thread takes 8 channels of a head of queries, keys or values; 4 neighbouring lanes are a block of 32 and share its largest
+// magnitude in two exchanges.  (A head's last block may be short: its missing lanes hold zeros.)
+struct Write4Args {
+    const float* q_in;      // [T, in_stride] 32-bit
+    const float* k_in;
+    const float* v_in;
+    int in_stride;
+    void* q_out;            // [T, H * D]
+    Pages4 pages;
+    const int* positions;   // [T]
+    const int* req_of_token;
+    const int* block_table; // [B, table_stride]
+    int table_stride, n_pages;
+    const float* inv_freq;  // [rot / 2] or null
+    int H, Hk, D, Dv, rot, interleaved, paired;
+    float mscale;
+    int page_shift, page_mask, page_size;
+    int q_units, k_units, units, per_block;     // of a token: queries' end, keys' end, all; and those of a workgroup
+    int lanes_k, lanes_v;                       // threads of a head of queries or keys, and of values (a multiple of 4)
+};
+
+template <typename T> __device__ inline void store_row8(T* dst, const float* v);
+template <> __device__ inline void store_row8<float>(float* dst, const float* v) {
+    *reinterpret_cast<float4*>(dst) = make_float4(v[0], v[1], v[2], v[3]);
+    *reinterpret_cast<float4*>(dst + 4) = make_float4(v[4], v[5], v[6], v[7]);
+}
+template <> __device__ inline void store_row8<bf16_t>(bf16_t* dst, const float* v) {
+    *reinterpret_cast<uint4*>(dst) = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void k_rope_kv_write4(Write4Args a) {
+    __shared__ float2 cs[128];
+    const int t = blockIdx.x, pos = a.positions[t];
+    const int half = a.rot >> 1;
+    const int u0 = blockIdx.y * a.per_block, u1 = min(a.units, u0 + a.per_block);
+    for (int j = threadIdx.x; j < half; j += 256) {
+        double turns = (double)pos * (double)a.inv_freq[j] * 0.15915494309189533577;
+        turns -= rint(turns);
+        float s, c;
+        sincospif((float)(2.0 * turns), &s, &c);
+        cs[j] = make_float2(c * a.mscale, s * a.mscale);
+    }
+    __syncthreads();
+    const int bi = pos >> a.page_shift, off = pos & a.page_mask;
+    const int page = a.Hk > 0 && bi >= 0 && bi < a.table_stride ? a.block_table[(size_t)a.req_of_token[t] * a.table_stride + bi] : -1;
+    for (int u = u0 + (int)threadIdx.x; u < u1; u += 256) {
+        const bool is_q = u < a.q_units, is_v = u >= a.k_units;
+        const int w = is_q ? u : is_v ? u - a.k_units : u - a.q_units;
+        const int lanes = is_v ? a.lanes_v : a.lanes_k, D = is_v ? a.Dv : a.D;
+        const int h = w / lanes, c0 = (w - h * lanes) * 8;
+        const float* src = (is_q ? a.q_in : is_v ? a.v_in : a.k_in) + (size_t)t * a.in_stride + (size_t)h * D;
+        float x[8];
+        if (c0 >= D) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = 0.f;
+        } else if (is_v || c0 >= a.rot) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = src[c0 + i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int c = c0 + i;
+                if (c >= a.rot) {
+                    x[i] = src[c];
+                } else {
+                    const int j = a.interleaved ? c >> 1 : c < half ? c : c - half;
+                    const bool second = a.interleaved ? (c & 1) : c >= half;
+                    int i0 = a.interleaved ? 2 * j : j, i1 = a.interleaved ? 2 * j + 1 : j + half;
+                    if (a.paired) { i0 = paired_col(i0, a.rot); i1 = paired_col(i1, a.rot); }
+                    const float x0 = src[i0], x1 = src[i1];
+                    const float2 r = cs[j];
+                    x[i] = second ? x0 * r.y + x1 * r.x : x0 * r.x - x1 * r.y;
+                }
+            }
+        }
+        if (is_q) {
+            if (c0 < D) store_row8<T>((T*)a.q_out + ((size_t)t * a.H + h) * D + c0, x);
+            continue;
+        }
+        uint32_t most = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) most = max(most, __float_as_uint(x[i]) & 0x7FFFFFFFu);
+        most = max(most, (uint32_t)__shfl_xor((int)most, 1, 64));
+        most = max(most, (uint32_t)__shfl_xor((int)most, 2, 64));
+        if (c0 >= D || (unsigned)page >= (unsigned)a.n_pages) continue;
+        const uint32_t byte = scale_byte4(most), codes = codes4(x, byte);
+        const size_t pb = (size_t)page * a.Hk + h;
+        uint8_t* scales = is_v ? a.pages.vs : a.pages.ks;
+        if ((c0 & 31) == 0) scales[scale_at4(pb, a.page_size, blocks4(D), off, c0 >> 5)] = (uint8_t)byte;
+        if (is_v) {
+            uint8_t* dst = a.pages.vc + value_at4(pb, a.page_size, D, off, c0 >> 1);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) dst[8 * i] = (uint8_t)(codes >> (8 * i));
+        } else {
+            *reinterpret_cast<uint32_t*>(a.pages.kc + key_at4(pb, a.page_size, D, off) + (c0 >> 1)) = codes;
+        }
+    }
+}
+
+static int check_pages4(const char* what, const Pages4& p, int Hk, int D, int Dv, int page_size, int n_pages) {
+    XR_REQUIRE(Hk > 0 && D > 0 && Dv > 0 && D <= 256 && Dv <= 256 && D % 8 == 0 && Dv % 8 == 0,
+               "%s: 4-bit pages hold heads of 8 to 256 channels in steps of 8, not %d keys and values of %d and %d", what, Hk, D, Dv);
+    XR_REQUIRE(ilog2_exact(page_size) >= 3, "%s: 4-bit pages have a power of two of at least 8 positions, not %d", what, page_size);
+    XR_REQUIRE(p.kc && p.ks && p.vc && p.vs && n_pages > 0, "%s: 4-bit pages with a null operand", what);
+    XR_REQUIRE((((uintptr_t)p.kc | (uintptr_t)p.vc) & 15) == 0 && (((uintptr_t)p.ks | (uintptr_t)p.vs) & 7) == 0,
+               "%s: 4-bit pages must be 16-byte aligned, their scales 8-byte", what);
+    return XR_OK;
+}
+
+extern "C" int xr_rope_kv_write4(const float* q_in, const float* k_in, const float* v_in, int in_stride, void* q_out,
+                                 void* kc, void* ks, void* vc, void* vs, int n_pages, const int* positions, const int* req_of_token,
+                                 const int* block_table, int table_stride, const float* inv_freq, int T, int H, int Hk, int D, int Dv,
+                                 int rot, int interleaved, float mscale, int page_size, int q_dtype, int paired, hipStream_t stream) {
+    Write4Args a;
+    a.pages = Pages4{(uint8_t*)kc, (uint8_t*)ks, (uint8_t*)vc, (uint8_t*)vs};
+    const int rc = check_pages4("rope_kv_write", a.pages, Hk, D, Dv, page_size, n_pages);
+    if (rc != XR_OK) return rc;
+    XR_REQUIRE(T >= 0 && H >= 0 && table_stride > 0, "rope_kv_write: bad sizes T=%d H=%d, block tables of %d pages", T, H, table_stride);
+    XR_REQUIRE(rot >= 0 && rot <= D && rot % 2 == 0, "rope_kv_write: rotary width %d must be even and at most head_dim %d", rot, D);
+    XR_REQUIRE(rot == 0 || inv_freq, "rope_kv_write: rotary width %d without a frequency table", rot);
+    XR_REQUIRE(q_dtype == XR_F32 || q_dtype == XR_BF16, "rope_kv_write: bad dtype %d", q_dtype);
+    XR_REQUIRE(!paired || (!interleaved && rot % 16 == 0), "rope_kv_write: paired order needs pairs (j, j + width/2) and a rotary width (%d) that is a multiple of 16", rot);
+    if (T == 0) return XR_OK;
+    XR_REQUIRE(k_in && v_in && block_table && req_of_token && positions, "rope_kv_write: keys and values to cache but a null operand");
+    XR_REQUIRE(H == 0 || (q_in && q_out && ((uintptr_t)q_out & 15) == 0), "rope_kv_write: queries but a null operand, or rows that are not 16-byte aligned");
+    a.q_in = q_in; a.k_in = k_in; a.v_in = v_in; a.in_stride = in_stride; a.q_out = q_out;
+    a.positions = positions; a.req_of_token = req_of_token; a.block_table = block_table; a.table_stride = table_stride; a.n_pages = n_pages;
+    a.inv_freq = inv_freq; a.H = H; a.Hk = Hk; a.D = D; a.Dv = Dv; a.rot = rot; a.interleaved = interleaved; a.paired = paired ? 1 : 0;
+    a.mscale = mscale; a.page_shift = ilog2_exact(page_size); a.page_mask = page_size - 1; a.page_size = page_size;
+    a.lanes_k = blocks4(D) * 4; a.lanes_v = blocks4(Dv) * 4;
+    a.q_units = H * a.lanes_k; a.k_units = a.q_units + Hk * a.lanes_k; a.units = a.k_units + Hk * a.lanes_v;
+    // a token a workgroup where there are tokens enough for the chip, else a round of threads each
+    int groups = (1024 + T - 1) / T;
+    const int most = (a.units + 255) / 256;
+    groups = groups < 1 ? 1 : groups > most ? most : groups;
+    a.per_block = ((a.units + groups - 1) / groups + 255) / 256 * 256;
+    const dim3 grid(T, (a.units + a.per_block - 1) / a.per_block);
+    if (q_dtype == XR_F32) k_rope_kv_write4<float><<<grid, 256, 0, stream>>>(a);
+    else k_rope_kv_write4<bf16_t><<<grid, 256, 0, stream>>>(a);
+    XR_CHECK_LAUNCH("rope_kv_write4");
+    return XR_OK;
+}
+
+// ---------------------------------------------------------------- reading back
+// 8 channels of one position, the lowest of them c0 (a multiple of 8)
+__device__ inline void key_row8(const Pages4& p, size_t pb, int page_size, int D, int off, int c0, float* x) {
+    const uint32_t w = *reinterpret_cast<const uint32_t*>(p.kc + key_at4(pb, page_size, D, off) + (c0 >> 1));
+    const uint32_t s = (uint32_t)p.ks[scale_at4(pb, page_size, blocks4(D), off, c0 >> 5)] << 23;
+    const float2 v[4] = {pair4_f32<0>(w, s), pair4_f32<1>(w, s), pair4_f32<2>(w, s), pair4_f32<3>(w, s)};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { x[2 * i] = v[i].x; x[2 * i + 1] = v[i].y; }
+}
+__device__ inline void value_row8(const Pages4& p, size_t pb, int page_size, int Dv, int off, int c0, float* x) {
+    const uint32_t s = (uint32_t)p.vs[scale_at4(pb, page_size, blocks4(Dv), off, c0 >> 5)] << 23;
+    const uint8_t* src = p.vc + value_at4(pb, page_size, Dv, off, c0 >> 1);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 v = pair4_f32<0>((uint32_t)src[8 * i], s);
+        x[2 * i] = v.x; x[2 * i + 1] = v.y;
+    }
+}
+
+struct Read4Args {
+    Pages4 pages;
+    const int* positions;       // rows: [n]
+    const int* req_of_row;
+    const int* block_table;
+    const int* slots;           // pages: [n, 3] request, place in its table, positions of the page that are the request's
+    void* k_out;                // rows: [n, Hk * D]; pages: [n, Hk, page_size, D]
+    void* v_out;                // rows: [n, Hk * Dv]; pages: [n, Hk, Dv, page_size]
+    int table_stride, n_pages, Hk, D, Dv, page_shift, page_size;
+    size_t total;               // threads of all rows, keys' first
+    size_t k_total;
+};
+
+// Rows of a list of (request, position): a thread 8 channels of a head.  Rows without a page read as zeros.
+template <typename T>
+__global__ __launch_bounds__(256) void k_read_rows4(Read4Args a) {
+    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < a.total; i += (size_t)gridDim.x * 256) {
+        const bool is_v = i >= a.k_total;
+        const int D = is_v ? a.Dv : a.D, per = a.Hk * (D >> 3);
+        const size_t j = is_v ? i - a.k_total : i;
+        const size_t r = j / per;
+        const int w = (int)(j - r * per), h = w / (D >> 3), c0 = (w - h * (D >> 3)) * 8;
+        const int pos = a.positions[r], bi = pos >> a.page_shift, off = pos & (a.page_size - 1);
+        const int page = bi >= 0 && bi < a.table_stride ? a.block_table[(size_t)a.req_of_row[r] * a.table_stride + bi] : -1;
+        float x[8];
+        if ((unsigned)page >= (unsigned)a.n_pages) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = 0.f;
+        } else {
+            const size_t pb = (size_t)page * a.Hk + h;
+            if (is_v) value_row8(a.pages, pb, a.page_size, D, off, c0, x);
+            else key_row8(a.pages, pb, a.page_size, D, off, c0, x);
+        }
+        store_row8<T>((T*)(is_v ? a.v_out : a.k_out) + (r * a.Hk + h) * D + c0, x);
+    }
+}
+
+// Whole pages in the layout of 16- and 32-bit caches (values transposed), a workgroup a page and head.  What lies behind a request's
+// end becomes zero, so that readers may multiply it.
+template <typename T>
+__global__ __launch_bounds__(256) void k_read_pages4(Read4Args a) {
+    const int n = blockIdx.x / a.Hk, h = blockIdx.x - n * a.Hk;
+    const int req = a.slots[3 * n], bi = a.slots[3 * n + 1], held = a.slots[3 * n + 2];
+    const int page = a.block_table[(size_t)req * a.table_stride + bi];
+    const bool there = (unsigned)page < (unsigned)a.n_pages;
+    const size_t pb = (size_t)(there ? page : 0) * a.Hk + h, to = (size_t)n * a.Hk + h;
+    const int P = a.page_size, oct = a.D >> 3;
+    for (int i = threadIdx.x; i < P * oct; i += 256) {
+        const int off = i / oct, c0 = (i - off * oct) * 8;
+        float x[8];
+        key_row8(a.pages, pb, P, a.D, off, c0, x);
+        if (!there || off >= held)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = 0.f;
+        store_row8<T>((T*)a.k_out + (to * P + off) * a.D + c0, x);
+    }
+    // values: a thread 8 positions of two channels
+    const int octs = P >> 3;
+    for (int i = threadIdx.x; i < octs * (a.Dv >> 1); i += 256) {
+        const int pair = i / octs, o8 = i - pair * octs;
+        const uint2 w = *reinterpret_cast<const uint2*>(a.pages.vc + value_at4(pb, P, a.Dv, o8 * 8, pair));
+        const uint2 s = *reinterpret_cast<const uint2*>(a.pages.vs + scale_at4(pb, P, blocks4(a.Dv), o8 * 8, pair >> 4));
+        const float2 v[8] = {pair4_f32<0>(w.x, s.x << 23), pair4_f32<1>(w.x, s.x << 15), pair4_f32<2>(w.x, s.x << 7), pair4_f32<3>(w.x, s.x >> 1),
+                             pair4_f32<0>(w.y, s.y << 23), pair4_f32<1>(w.y, s.y << 15), pair4_f32<2>(w.y, s.y << 7), pair4_f32<3>(w.y, s.y >> 1)};
+        float x[8], y[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const bool ok = there && o8 * 8 + e < held;
+            x[e] = ok ? v[e].x : 0.f;
+            y[e] = ok ? v[e].y : 0.f;
+        }
+        T* dst = (T*)a.v_out + (to * a.Dv + 2 * pair) * P + o8 * 8;
+        store_row8<T>(dst, x);
+        store_row8<T>(dst + P, y);
+    }
+}
+
+extern "C" int xr_read_rows4(void* k_out, void* v_out, void* kc, void* ks, void* vc, void* vs, int n_pages, const int* positions,
+                             const int* req_of_row, const int* block_table, int table_stride, int n, int Hk, int D, int Dv,
+                             int page_size, int dtype, hipStream_t stream) {
+    Read4Args a;
+    a.pages = Pages4{(uint8_t*)kc, (uint8_t*)ks, (uint8_t*)vc, (uint8_t*)vs};
+    const int rc = check_pages4("read_rows", a.pages, Hk, D, Dv, page_size, n_pages);
+    if (rc != XR_OK) return rc;
+    XR_REQUIRE(n >= 0 && table_stride > 0 && (dtype == XR_F32 || dtype == XR_BF16), "read_rows: bad sizes n=%d table=%d or dtype %d", n, table_stride, dtype);
+    if (n == 0) return XR_OK;
+    XR_REQUIRE(k_out && v_out && positions && req_of_row && block_table, "read_rows: a null operand");
+    XR_REQUIRE((((uintptr_t)k_out | (uintptr_t)v_out) & 15) == 0, "read_rows: outputs must be 16-byte aligned");
+    a.positions = positions; a.req_of_row = req_of_row; a.block_table = block_table; a.slots = nullptr;
+    a.k_out = k_out; a.v_out = v_out; a.table_stride = table_stride; a.n_pages = n_pages; a.Hk = Hk; a.D = D; a.Dv = Dv;
+    a.page_shift = ilog2_exact(page_size); a.page_size = page_size;
+    a.k_total = (size_t)n * Hk * (D >> 3);
+    a.total = a.k_total + (size_t)n * Hk * (Dv >> 3);
+    const size_t blocks = (a.total + 255) / 256;
+    const unsigned grid = (unsigned)(blocks < 65536 ? blocks : 65536);
+    if (dtype == XR_F32) k_read_rows4<float><<<grid, 256, 0, stream>>>(a);
+    else k_read_rows4<bf16_t><<<grid, 256, 0, stream>>>(a);
+    XR_CHECK_LAUNCH("read_rows4");
+    return XR_OK;
+}
+
+extern "C" int xr_read_pages4(void* k_out, void* v_out, void* kc, void* ks, void* vc, void* vs, int n_pages, const int* slots, int n,
+                              const int* block_table, int table_stride, int Hk, int D, int Dv, int page_size, int dtype, hipStream_t stream) {
+    Read4Args a;
+    a.pages = Pages4{(uint8_t*)kc, (uint8_t*)ks, (uint8_t*)vc, (uint8_t*)vs};
+    const int rc = check_pages4("read_pages", a.pages, Hk, D, Dv, page_size, n_pages);
+    if (rc != XR_OK) return rc;
+    XR_REQUIRE(n >= 0 && table_stride > 0 && (dtype == XR_F32 || dtype == XR_BF16), "read_pages: bad sizes n=%d table=%d or dtype %d", n, table_stride, dtype);
+    if (n == 0) return XR_OK;
+    XR_REQUIRE((long long)n * Hk < (1LL << 31), "read_pages: %d pages of %d heads are more workgroups than a launch takes", n, Hk);
+    XR_REQUIRE(k_out && v_out && slots && block_table, "read_pages: a null operand");
+    XR_REQUIRE((((uintptr_t)k_out | (uintptr_t)v_out) & 15) == 0, "read_pages: outputs must be 16-byte aligned");
+    a.positions = nullptr; a.req_of_row = nullptr; a.block_table = block_table; a.slots = slots;
+    a.k_out = k_out; a.v_out = v_out; a.table_stride = table_stride; a.n_pages = n_pages; a.Hk = Hk; a.D = D; a.Dv = Dv;
+    a.page_shift = ilog2_exact(page_size); a.page_size = page_size; a.total = a.k_total = 0;
+    const unsigned grid = (unsigned)n * (unsigned)Hk;
+    if (dtype == XR_F32) k_read_pages4<float><<<grid, 256, 0, stream>>>(a);
+    else k_read_pages4<bf16_t><<<grid, 256, 0, stream>>>(a);
+    XR_CHECK_LAUNCH("read_pages4");
+    return XR_OK;
+}
+
+// ---------------------------------------------------------------- attention, any head size
+// k_attention_ref over 4-bit pages: a wave a token and query head, 64 keys a turn, a key a lane for the scores and channels a lane for the
+// values; the same options.  For what the matrix-core kernel does not take and a recorded step cannot read back first.
+struct Any4Args {
+    Pages4 pages;
+    const void* q;              // [T, H * D]
+    void* out;                  // [T, H, Dv], rows ld_out apart
+    const int* positions;
+    const int* req_of_token;
+    const int* block_table;
+    const float* slopes;
+    const float* sinks;
+    const float* gate;
+    int table_stride, n_pages, H, Hk, D, Dv, page_shift, page_size, window, chunk, keep, ld_gate, ld_out;
+    float scale, cap, out_scale;
+};
+
+template <typename T>
+__global__ __launch_bounds__(64) void k_attention_any4(Any4Args a) {
+    __shared__ float qs[256];
+    const int t = blockIdx.x, h = blockIdx.y, lane = threadIdx.x;
+    const int pos = a.positions[t], kvh = h / (a.H / a.Hk);
+    const int lo = a.chunk > 0 ? pos - pos % a.chunk : (a.window > 0 && pos - a.window + 1 > 0) ? pos - a.window + 1 : 0;
+    const int kept = a.keep < lo ? a.keep : lo;
+    for (int d = lane; d < a.D; d += 64) qs[d] = ld<T>((const T*)a.q, ((size_t)t * a.H + h) * a.D + d);
+    __syncthreads();
+    const int* bt = a.block_table + (size_t)a.req_of_token[t] * a.table_stride;
+    const float slope = a.slopes ? a.slopes[h] : 0.f;
+    auto page_at = [&](int key) {           // (a place past the table, or a page that was given back: none)
+        const int bi = key >> a.page_shift;
+        const int p = bi < a.table_stride ? bt[bi] : -1;
+        return (unsigned)p < (unsigned)a.n_pages ? p : -1;
+    };
+    float m = -INFINITY, l = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int seg = kept > 0 ? 0 : 1; seg < 2; ++seg)
+        for (int k0 = seg ? lo : 0, last = seg ? pos : kept - 1; k0 <= last; k0 += 64) {
+            const int key = k0 + lane;
+            const int page = key <= last ? page_at(key) : -1;
+            float s = -INFINITY;
+            if (page >= 0) {
+                float dot = 0.f, x[8];
+                for (int c0 = 0; c0 < a.D; c0 += 8) {
+                    key_row8(a.pages, (size_t)page * a.Hk + kvh, a.page_size, a.D, key & (a.page_size - 1), c0, x);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) dot = fmaf(qs[c0 + i], x[i], dot);
+                }
+                s = dot * a.scale;
+                if (a.cap > 0.f) s = a.cap * tanhf(s / a.cap);
+                s -= slope * (float)(pos - key);
+            }
+            const float mn = fmaxf(m, wave_max(s));
+            const float p = page >= 0 ? expf(s - mn) : 0.f;
+            const float corr = m == -INFINITY ? 0.f : expf(m - mn);
+            l = l * corr + wave_sum(p);
+#pragma unroll
+            for (int dd = 0; dd < 4; ++dd) acc[dd] *= corr;
+            const int nk = min(64, last - k0 + 1);
+            for (int j = 0; j < nk; ++j) {
+                const float pj = __shfl(p, j, 64);
+                const int pg = __shfl(page, j, 64);
+                if (pg < 0) continue;
+                const size_t pb = (size_t)pg * a.Hk + kvh;
+                const int off = (k0 + j) & (a.page_size - 1);
+#pragma unroll
+                for (int dd = 0; dd < 4; ++dd) {
+                    const int d = lane + 64 * dd;
+                    if (d < a.Dv) {
+                        const uint32_t sc = (uint32_t)a.pages.vs[scale_at4(pb, a.page_size, blocks4(a.Dv), off, d >> 5)] << 23;
+                        const float2 v = pair4_f32<0>((uint32_t)a.pages.vc[value_at4(pb, a.page_size, a.Dv, off, d >> 1)], sc);
+                        acc[dd] = fmaf(pj, d & 1 ? v.y : v.x, acc[dd]);
+                    }
+                }
+            }
+            m = mn;
+        }
+    if (a.sinks) {
+        const float sk = a.sinks[h], mn = fmaxf(m, sk), corr = m == -INFINITY ? 0.f : expf(m - mn);
+        l = l * corr + expf(sk - mn);
+#pragma unroll
+        for (int dd = 0; dd < 4; ++dd) acc[dd] *= corr;
+    }
+    const float f = a.gate ? a.out_scale / (1.0f + expf(-a.gate[(size_t)t * a.ld_gate + h])) : a.out_scale;
+    T* orow = (T*)a.out + (size_t)t * a.ld_out + (size_t)h * a.Dv;
+#pragma unroll
+    for (int dd = 0; dd < 4; ++dd) {
+        const int d = lane + 64 * dd;
+        if (d < a.Dv) st<T>(orow, d, l == 0.f ? 0.f : acc[dd] / l * f);      // (0: no key that exists and no sink)
+    }
+}
+
+extern "C" int xr_attention_any4(void* out, const void* q, void* kc, void* ks, void* vc, void* vs, int n_pages, const int* positions,
+                                 const int* req_of_token, const int* block_table, int table_stride, int T, int H, int Hk, int D, int Dv,
+                                 int page_size, float scale, int window, int chunk, int keep, int dtype, const float* slopes,
+                                 const float* sinks, float cap, const float* gate, int ld_gate, float out_scale, int ld_out,
+                                 hipStream_t stream) {
+    Any4Args a;
+    a.pages = Pages4{(uint8_t*)kc, (uint8_t*)ks, (uint8_t*)vc, (uint8_t*)vs};
+    const int rc = check_pages4("attention", a.pages, Hk, D, Dv, page_size, n_pages);
+    if (rc != XR_OK) return rc;
+    XR_REQUIRE(T >= 0 && H > 0 && H <= 65535 && H % Hk == 0, "attention: %d query heads are not a multiple of %d key/value heads (65,535 at most)", H, Hk);
+    XR_REQUIRE(window >= 0 && chunk >= 0 && keep >= 0 && !(window && chunk), "attention: window %d, chunk %d or kept keys %d", window, chunk, keep);
+    XR_REQUIRE(cap >= 0.f, "attention: soft cap %g is negative", (double)cap);
+    XR_REQUIRE(ld_out >= H * Dv && (!gate || ld_gate >= H), "attention: output rows %d apart, a gate's %d", ld_out, ld_gate);
+    XR_REQUIRE(dtype == XR_F32 || dtype == XR_BF16, "attention: bad dtype %d", dtype);
+    if (T == 0) return XR_OK;
+    XR_REQUIRE(out && q && positions && req_of_token && block_table && table_stride > 0, "attention: a null operand");
+    a.q = q; a.out = out; a.positions = positions; a.req_of_token = req_of_token; a.block_table = block_table;
+    a.slopes = slopes; a.sinks = sinks; a.gate = gate; a.table_stride = table_stride; a.n_pages = n_pages; a.H = H; a.Hk = Hk;
+    a.D = D; a.Dv = Dv; a.page_shift = ilog2_exact(page_size); a.page_size = page_size; a.window = window; a.chunk = chunk; a.keep = keep;
+    a.ld_gate = ld_gate; a.ld_out = ld_out; a.scale = scale; a.cap = cap; a.out_scale = out_scale;
+    if (dtype == XR_F32) k_attention_any4<float><<<dim3(T, H), 64, 0, stream>>>(a);
+    else k_attention_any4<bf16_t><<<dim3(T, H), 64, 0, stream>>>(a);
+    XR_CHECK_LAUNCH("attention_any4");
+    return XR_OK;
+}

@@ -345,9 +345,11 @@ class StepContext:
         h[offs[6]:offs[6] + B] = [1 if rc.fresh else 0 for rc in request_caches]
         h[offs[6] + B:offs[7]] = self.starts
         h[offs[7]:offs[8]] = want_rows
+        self._held, self._page_hosts = [], []
         for g in range(n_groups):
             w = self.table_width[g]
             tab = h[offs[8 + g]:offs[9 + g]].reshape(B, w)
+            self._held.append(tab)
             tab[:] = -1
             for b, rc in enumerate(request_caches):
                 t = rc.tables[g]
@@ -408,6 +410,26 @@ class StepContext:
             plan._host = host
             self._plans[key] = plan
         return plan
+
+    def page_list(self, group: int, page_size: int, requests, mask, keep_first: int = 0):
+        """The pages that hold what the rows of ``requests`` (None: all) read, numbered from 0: ``(slots [n, 3], table, n)``, a slot's request,
+        its place in the request's block table and how many of its positions are the request's; the table as ``block_table`` with these numbers.
+        A mask's rows read from the first row's first key on (and the ``keep_first`` first positions)."""
+        slots, table = [], np.full((self.B, self.table_width[group]), -1, dtype=np.int32)
+        for b in range(self.B) if requests is None else requests:
+            end = self.seq_lens[b]
+            first = first_key(mask, self.starts[b]) // page_size
+            kept = -(-keep_first // page_size) if mask else 0
+            for i in range(-(-end // page_size)):
+                if (i >= first or i < kept) and self._held[group][b, i] >= 0:
+                    table[b, i] = len(slots)
+                    slots.append((b, i, min(page_size, end - i * page_size)))
+        n = len(slots)
+        flat = np.concatenate([np.asarray(slots, dtype=np.int32).reshape(-1), table.reshape(-1)])
+        host = torch.from_numpy(flat).pin_memory()
+        dev = host.to(self.device, non_blocking=True)
+        self._page_hosts.append(host)           # the pinned buffer lives until the copy has run
+        return dev[:3 * n], dev[3 * n:].view(table.shape), n
 
     def block_table(self, group: int) -> torch.Tensor:
         """``[B, width]`` int32: page of each block of each request of this step, -1 where none."""
