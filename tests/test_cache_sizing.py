@@ -68,3 +68,27 @@ def test_windowed_groups_take_a_fixed_share_first():
         [-(-100_000 // 64), win_pages]
     with pytest.raises(ValueError):
         size_pools([FULL], [1], 64, 2, max_requests=1)
+
+
+def test_four_bit_pages():
+    # half a byte a channel and a byte of scale for every 32: 68 bytes for a head of 128
+    assert page_bytes(FULL, 32, 64, 2, four_bit=True) == 32 * 8 * 64 * 2 * 68
+    assert page_bytes(KVSpec(1, 80, None, v_head_dim=48), 1, 16, 2, four_bit=True) == 16 * (40 + 3 + 24 + 2)
+    need = (2048 + 1) * page_bytes(FULL, 80, 64, 2, four_bit=True)
+    assert size_pools([FULL], [80], 64, 2, max_requests=64, budget_bytes=need, max_model_len=131072, four_bit=True) == [2048]
+
+
+def test_four_bit_storage():
+    import torch
+    from xyntetik_runner_amd.cache import CacheStorage, parse_cache_dtype
+    kv = [KVSpec(2, 64, None), KVSpec(2, 64, None), KVSpec(1, 64, 128, v_head_dim=32)]
+    st = CacheStorage(kv, [None] * 3, [None, 0, None], 16, 5, 2, torch.bfloat16, torch.device("cpu"), cache_dtype="mxfp4")
+    assert st.layers[1].k is st.layers[0].k and st.layers[0].v.values and not st.layers[0].k.values
+    assert (st.layers[2].k.heads, st.layers[2].k.dim, st.layers[2].v.dim, st.layers[2].v.num_pages) == (1, 64, 32, 6)
+    assert st.bytes_per_token() == 2 * 2 * 34 + 34 + 17
+    assert parse_cache_dtype("auto") is None and parse_cache_dtype("mxfp4") == "mxfp4"
+    for bad in ("fp8", "bfloat16"):
+        with pytest.raises(ValueError):
+            parse_cache_dtype(bad)
+    with pytest.raises(ValueError, match="block means"):
+        CacheStorage([KVSpec(2, 64, 128, pooled=16)], [None], [None], 16, 5, 2, torch.bfloat16, torch.device("cpu"), cache_dtype="mxfp4")

@@ -42,14 +42,17 @@ def cache_groups(kv_specs: Sequence[Optional[KVSpec]], cache_of: Sequence[Option
     return specs, owners
 
 
-def page_bytes(spec: KVSpec, n_layers: int, page_size: int, element_size: int) -> int:
-    """Bytes of one page number of a group: keys and values of all its layers."""
+def page_bytes(spec: KVSpec, n_layers: int, page_size: int, element_size: int, four_bit: bool = False) -> int:
+    """Bytes of one page number of a group: keys and values of all its layers (``four_bit``: half a byte a channel, and one for every 32)."""
+    if four_bit:
+        return n_layers * spec.num_kv_heads * page_size * sum(d // 2 + -(-d // 32) for d in (spec.head_dim, spec.value_dim))
     return n_layers * spec.num_kv_heads * (spec.head_dim + spec.value_dim) * page_size * element_size
 
 
 def size_pools(specs: Sequence[KVSpec], owners: Sequence[int], page_size: int, element_size: int,
                max_requests: int, max_step_tokens: Optional[int] = None, *, max_tokens: Optional[int] = None,
-               budget_bytes: Optional[int] = None, max_model_len: Optional[int] = None) -> List[int]:
+               budget_bytes: Optional[int] = None, max_model_len: Optional[int] = None,
+               four_bit: bool = False) -> List[int]:
     """Pages per group (the null page not counted).
 
     With ``max_tokens``: what that many tokens need (``pages_for_spec``).  Otherwise from
@@ -62,7 +65,7 @@ def size_pools(specs: Sequence[KVSpec], owners: Sequence[int], page_size: int, e
         return [pages_for_spec(s, page_size, max_tokens, max_requests, max_step_tokens) for s in specs]
     if budget_bytes is None or max_model_len is None:
         raise ValueError("a cache is sized from max_tokens, or from budget_bytes and max_model_len")
-    bpp = [page_bytes(s, n, page_size, element_size) for s, n in zip(specs, owners)]
+    bpp = [page_bytes(s, n, page_size, element_size, four_bit) for s, n in zip(specs, owners)]
     want = max(1, -(-int(max_model_len) // page_size))          # pages of one request
     step = max_step_tokens if max_step_tokens is not None else max_model_len
     sizes: List[Optional[int]] = []

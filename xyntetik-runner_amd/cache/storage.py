@@ -3,7 +3,7 @@
 For every entry of the run order that owns a cache: keys ``[pages, Hk, page_size, D]``
 and values ``[pages, Hk, D, page_size]`` (values transposed inside a page so that
 attention reads several positions of one channel with one load), in the engine's
-dtype.  A layer that keeps block means (``KVSpec.pooled``) has a second pair of tensors of the
+dtype; or, with ``cache_dtype`` "mxfp4", both in 4 bits (``FourBitPages``).  A layer that keeps block means (``KVSpec.pooled``) has a second pair of tensors of the
 same layout in the group of its blocks.  For every tensor of fixed-size state a layer names:
 ``[slots + 1, *shape]``; row ``null_slot`` (the last) belongs to no request.
 Page 0 is the null page.  Nothing is zeroed when a page changes hands: reads are
@@ -16,7 +16,18 @@ from typing import Callable, Dict, List, Optional, Union
 
 import torch
 
+from ..csrc.ops import FourBitPages
 from ..parts.base import KVSpec, StateSpec
+
+CACHE_DTYPES = (None, "mxfp4")      # the engine's dtype, or 4 bits
+
+
+def parse_cache_dtype(name: Optional[str]) -> Optional[str]:
+    """``name`` as ``CACHE_DTYPES`` has it ("auto": the engine's dtype)."""
+    name = None if name == "auto" else name
+    if name not in CACHE_DTYPES:
+        raise ValueError(f"cache dtype {name!r}: expected auto (the engine's) or mxfp4")
+    return name
 
 
 @dataclass
@@ -25,8 +36,8 @@ class LayerCache:
     group: int                 # which block table of a request applies
     page_size: int
     owns: bool                 # this entry writes keys and values (False: it reads another entry's)
-    k: Optional[torch.Tensor]
-    v: Optional[torch.Tensor]
+    k: Union[torch.Tensor, FourBitPages, None]
+    v: Union[torch.Tensor, FourBitPages, None]
     state: Optional[torch.Tensor] = None    # [slots + 1, *shape]; the last row is nobody's (the mixer's own, if it has one)
     states: Dict[str, torch.Tensor] = field(default_factory=dict)     # every state tensor of the layer by name
     pool_group: int = -1                    # the block table of the block means, for a layer that keeps them
@@ -39,11 +50,15 @@ class CacheStorage:
     def __init__(self, kv_specs: List[Optional[KVSpec]], state_specs: List[Optional[StateSpec]],
                  cache_of: List[Optional[int]], page_size: int,
                  pages_per_group: Union[int, Callable[[KVSpec], int]], n_slots: int,
-                 dtype: torch.dtype, device: torch.device, model_states: Optional[Dict[str, StateSpec]] = None):
+                 dtype: torch.dtype, device: torch.device, model_states: Optional[Dict[str, StateSpec]] = None,
+                 cache_dtype: Optional[str] = None):
         """``kv_specs[i]``/``state_specs[i]``/``cache_of[i]`` describe entry ``i`` of the run order.
         ``pages_per_group``: one number for every group, or a function of a group's ``KVSpec``
         (a group that keeps a window of keys needs fewer pages than one that keeps them all)."""
         self.page_size, self.n_slots = page_size, n_slots
+        self.cache_dtype = parse_cache_dtype(cache_dtype)
+        if self.cache_dtype is not None and any(kv is not None and kv.pooled for kv in kv_specs):
+            raise ValueError(f"a layer that keeps block means has no {cache_dtype} cache")
         sized = pages_per_group if callable(pages_per_group) else (lambda spec: pages_per_group)
         self.null_slot = n_slots
         self.group_specs: List[KVSpec] = []
@@ -58,6 +73,9 @@ class CacheStorage:
 
         def pages_of(spec: KVSpec):
             n_pages = self.group_pages[group_of(spec)] + 1
+            if self.cache_dtype is not None:
+                return tuple(FourBitPages.zeros(n_pages, spec.num_kv_heads, page_size, dim, values, device)
+                             for dim, values in ((spec.head_dim, False), (spec.value_dim, True)))
             return (torch.zeros((n_pages, spec.num_kv_heads, page_size, spec.head_dim), dtype=dtype, device=device),
                     torch.zeros((n_pages, spec.num_kv_heads, spec.value_dim, page_size), dtype=dtype, device=device))
 
@@ -112,5 +130,8 @@ class CacheStorage:
         total = 0
         for lc in self.layers:
             if lc.owns and lc.k is not None:
-                total += lc.k.shape[1] * (lc.k.shape[3] + lc.v.shape[2]) * lc.k.element_size()
+                if self.cache_dtype is not None:
+                    total += (lc.k.nbytes + lc.v.nbytes) // (lc.k.num_pages * self.page_size)
+                else:
+                    total += lc.k.shape[1] * (lc.k.shape[3] + lc.v.shape[2]) * lc.k.element_size()
         return total

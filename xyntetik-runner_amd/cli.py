@@ -50,6 +50,7 @@ options:
   --no-bos       do not put the begin-of-sequence token before the prompt
   --ignore-eos   go on generating when an end token comes
   --dtype T      bfloat16 (default) or float32
+  --cache-dtype T  auto (default: as --dtype) or mxfp4 (keys and values in 4 bits)
   --bench-json   time a short generation and print the figures as JSON
   --version      print the version and leave
   -v             print the model's sizes while loading
@@ -76,7 +77,7 @@ def unescape(s: str) -> str:
 def parse_args(argv: List[str]) -> dict:
     o = dict(model=None, prompt=None, file=None, ids=None, n=256, ctx=0, batch=512, seed=None, temp=0.0,
              top_k=0, top_p=1.0, min_p=0.0, repeat_penalty=1.0, no_bos=False, ignore_eos=False,
-             dtype="bfloat16", bench_json=False, version=False, verbose=False, help=False)
+             dtype="bfloat16", cache_dtype="auto", bench_json=False, version=False, verbose=False, help=False)
     i = 0
 
     def val(flag):
@@ -111,6 +112,7 @@ def parse_args(argv: List[str]) -> dict:
         elif a == "--no-bos": o["no_bos"] = True
         elif a == "--ignore-eos": o["ignore_eos"] = True
         elif a == "--dtype": o["dtype"] = val(a)
+        elif a == "--cache-dtype": o["cache_dtype"] = val(a)
         elif a == "--bench-json": o["bench_json"] = True
         elif a == "--version": o["version"] = True
         elif a == "-v": o["verbose"] = True
@@ -217,7 +219,8 @@ def main(argv: Optional[List[str]] = None) -> int:
     from .engine import Engine, ModelRunner
     from .sampling import SamplingParams
     try:
-        runner = ModelRunner.from_folder(o["model"], dtype=o["dtype"], max_tokens=ctx, page_size=64, max_requests=1)
+        runner = ModelRunner.from_folder(o["model"], dtype=o["dtype"], max_tokens=ctx, page_size=64, max_requests=1,
+                                         cache_dtype=o["cache_dtype"])
     except (WeightError, SafetensorsError, ValueError) as e:
         sys.stderr.write(f"error: {e}\n")
         return 1
@@ -253,7 +256,7 @@ def main(argv: Optional[List[str]] = None) -> int:
     g_rate = max(n_gen - 1, 0) / gen_s if n_gen > 1 else 0.0
     if o["bench_json"]:
         print(json.dumps({"prompt_tokens": len(prompt), "prompt_s": prompt_s, "prompt_tok_s": p_rate,
-                          "gen_tokens": n_gen, "gen_s": gen_s, "gen_tok_s": g_rate, "dtype": o["dtype"]}))
+                          "gen_tokens": n_gen, "gen_s": gen_s, "gen_tok_s": g_rate, "dtype": o["dtype"], "cache_dtype": o["cache_dtype"]}))
         return 0
     sys.stdout.write("\n")
     if req.finish_reason == "stop":

@@ -221,6 +221,14 @@ class FourBitPages:
         return self.codes.is_cuda
 
     @property
+    def dtype(self):            # (what takes 16- or 32-bit caches refuses these by it)
+        return self.codes.dtype
+
+    @property
+    def shape(self):
+        return self.codes.shape
+
+    @property
     def nbytes(self) -> int:
         return self.codes.numel() + self.scales.numel()
 

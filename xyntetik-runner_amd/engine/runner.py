@@ -12,7 +12,7 @@ from typing import Dict, Hashable, List, Optional, Sequence
 
 import torch
 
-from ..cache import CacheManager, CacheStorage, OutOfPages, cache_groups, memory_budget, size_pools
+from ..cache import CacheManager, CacheStorage, OutOfPages, cache_groups, memory_budget, page_bytes, parse_cache_dtype, size_pools
 from ..config import ModelSpec, load_config
 from ..csrc.ops import load_ops
 from ..parts.base import Runtime
@@ -38,8 +38,9 @@ class ModelRunner:
     def __init__(self, spec: ModelSpec, tensors_or_store, dtype, max_tokens: Optional[int] = None, page_size: int = 64,
                  max_requests: int = 64, device: str = "cuda:0", use_graphs: bool = True, consume_state: bool = False,
                  max_step_tokens: Optional[int] = None, gpu_memory_fraction: float = 0.9,
-                 max_model_len: Optional[int] = None):
-        """``max_tokens``: cache positions over all live requests.  None sizes the cache from the
+                 max_model_len: Optional[int] = None, cache_dtype: Optional[str] = None):
+        """``cache_dtype``: None or "auto" keeps keys and values in ``dtype``, "mxfp4" in 4 bits (4.25 with the scales), rounded as they are
+        written; models whose every attention takes such a cache (``Mixer.four_bit_cache``), others are refused.  ``max_tokens``: cache positions over all live requests.  None sizes the cache from the
         card instead: ``gpu_memory_fraction`` of its memory, less what is in use once the weights
         are bound and what a step's activations take, but no more than ``max_requests`` requests of
         ``max_model_len`` tokens (default: the model's context) can fill; ``CacheTooSmall`` if not even
@@ -52,8 +53,18 @@ class ModelRunner:
         self.dtype = parse_dtype(dtype)
         self.spec = spec
         self.ops = load_ops()
-        self.rt = Runtime(self.device, self.dtype, self.ops)
+        self.cache_dtype = parse_cache_dtype(cache_dtype)
+        four_bit = self.cache_dtype is not None
+        self.rt = Runtime(self.device, self.dtype, self.ops, four_bit)
         self.model = Model(spec)
+        if four_bit:
+            for i, step in enumerate(spec.order):
+                mixer = self.model.blocks[step.layer].mixer
+                if mixer is not None and mixer.kv_spec() is not None and not mixer.four_bit_cache:
+                    raise ValueError(f"cache dtype {cache_dtype}: run order entry {i} ({spec.layers[step.layer].mixer.kind}) keeps its keys and values "
+                                     f"in the engine's dtype only, or has heads that are no multiple of 8 channels")
+            if page_size < 8:
+                raise ValueError(f"cache dtype {cache_dtype}: pages hold at least 8 positions, not {page_size}")
         expected = self.model.expected()
         if isinstance(tensors_or_store, SafetensorsStore):
             tensors = load_tensors(tensors_or_store, expected, self.dtype, self.device)
@@ -66,18 +77,21 @@ class ModelRunner:
         specs, owners = cache_groups(kv, of)
         elt = torch.empty((), dtype=self.dtype).element_size()
         if max_tokens is not None:
-            sizes = size_pools(specs, owners, page_size, elt, max_requests, max_step_tokens, max_tokens=max_tokens)
+            sizes = size_pools(specs, owners, page_size, elt, max_requests, max_step_tokens, max_tokens=max_tokens, four_bit=four_bit)
         else:
             torch.cuda.synchronize(self.device)
             free, total = torch.cuda.mem_get_info(self.device)
             # what torch holds without having handed it out is as good as free
             free += torch.cuda.memory_reserved(self.device) - torch.cuda.memory_allocated(self.device)
             working = max(1 << 30, (max_step_tokens or 2048) << 20)     # a step's activations, generously
+            if four_bit and specs:      # and the longest request's pages of a layer, read back for the attention of a portion
+                working += max(page_bytes(s, 1, page_size, elt) for s in specs) * -(-(max_model_len or spec.max_position) // page_size)
             sizes = size_pools(specs, owners, page_size, elt, max_requests, max_step_tokens,
                                budget_bytes=memory_budget(total, free, gpu_memory_fraction, working),
-                               max_model_len=max_model_len or spec.max_position)
+                               max_model_len=max_model_len or spec.max_position, four_bit=four_bit)
         self.storage = CacheStorage(kv, st, of, page_size, lambda s: sizes[specs.index(s)], max_requests,
-                                    self.dtype, self.device, model_states=self.model.model_states())
+                                    self.dtype, self.device, model_states=self.model.model_states(),
+                                    cache_dtype=self.cache_dtype)
         self.model.attach_states(self.storage.model_states)
         assert self.storage.group_specs == specs
         self.manager = CacheManager(specs, page_size, self.storage.group_pages, max_requests)

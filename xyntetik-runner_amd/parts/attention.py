@@ -113,6 +113,11 @@ class PagedAttention(Mixer):
         self.v_size = self.num_kv_heads * self.v_head_dim
         self.w_in = self.b_in = self.w_out = self.b_out = None
 
+    @property
+    def four_bit_cache(self) -> bool:
+        # (a norm behind the rotation is part of a kernel that writes the engine's type)
+        return not self.by_head and self.head_dim % 8 == 0 and self.v_head_dim % 8 == 0
+
     # what the cache manager must keep
     def kv_spec(self) -> Optional[KVSpec]:
         # a chunk never reaches further back than its length: its pages are kept as a window's of that length are
@@ -208,6 +213,8 @@ class PagedAttention(Mixer):
         H, Hk, D = self.num_heads, self.num_kv_heads, self.head_dim
         ws, bsf = self.w_sfx, self.b_sfx
         self.paired = False
+        # 4-bit pages are written by the kernel that rotates; a norm of whole rows then is the transform it is elsewhere
+        self.row_normed = self.row_normed and not rt.four_bit_cache
         if self.by_head:
             w_in, self.b_in = self.joint_inputs(tensors)
             self.w_in = rt.ops.pack_weight(w_in)
@@ -292,7 +299,12 @@ class PagedAttention(Mixer):
                 ops.rotate_rows_(q_in, ctx.positions, rot.inv_freq, H, D, rot.rotary_dim, 1.0)
                 if writes:
                     ops.rotate_rows_(k_in, ctx.positions, rot.inv_freq, Hk, D, rot.rotary_dim, 1.0)
-            q = ops.qkv_store(q_in, k_in, v_in, cache.k, cache.v, ctx, cache.group, H, Hk, D, Dv, cache.page_size, rt.dtype)
+            if writes and rt.four_bit_cache:
+                q = torch.empty((T, Q), dtype=rt.dtype, device=h.device)
+                ops.rope_kv_write(q_in, k_in, v_in, q, cache.k, cache.v, ctx.positions, ctx.req_of_token, table, None, H, Hk, D, 0, False, 1.0,
+                                  cache.page_size)
+            else:
+                q = ops.qkv_store(q_in, k_in, v_in, cache.k, cache.v, ctx, cache.group, H, Hk, D, Dv, cache.page_size, rt.dtype)
         elif self.row_normed:
             # norm over all heads, rotation and cache write in one kernel behind the product
             proj = ops.linear(h, self.w_in, bias=self.b_in, out_dtype=torch.float32)

@@ -202,6 +202,9 @@ class Mixer(Part):
     def forward(self, ctx, cache, h: torch.Tensor) -> torch.Tensor:
         raise NotImplementedError
 
+    #: True if the mixer writes and reads keys and values held in 4 bits (``cache.k`` and ``cache.v`` are then ``FourBitPages``)
+    four_bit_cache = False
+
     #: True if ``h`` may be an ``UnscaledRows`` or an ``UnnormedRows`` (it only goes into ``Ops.linear``)
     takes_unscaled_rows = False
 
@@ -373,6 +376,7 @@ class Runtime:
     device: torch.device
     dtype: torch.dtype              # compute dtype: torch.float32 or torch.bfloat16
     ops: Any                        # xyntetik_runner_amd.csrc.ops.Ops
+    four_bit_cache: bool = False    # keys and values are kept in 4 bits (``FourBitPages``), not in the compute dtype
 
     @property
     def is_fp32(self) -> bool:

@@ -59,6 +59,7 @@ def main(argv=None) -> int:
     ap = argparse.ArgumentParser(prog="trace_run", description="replay token traces through the engine and dump logits")
     ap.add_argument("--model", required=True, help="folder with config.json and model.safetensors")
     ap.add_argument("--dtype", required=True, choices=["bfloat16", "float32"])
+    ap.add_argument("--cache-dtype", default="auto", choices=["auto", "mxfp4"], help="keys and values in the engine's dtype (auto) or in 4 bits")
     ap.add_argument("--out", required=True, help="folder for <step>.f32 files")
     ap.add_argument("--max-tokens", type=int, required=True,
                     help="most tokens live requests hold at any time (each rounded up to the page size)")
@@ -67,7 +68,7 @@ def main(argv=None) -> int:
     args = ap.parse_args(argv)
     from .engine.runner import ModelRunner
     runner = ModelRunner.from_folder(args.model, dtype=args.dtype, max_tokens=args.max_tokens,
-                                     page_size=args.page_size, max_requests=args.max_requests)
+                                     page_size=args.page_size, max_requests=args.max_requests, cache_dtype=args.cache_dtype)
     replay(runner, sys.stdin, args.out)
     return 0
 
