@@ -253,7 +253,7 @@ ATTEND = [
     (16, 1, 64, 32, 32, None, [300, 2], [1, 1]),
     (5, 5, 128, 128, 128, 100, [0, 99, 100, 101, 700], [16, 9, 3, 1, 2]),
     (6, 2, 256, 256, 32, None, [400, 2], [5, 1]),
-    (4, 2, 256, 128, 64, Chunked(64), [63, 64, 200], [2, 1, 3]),
+    (4, 2, 256, 192, 64, Chunked(64), [63, 64, 200], [2, 1, 3]),
     (4, 2, 128, 128, 64, None, [5000], [1]),
     (3, 3, 96, 96, 32, 33, [3000, 40], [1, 1]),
     (4, 2, 64, 64, 64, None, [0, 300, 10], [130, 1, 33]),                  # a portion beside a decoded token

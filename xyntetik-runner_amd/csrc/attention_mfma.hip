@@ -32,6 +32,7 @@
 
 #include "common.h"
 #include "async_copy.h"
+#include "pages4.h"
 
 #ifndef XR_HEAD_DIM
 #error "compile with -DXR_HEAD_DIM=<head size>"
@@ -84,6 +85,7 @@ struct AttnArgs {
     int ld_gate;
     float out_scale;
     int ld_out;
+    Pages4 four;            // the cache where it is held in 4 bits (kc and vc are not read then)
 };
 
 __device__ inline float row_factor(const float* gate, int ld_gate, float out_scale, int t, int h) {
@@ -1108,10 +1110,206 @@ __device__ __forceinline__ float2 load_agent(const float* p) {
     return make_float2(__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32)));
 }
 
+// The end of a kernel for few rows: every wave has left its rows' unnormalised outputs in `mo`, their references and sums in `mml`; they are combined
+// here (sum_w 2^(m_w - max) O_w over sum_w 2^(m_w - max) l_w), and the row block's key ranges added up.
+constexpr int FEW_MS = HV + 4;                                // floats between rows of the combining buffer
+__device__ __forceinline__ void few_finish(const AttnArgs& a, const int* it, int kvh, int row0, int slot, int q0, int q_len, int G, float* mo, float* mml,
+                                           int* last_one) {
+    constexpr int MS = FEW_MS;
+    const int tid = threadIdx.x;
+    __syncthreads();
+    const int n_rows = q_len * G - row0 < FEW_ROWS ? q_len * G - row0 : FEW_ROWS;
+    for (int idx = tid; idx < n_rows * (HV / 2); idx += 64 * FEW_WAVES) {
+        const int r = idx / (HV / 2), d2 = (idx - r * (HV / 2)) * 2;
+        float mx = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < FEW_WAVES; ++w) mx = fmaxf(mx, mml[(w * FEW_ROWS + r) * 2]);
+        float2 acc = make_float2(0.f, 0.f);
+        float lsum = 0.f;
+#pragma unroll
+        for (int w = 0; w < FEW_WAVES; ++w) {
+            const float mw = mml[(w * FEW_ROWS + r) * 2], lw = mml[(w * FEW_ROWS + r) * 2 + 1];
+            const float f = lw > 0.f ? __builtin_amdgcn_exp2f(mw - mx) : 0.f;
+            const float2 v = *reinterpret_cast<const float2*>(mo + (w * FEW_ROWS + r) * MS + d2);
+            acc.x += f * v.x; acc.y += f * v.y;
+            lsum += f * lw;
+        }
+        const int rr = row0 + r, tk = rr / G, hh = kvh * G + (rr - tk * G);
+        if (slot < 0) {
+            lsum = with_sink(a.sinks, hh, mx, lsum);
+            const float inv = (lsum > 0.f ? 1.0f / lsum : 0.f) * row_factor(a.gate, a.ld_gate, a.out_scale, q0 + tk, hh);
+            bf16_t* op = a.out + (size_t)(q0 + tk) * a.ld_out + hh * HV + d2;
+            *reinterpret_cast<uint32_t*>(op) = pack2(acc.x * inv, acc.y * inv);
+        } else {
+            const float inv = lsum > 0.f ? 1.0f / lsum : 0.f;
+            store_agent(a.part_o + (((size_t)slot * a.Hk + kvh) * ROWS + r) * HV + d2, acc.x * inv, acc.y * inv);
+            if (d2 == 0) store_agent(a.part_ml + (((size_t)slot * a.Hk + kvh) * ROWS + r) * 2, mx, lsum);
+        }
+    }
+    if (slot < 0) return;
+
+    // ---- the last of a row block's workgroups adds the key ranges up.  Each has its partial result where all others read it
+    // (the wait is for this wave's own stores) before it counts itself in; the counter is zero again afterwards.
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    const int s0 = it[8], ns = it[9];
+    if (tid == 0) {
+        int* count = a.counters + (size_t)it[10] * a.Hk + kvh;
+        const int before = __hip_atomic_fetch_add(count, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        *last_one = before == it[11] - 1;
+        if (before == it[11] - 1) __hip_atomic_store(count, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __syncthreads();
+    if (!*last_one) return;
+    const int total = n_rows * (HV / 2);
+    const size_t ml_step = (size_t)a.Hk * ROWS * 2, po_step = (size_t)a.Hk * ROWS * HV;
+    if (total <= 64 * FEW_WAVES) {
+        // a pair of channels a thread, which weighs its row's ranges by itself, 16 at a time
+        if (tid >= total) return;
+        const int r = tid / (HV / 2), d2 = (tid - r * (HV / 2)) * 2;
+        const float* ml = a.part_ml + (((size_t)s0 * a.Hk + kvh) * ROWS + r) * 2;
+        const float* po = a.part_o + (((size_t)s0 * a.Hk + kvh) * ROWS + r) * HV + d2;
+        constexpr int U = 16;
+        float mx = -INFINITY, wsum = 0.f;
+        float2 acc = make_float2(0.f, 0.f);
+        for (int b = 0; b < ns; b += U) {
+            float2 mlv[U], pv[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int sc = b + u < ns ? b + u : b;
+                mlv[u] = load_agent(ml + sc * ml_step);
+                pv[u] = load_agent(po + sc * po_step);
+            }
+            __builtin_amdgcn_sched_barrier(0);           // (or the first numbers are waited for one by one: 2 us)
+            float cm = mx;
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (b + u < ns) cm = fmaxf(cm, mlv[u].x);
+            const float resc = mx == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mx - cm);
+            acc.x *= resc; acc.y *= resc;
+            wsum *= resc;
+            mx = cm;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const float w = (b + u < ns && mlv[u].y > 0.f) ? mlv[u].y * __builtin_amdgcn_exp2f(mlv[u].x - mx) : 0.f;
+                acc.x += w * pv[u].x; acc.y += w * pv[u].y;
+                wsum += w;
+            }
+        }
+        const int rr = row0 + r, tk = rr / G, hh = kvh * G + (rr - tk * G);
+        wsum = with_sink(a.sinks, hh, mx, wsum);
+        const float inv = (wsum > 0.f ? 1.0f / wsum : 0.f) * row_factor(a.gate, a.ld_gate, a.out_scale, q0 + tk, hh);
+        bf16_t* op = a.out + (size_t)(q0 + tk) * a.ld_out + hh * HV + d2;
+        *reinterpret_cast<uint32_t*>(op) = pack2(acc.x * inv, acc.y * inv);
+        return;
+    }
+    // More: 16 lanes a row weigh its ranges, 64 of them a turn, while a thread's pairs of channels are on their way, up to 64 loads.  (As above, a pair after
+    // the other, each with the weights anew: 6 trips for 16 rows of 192 channels.  A request of 500 keys, 16 heads over one of 256 x 192 21.6 us -> 13.3, of 128 x 128
+    // 11.3 -> 9.4, the streaming kernel and its merge 15.1 and 10.7; for 4 rows of 128 channels the way above is 0.6 us shorter.)
+    float* const weight = mo;                            // [FEW_ROWS][FEW_TURN]
+    float* const factor = mml;                           // [FEW_ROWS] what a turn's sums before it are multiplied by, then [FEW_ROWS] the results
+    const int wr = tid >> 4, wj = tid & 15;
+    const float* const ml = a.part_ml + (((size_t)s0 * a.Hk + kvh) * ROWS + (wr < n_rows ? wr : 0)) * 2;
+    const float* const po = a.part_o + ((size_t)s0 * a.Hk + kvh) * ROWS * HV;      // (a row block's rows lie one after the other)
+    constexpr int PB = FEW_PAIRS, U = 16;
+    for (int p0 = 0; p0 < total; p0 += PB * 64 * FEW_WAVES) {
+        float2 acc[PB];
+        int at[PB];
+#pragma unroll
+        for (int p = 0; p < PB; ++p) {
+            acc[p] = make_float2(0.f, 0.f);
+            at[p] = p0 + p * 64 * FEW_WAVES + tid < total ? p0 + p * 64 * FEW_WAVES + tid : 0;
+        }
+        float mx = -INFINITY, wsum = 0.f;
+        for (int g = 0; g < ns; g += FEW_TURN) {
+            const int n = ns - g < FEW_TURN ? ns - g : FEW_TURN;
+            const bool weigh = p0 == 0 || ns > FEW_TURN;
+            float2 mlv[FEW_TURN / 16], pv[PB][U];
+            if (weigh)
+#pragma unroll
+                for (int i = 0; i < FEW_TURN / 16; ++i)
+                    if (16 * i < n) mlv[i] = load_agent(ml + (g + (wj + 16 * i < n ? wj + 16 * i : 0)) * ml_step);
+            auto load = [&](int b) __attribute__((always_inline)) {
+#pragma unroll
+                for (int p = 0; p < PB; ++p)
+                    if (p0 + p * 64 * FEW_WAVES < total)
+#pragma unroll
+                        for (int e = 0; e < U; e += 8) {
+                            if (b + e < n) {
+#pragma unroll
+                                for (int u = e; u < e + 8; ++u) pv[p][u] = load_agent(po + (g + (b + u < n ? b + u : b)) * po_step + 2 * at[p]);
+                            } else {
+#pragma unroll
+                                for (int u = e; u < e + 8; ++u) pv[p][u] = make_float2(0.f, 0.f);
+                            }
+                        }
+            };
+            load(0);
+            __builtin_amdgcn_sched_barrier(0);
+            if (weigh) {
+                float cm = mx, sum = 0.f;
+#pragma unroll
+                for (int i = 0; i < FEW_TURN / 16; ++i)
+                    if (wj + 16 * i < n) cm = fmaxf(cm, mlv[i].x);
+#pragma unroll
+                for (int o = 1; o < 16; o <<= 1) cm = fmaxf(cm, __shfl_xor(cm, o, 64));
+                const float before = mx == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mx - cm);
+                if (g > 0 || p0 > 0) __syncthreads();        // (the weights of the turn before are read)
+#pragma unroll
+                for (int i = 0; i < FEW_TURN / 16; ++i) {
+                    const float w = wj + 16 * i < n && mlv[i].y > 0.f ? mlv[i].y * __builtin_amdgcn_exp2f(mlv[i].x - cm) : 0.f;
+                    weight[wr * FEW_TURN + wj + 16 * i] = w;
+                    sum += w;
+                }
+#pragma unroll
+                for (int o = 1; o < 16; o <<= 1) sum += __shfl_xor(sum, o, 64);
+                wsum = wsum * before + sum;
+                mx = cm;
+                if (wj == 0) {
+                    factor[wr] = before;
+                    if (g + FEW_TURN >= ns && wr < n_rows) {
+                        const int rr = row0 + wr, tk = rr / G, hh = kvh * G + (rr - tk * G);
+                        const float all = with_sink(a.sinks, hh, mx, wsum);
+                        factor[FEW_ROWS + wr] = (all > 0.f ? 1.0f / all : 0.f) * row_factor(a.gate, a.ld_gate, a.out_scale, q0 + tk, hh);
+                    }
+                }
+                __syncthreads();
+            }
+            if (g > 0)
+#pragma unroll
+                for (int p = 0; p < PB; ++p) {
+                    const float f = factor[at[p] / (HV / 2)];
+                    acc[p].x *= f; acc[p].y *= f;
+                }
+            for (int b = 0; b < n; b += U) {
+                if (b > 0) load(b);
+#pragma unroll
+                for (int p = 0; p < PB; ++p)
+                    if (p0 + p * 64 * FEW_WAVES < total) {
+                        const float* const w = weight + at[p] / (HV / 2) * FEW_TURN + b;
+#pragma unroll
+                        for (int u = 0; u < U; ++u) {         // (weights past the last range are 0)
+                            acc[p].x += w[u] * pv[p][u].x; acc[p].y += w[u] * pv[p][u].y;
+                        }
+                    }
+            }
+        }
+#pragma unroll
+        for (int p = 0; p < PB; ++p) {
+            if (p0 + p * 64 * FEW_WAVES + tid >= total) continue;
+            const int r = at[p] / (HV / 2), d2 = (at[p] - r * (HV / 2)) * 2;
+            const int rr = row0 + r, tk = rr / G, hh = kvh * G + (rr - tk * G);
+            const float inv = factor[FEW_ROWS + r];
+            bf16_t* op = a.out + (size_t)(q0 + tk) * a.ld_out + hh * HV + d2;
+            *reinterpret_cast<uint32_t*>(op) = pack2(acc[p].x * inv, acc[p].y * inv);
+        }
+    }
+}
+
 template <int MODE, bool OK = FEW_OK>
 __global__ __launch_bounds__(64 * FEW_WAVES, FEW_PER_CU) void k_attn_few(AttnArgs a) {
     if constexpr (OK) {
-    constexpr int MS = HV + 4;                                // floats between rows of the combining buffer
+    constexpr int MS = FEW_MS;
     __shared__ float mo[FEW_WAVES * FEW_ROWS * MS];
     __shared__ float mml[FEW_WAVES * FEW_ROWS * 2];
     __shared__ int last_one;
@@ -1292,193 +1490,305 @@ __global__ __launch_bounds__(64 * FEW_WAVES, FEW_PER_CU) void k_attn_few(AttnArg
             mml[(wave * FEW_ROWS + lr) * 2 + 1] = l;
         }
     }
-    __syncthreads();
-    const int n_rows = q_len * G - row0 < FEW_ROWS ? q_len * G - row0 : FEW_ROWS;
-    for (int idx = tid; idx < n_rows * (HV / 2); idx += 64 * FEW_WAVES) {
-        const int r = idx / (HV / 2), d2 = (idx - r * (HV / 2)) * 2;
-        float mx = -INFINITY;
-#pragma unroll
-        for (int w = 0; w < FEW_WAVES; ++w) mx = fmaxf(mx, mml[(w * FEW_ROWS + r) * 2]);
-        float2 acc = make_float2(0.f, 0.f);
-        float lsum = 0.f;
-#pragma unroll
-        for (int w = 0; w < FEW_WAVES; ++w) {
-            const float mw = mml[(w * FEW_ROWS + r) * 2], lw = mml[(w * FEW_ROWS + r) * 2 + 1];
-            const float f = lw > 0.f ? __builtin_amdgcn_exp2f(mw - mx) : 0.f;
-            const float2 v = *reinterpret_cast<const float2*>(mo + (w * FEW_ROWS + r) * MS + d2);
-            acc.x += f * v.x; acc.y += f * v.y;
-            lsum += f * lw;
-        }
-        const int rr = row0 + r, tk = rr / G, hh = kvh * G + (rr - tk * G);
-        if (slot < 0) {
-            lsum = with_sink(a.sinks, hh, mx, lsum);
-            const float inv = (lsum > 0.f ? 1.0f / lsum : 0.f) * row_factor(a.gate, a.ld_gate, a.out_scale, q0 + tk, hh);
-            bf16_t* op = a.out + (size_t)(q0 + tk) * a.ld_out + hh * HV + d2;
-            *reinterpret_cast<uint32_t*>(op) = pack2(acc.x * inv, acc.y * inv);
-        } else {
-            const float inv = lsum > 0.f ? 1.0f / lsum : 0.f;
-            store_agent(a.part_o + (((size_t)slot * a.Hk + kvh) * ROWS + r) * HV + d2, acc.x * inv, acc.y * inv);
-            if (d2 == 0) store_agent(a.part_ml + (((size_t)slot * a.Hk + kvh) * ROWS + r) * 2, mx, lsum);
-        }
+    few_finish(a, it, kvh, row0, slot, q0, q_len, G, mo, mml, &last_one);
     }
-    if (slot < 0) return;
+}
 
-    // ---- the last of a row block's workgroups adds the key ranges up.  Each has its partial result where all others read it
-    // (the wait is for this wave's own stores) before it counts itself in; the counter is zero again afterwards.
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    const int s0 = it[8], ns = it[9];
-    if (tid == 0) {
-        int* count = a.counters + (size_t)it[10] * a.Hk + kvh;
-        const int before = __hip_atomic_fetch_add(count, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        last_one = before == it[11] - 1;
-        if (before == it[11] - 1) __hip_atomic_store(count, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+// ------------------------------------------------------------------------------ few rows over 4-bit pages
+// k_attn_few with codes in place of keys and values: 68 bytes a position and head of 128 for 256 (pages4.h).  The products are the same bfloat16 ones: a
+// block's codes become bfloat16 with their scale in one instruction for two numbers, exactly, so nothing is rounded that was not rounded when it was
+// written.  The arrangement follows from what a lane may convert without asking its neighbours:
+//
+// Keys: a lane's share of a key, a fourth of its channels, is whole words of codes with one scale (a block for heads of 128), so step kd of the score product
+// takes word kd of every lane; queries are read in that order.
+// Values: operands want two positions side by side in a word, codes have two channels, and a scale belongs to a position.  A lane holds 8 positions of HV / 16
+// neighbouring channels; a pair of channels is converted position by position and two positions' words change halves (32 conversions and 32 exchanges of
+// halves for 32 keys x 128 channels).  Row m of output block d so stands for channel m * HV / 16 + d.
+// Scales past a request's end are taken as zeros' and codes there are any numbers: no operand has to be masked.
+constexpr bool FOUR_OK = HD % 32 == 0 && HV % 32 == 0;
+constexpr int NB4K = HD / 32, NB4V = FOUR_OK ? HV / 32 : 1;              // blocks of a key and of a value
+constexpr int KS4 = FKD % 4 == 0 ? FKD / 4 : 4 % FKD == 0 ? 1 : FKD;      // scales of a lane's share of a key: of whole blocks, of a part of one, or word by word
+constexpr int VP4 = FDB >= 2 ? FDB / 2 : 1;                               // pairs of channels of a lane
+constexpr int VS4 = 32 % FDB == 0 ? 1 : VP4;                              // scales of its values: one, or pair by pair
+constexpr int FOUR_SUBS = HD + HV <= 256 ? 2 : 1;
+constexpr int FOUR_STEP = 32 * FOUR_SUBS;
+typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
+
+struct FourTile {
+    uint32_t k[FOUR_SUBS][2][FKD];
+    u32x2_t ks[FOUR_SUBS][KS4], v[FOUR_SUBS][VP4], vs[FOUR_SUBS][VS4];
+    int pg[FOUR_SUBS];
+};
+
+// N words from where they lie side by side, in as few loads as their alignment (a multiple of N * 4 bytes, or of 4) allows
+template <int N> __device__ __forceinline__ void load_words(uint32_t* dst, const uint8_t* src) {
+    if constexpr (N % 4 == 0) {
+#pragma unroll
+        for (int i = 0; i < N; i += 4) {
+            const u32x4_t w = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(src + 4 * i));
+#pragma unroll
+            for (int j = 0; j < 4; ++j) dst[i + j] = w[j];
+        }
+    } else if constexpr (N % 2 == 0) {
+#pragma unroll
+        for (int i = 0; i < N; i += 2) {
+            const u32x2_t w = __builtin_nontemporal_load(reinterpret_cast<const u32x2_t*>(src + 4 * i));
+            dst[i] = w[0];
+            dst[i + 1] = w[1];
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) dst[i] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(src + 4 * i));
     }
-    __syncthreads();
-    if (!last_one) return;
-    const int total = n_rows * (HV / 2);
-    const size_t ml_step = (size_t)a.Hk * ROWS * 2, po_step = (size_t)a.Hk * ROWS * HV;
-    if (total <= 64 * FEW_WAVES) {
-        // a pair of channels a thread, which weighs its row's ranges by itself, 16 at a time
-        if (tid >= total) return;
-        const int r = tid / (HV / 2), d2 = (tid - r * (HV / 2)) * 2;
-        const float* ml = a.part_ml + (((size_t)s0 * a.Hk + kvh) * ROWS + r) * 2;
-        const float* po = a.part_o + (((size_t)s0 * a.Hk + kvh) * ROWS + r) * HV + d2;
-        constexpr int U = 16;
-        float mx = -INFINITY, wsum = 0.f;
-        float2 acc = make_float2(0.f, 0.f);
-        for (int b = 0; b < ns; b += U) {
-            float2 mlv[U], pv[U];
+}
+__device__ __forceinline__ uint32_t last_byte4(uint32_t x) { return (~x - 0x01010101u) & x & 0x80808080u; }    // not 0: a byte of x is 255
+// byte i of two words where a scale's exponent is wanted
+template <int I> __device__ __forceinline__ uint32_t scale_bits4(u32x2_t w) {
+    const uint32_t x = w[I >> 2];
+    return (I & 3) == 0 ? x << 23 : (I & 3) == 1 ? x << 15 : (I & 3) == 2 ? x << 7 : x >> 1;
+}
+// a pair of channels at 8 positions as bfloat16: the operands of the even and of the odd channel
+__device__ __forceinline__ void values4(u32x2_t codes, u32x2_t s, u32x4_t& even, u32x4_t& odd) {
+    const uint32_t c[8] = {pair4_bf16<0>(codes[0], scale_bits4<0>(s)), pair4_bf16<1>(codes[0], scale_bits4<1>(s)), pair4_bf16<2>(codes[0], scale_bits4<2>(s)),
+                           pair4_bf16<3>(codes[0], scale_bits4<3>(s)), pair4_bf16<0>(codes[1], scale_bits4<4>(s)), pair4_bf16<1>(codes[1], scale_bits4<5>(s)),
+                           pair4_bf16<2>(codes[1], scale_bits4<6>(s)), pair4_bf16<3>(codes[1], scale_bits4<7>(s))};
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int sc = b + u < ns ? b + u : b;
-                mlv[u] = load_agent(ml + sc * ml_step);
-                pv[u] = load_agent(po + sc * po_step);
+    for (int j = 0; j < 4; ++j) {
+        even[j] = __builtin_amdgcn_perm(c[2 * j + 1], c[2 * j], 0x05040100u);
+        odd[j] = __builtin_amdgcn_perm(c[2 * j + 1], c[2 * j], 0x07060302u);
+    }
+}
+
+template <int MODE, bool OK = FOUR_OK>
+__global__ __launch_bounds__(64 * FEW_WAVES, FEW_PER_CU) void k_attn_few4(AttnArgs a) {
+    if constexpr (OK) {
+    __shared__ float mo[FEW_WAVES * FEW_ROWS * FEW_MS];
+    __shared__ float mml[FEW_WAVES * FEW_ROWS * 2];
+    __shared__ int last_one;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int item_no = (int)(blockIdx.x / (unsigned)a.Hk);
+    const int kvh = (int)blockIdx.x - item_no * a.Hk;
+    const int* it = a.few_items + (size_t)item_no * FEW_INTS;
+    const int req = it[0], row0 = it[1], kbeg = it[2], kend = it[3], slot = it[4];
+    const int q0 = it[5], q_len = it[6], start = it[7];
+    if (kend <= kbeg) return;                                 // (an item that pads a recorded step's list)
+    const int G = a.H / a.Hk;
+    const int lr = lane & 15, quad = lane >> 4;
+    const int seq_len = start + q_len;
+    const int* bt = a.block_table + (size_t)req * a.table_stride;
+
+    int pages_base = kbeg >> a.page_shift;
+    int my_page;
+    auto look_up = [&]() {
+        const int pi = pages_base + lane;
+        const bool in = ((long)pi << a.page_shift) < seq_len;
+        my_page = bt[in ? pi : 0];
+        my_page = in ? my_page : -1;
+    };
+    look_up();
+
+    const int rho = row0 + lr;
+    const int tok = rho / G, hg = rho - tok * G;
+    const bool row_ok = tok < q_len;
+    const int t = q0 + tok, h = kvh * G + hg;
+    const int pos = start + tok;
+    auto first = [&](int p) { return a.chunk > 0 ? p - p % a.chunk : (a.window > 0 && p - a.window + 1 > 0) ? p - a.window + 1 : 0; };
+    const int lo = first(pos);
+    const int last_tok = (row0 + FEW_ROWS - 1) / G;
+    const int pos_min = start + row0 / G;
+    const int lo_max = first(start + (last_tok < q_len ? last_tok : q_len - 1));
+    const float sb = MODE == MODE_SLOPES ? a.slopes[row_ok ? h : 0] / a.scale : 0.f;
+    bf16x8 qf[FKD];
+    {
+        const bf16_t* qp = a.q + ((size_t)(row_ok ? t : q0) * a.H + (row_ok ? h : 0)) * HD + quad * (8 * FKD);
+#pragma unroll
+        for (int kd = 0; kd < FKD; ++kd) qf[kd] = as_bf16x8(keep_if(row_ok, ldg16(qp + kd * 8)));
+    }
+    // where a lane's bytes lie behind a tile's first
+    const uint32_t koff = (uint32_t)(((lr >> 2) * 8 + (lr & 3)) * (HD / 2) + quad * (4 * FKD));
+    const uint32_t voff = (uint32_t)((quad * (HV / 2) + lr * VP4) * 8);
+    uint32_t ksoff[KS4], vsoff[VS4];
+#pragma unroll
+    for (int i = 0; i < KS4; ++i) ksoff[i] = (uint32_t)(((lr >> 2) * NB4K + (FKD % 4 == 0 ? quad * KS4 + i : (quad * FKD + i) >> 2)) * 8);
+#pragma unroll
+    for (int i = 0; i < VS4; ++i) vsoff[i] = (uint32_t)((quad * NB4V + ((lr * FDB + 2 * i) >> 5)) * 8);
+    const uint32_t kturn = (uint32_t)((8 * (lr & 3) + 9) & 31);            // what brings the byte of the lane's key to a scale's exponent
+
+    auto load = [&](FourTile& x, int j) __attribute__((always_inline)) {
+        const int k0 = kbeg + (wave + j * FEW_WAVES) * FOUR_STEP;
+        if (((k0 + FOUR_STEP - 1) >> a.page_shift) - pages_base >= 64) {
+            pages_base = k0 >> a.page_shift;
+            look_up();
+        }
+#pragma unroll
+        for (int u = 0; u < FOUR_SUBS; ++u) {
+            const int kt = k0 + 32 * u;
+            const int pg = __builtin_amdgcn_readlane(my_page, __builtin_amdgcn_readfirstlane((kt >> a.page_shift) - pages_base));
+            x.pg[u] = pg;
+            const size_t pb = (size_t)(pg < 0 ? 0 : pg) * a.Hk + kvh;
+            const int ko = kt & a.page_mask;
+            const size_t octet = pb * (size_t)(a.page_size >> 3) + (ko >> 3);
+            const uint8_t* kb = a.four.kc + (pb * a.page_size + ko) * (size_t)(HD / 2);
+            const uint8_t* ksb = a.four.ks + octet * (NB4K * 8);
+            const uint8_t* vb = a.four.vc + octet * (HV / 2 * 8);
+            const uint8_t* vsb = a.four.vs + octet * (NB4V * 8);
+#pragma unroll
+            for (int b = 0; b < 2; ++b) load_words<FKD>(x.k[u][b], kb + (koff + (uint32_t)(b * 4 * (HD / 2))));
+#pragma unroll
+            for (int i = 0; i < KS4; ++i) x.ks[u][i] = *reinterpret_cast<const u32x2_t*>(ksb + ksoff[i]);
+            uint32_t w[2 * VP4];
+            load_words<2 * VP4>(w, vb + voff);
+#pragma unroll
+            for (int p = 0; p < VP4; ++p) { x.v[u][p][0] = w[2 * p]; x.v[u][p][1] = w[2 * p + 1]; }
+#pragma unroll
+            for (int i = 0; i < VS4; ++i) x.vs[u][i] = *reinterpret_cast<const u32x2_t*>(vsb + vsoff[i]);
+        }
+    };
+
+    f32x4 o[FDB];
+#pragma unroll
+    for (int d = 0; d < FDB; ++d)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[d][e] = 0.f;
+    float m = -INFINITY, l = 0.f;      // m in units of log2
+    const float c2 = MODE == MODE_CAP ? 1.0f : a.scale * 1.44269504088896340736f;
+    const SoftCap cap(a.scale, a.cap);
+
+    auto compute = [&](FourTile& x, int j) __attribute__((always_inline)) {
+#pragma unroll
+        for (int u = 0; u < FOUR_SUBS; ++u) {
+            const int kt = kbeg + (wave + j * FEW_WAVES) * FOUR_STEP + 32 * u;
+            if (FOUR_SUBS > 1 && u > 0 && kt >= kend) break;
+            float s[8];
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                f32x4 z;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) z[e] = MODE == MODE_SLOPES ? sb * (float)(kt + 8 * quad + 4 * b + e - pos) : 0.f;
+#pragma unroll
+                for (int kd = 0; kd < FKD; ++kd) {
+                    const uint32_t c = x.k[u][b][kd], ss = x.ks[u][FKD % 4 == 0 ? kd / 4 : KS4 == 1 ? 0 : kd][b];
+                    const uint32_t sc = __builtin_amdgcn_alignbit(ss, ss, kturn);
+                    const bf16x8 kf = as_bf16x8(make_uint4(pair4_bf16<0>(c, sc), pair4_bf16<1>(c, sc), pair4_bf16<2>(c, sc), pair4_bf16<3>(c, sc)));
+                    z = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[kd], z, 0, 0, 0);
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[4 * b + e] = MODE == MODE_CAP ? cap.less(z[e], 0.f) : z[e];
             }
-            __builtin_amdgcn_sched_barrier(0);           // (or the first numbers are waited for one by one: 2 us)
-            float cm = mx;
+            const bool whole = kt + 32 <= kend && kt + 31 <= pos_min && kt >= lo_max;
+            if (!whole) {
 #pragma unroll
-            for (int u = 0; u < U; ++u)
-                if (b + u < ns) cm = fmaxf(cm, mlv[u].x);
-            const float resc = mx == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mx - cm);
-            acc.x *= resc; acc.y *= resc;
-            wsum *= resc;
-            mx = cm;
+                for (int e = 0; e < 8; ++e) {
+                    const int key = kt + 8 * quad + e;
+                    const bool ok = row_ok && key <= pos && key >= lo && key < kend;
+                    s[e] = ok ? s[e] : -INFINITY;
+                }
+            }
+            if (kt + 32 > seq_len || x.pg[u] < 0) {        // the request's last tile: slots past its end hold old scales
+                const int k8 = kt + 8 * quad, end = x.pg[u] < 0 ? 0 : seq_len;
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const float w = (b + u < ns && mlv[u].y > 0.f) ? mlv[u].y * __builtin_amdgcn_exp2f(mlv[u].x - mx) : 0.f;
-                acc.x += w * pv[u].x; acc.y += w * pv[u].y;
-                wsum += w;
+                for (int w = 0; w < 2; ++w) {
+                    uint32_t mk = 0;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) mk |= k8 + 4 * w + e < end ? 0xFFu << (8 * e) : 0u;
+#pragma unroll
+                    for (int i = 0; i < VS4; ++i) x.vs[u][i][w] &= mk;
+                }
+            }
+            uint32_t none = 0;
+#pragma unroll
+            for (int i = 0; i < VS4; ++i) none |= last_byte4(x.vs[u][i][0]) | last_byte4(x.vs[u][i][1]);
+            if (__any(none != 0)) {
+                // blocks that read as NaN: they become so in the rows that see them and in no other
+#pragma unroll
+                for (int i = 0; i < VS4; ++i)
+#pragma unroll
+                    for (int w = 0; w < 2; ++w)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (((x.vs[u][i][w] >> (8 * e)) & 255u) == 255u) x.vs[u][i][w] &= ~(255u << (8 * e));
+                const uint8_t* vsb = a.four.vs + (((size_t)x.pg[u] * a.Hk + kvh) * (size_t)(a.page_size >> 3) + ((kt & a.page_mask) >> 3)) * (NB4V * 8);
+                for (int e = 0; e < 32; ++e) {
+                    const int key = kt + e;
+                    if (!(row_ok && key <= pos && key >= lo && key < kend)) continue;
+#pragma unroll
+                    for (int d = 0; d < FDB; ++d)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            if (vsb[((e >> 3) * NB4V + (((4 * quad + r) * FDB + d) >> 5)) * 8 + (e & 7)] == 255) o[d][r] = __builtin_nanf("");
+                }
+            }
+            float mt = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7]))) * c2;
+            // (the reference moves only where a maximum is more than 2^MAX_SLACK above it: no exchange between lanes otherwise)
+            if (__any(mt > m + MAX_SLACK)) {
+                mt = fmaxf(mt, __shfl_xor(mt, 16, 64));
+                mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
+                const float mn = mt > m + MAX_SLACK ? mt : m;
+                const float corr = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
+                m = mn;
+                l *= corr;
+#pragma unroll
+                for (int d = 0; d < FDB; ++d)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[d][e] *= corr;
+            }
+            const float mu = m == -INFINITY ? 0.f : m;
+            float p[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                p[e] = __builtin_amdgcn_exp2f(fmaf(s[e], c2, -mu));
+                l += p[e];
+            }
+            const bf16x8 pf = as_bf16x8(make_uint4(pack2(p[0], p[1]), pack2(p[2], p[3]), pack2(p[4], p[5]), pack2(p[6], p[7])));
+#pragma unroll
+            for (int i = 0; i < VP4; ++i) {
+                u32x4_t even, odd;
+                values4(x.v[u][i], x.vs[u][VS4 == 1 ? 0 : i], even, odd);
+                o[2 * i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(frag(even), pf, o[2 * i], 0, 0, 0);
+                o[2 * i + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(frag(odd), pf, o[2 * i + 1], 0, 0, 0);
             }
         }
-        const int rr = row0 + r, tk = rr / G, hh = kvh * G + (rr - tk * G);
-        wsum = with_sink(a.sinks, hh, mx, wsum);
-        const float inv = (wsum > 0.f ? 1.0f / wsum : 0.f) * row_factor(a.gate, a.ld_gate, a.out_scale, q0 + tk, hh);
-        bf16_t* op = a.out + (size_t)(q0 + tk) * a.ld_out + hh * HV + d2;
-        *reinterpret_cast<uint32_t*>(op) = pack2(acc.x * inv, acc.y * inv);
-        return;
-    }
-    // More: 16 lanes a row weigh its ranges, 64 of them a turn, while a thread's pairs of channels are on their way, up to 64 loads.  (As above, a pair after
-    // the other, each with the weights anew: 6 trips for 16 rows of 192 channels.  A request of 500 keys, 16 heads over one of 256 x 192 21.6 us -> 13.3, of 128 x 128
-    // 11.3 -> 9.4, the streaming kernel and its merge 15.1 and 10.7; for 4 rows of 128 channels the way above is 0.6 us shorter.)
-    float* const weight = mo;                            // [FEW_ROWS][FEW_TURN]
-    float* const factor = mml;                           // [FEW_ROWS] what a turn's sums before it are multiplied by, then [FEW_ROWS] the results
-    const int wr = tid >> 4, wj = tid & 15;
-    const float* const ml = a.part_ml + (((size_t)s0 * a.Hk + kvh) * ROWS + (wr < n_rows ? wr : 0)) * 2;
-    const float* const po = a.part_o + ((size_t)s0 * a.Hk + kvh) * ROWS * HV;      // (a row block's rows lie one after the other)
-    constexpr int PB = FEW_PAIRS, U = 16;
-    for (int p0 = 0; p0 < total; p0 += PB * 64 * FEW_WAVES) {
-        float2 acc[PB];
-        int at[PB];
-#pragma unroll
-        for (int p = 0; p < PB; ++p) {
-            acc[p] = make_float2(0.f, 0.f);
-            at[p] = p0 + p * 64 * FEW_WAVES + tid < total ? p0 + p * 64 * FEW_WAVES + tid : 0;
-        }
-        float mx = -INFINITY, wsum = 0.f;
-        for (int g = 0; g < ns; g += FEW_TURN) {
-            const int n = ns - g < FEW_TURN ? ns - g : FEW_TURN;
-            const bool weigh = p0 == 0 || ns > FEW_TURN;
-            float2 mlv[FEW_TURN / 16], pv[PB][U];
-            if (weigh)
-#pragma unroll
-                for (int i = 0; i < FEW_TURN / 16; ++i)
-                    if (16 * i < n) mlv[i] = load_agent(ml + (g + (wj + 16 * i < n ? wj + 16 * i : 0)) * ml_step);
-            auto load = [&](int b) __attribute__((always_inline)) {
-#pragma unroll
-                for (int p = 0; p < PB; ++p)
-                    if (p0 + p * 64 * FEW_WAVES < total)
-#pragma unroll
-                        for (int e = 0; e < U; e += 8) {
-                            if (b + e < n) {
-#pragma unroll
-                                for (int u = e; u < e + 8; ++u) pv[p][u] = load_agent(po + (g + (b + u < n ? b + u : b)) * po_step + 2 * at[p]);
-                            } else {
-#pragma unroll
-                                for (int u = e; u < e + 8; ++u) pv[p][u] = make_float2(0.f, 0.f);
-                            }
-                        }
-            };
-            load(0);
+    };
+
+    const int n_steps = (kend - kbeg + FOUR_STEP - 1) / FOUR_STEP;
+    const int n = n_steps > wave ? (n_steps - wave + FEW_WAVES - 1) / FEW_WAVES : 0;
+    if (n > 0) {
+        FourTile x, y;
+        load(x, 0);
+        int j = 0;
+        for (; j + 2 < n; j += 2) {
+            load(y, j + 1);
             __builtin_amdgcn_sched_barrier(0);
-            if (weigh) {
-                float cm = mx, sum = 0.f;
-#pragma unroll
-                for (int i = 0; i < FEW_TURN / 16; ++i)
-                    if (wj + 16 * i < n) cm = fmaxf(cm, mlv[i].x);
-#pragma unroll
-                for (int o = 1; o < 16; o <<= 1) cm = fmaxf(cm, __shfl_xor(cm, o, 64));
-                const float before = mx == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mx - cm);
-                if (g > 0 || p0 > 0) __syncthreads();        // (the weights of the turn before are read)
-#pragma unroll
-                for (int i = 0; i < FEW_TURN / 16; ++i) {
-                    const float w = wj + 16 * i < n && mlv[i].y > 0.f ? mlv[i].y * __builtin_amdgcn_exp2f(mlv[i].x - cm) : 0.f;
-                    weight[wr * FEW_TURN + wj + 16 * i] = w;
-                    sum += w;
-                }
-#pragma unroll
-                for (int o = 1; o < 16; o <<= 1) sum += __shfl_xor(sum, o, 64);
-                wsum = wsum * before + sum;
-                mx = cm;
-                if (wj == 0) {
-                    factor[wr] = before;
-                    if (g + FEW_TURN >= ns && wr < n_rows) {
-                        const int rr = row0 + wr, tk = rr / G, hh = kvh * G + (rr - tk * G);
-                        const float all = with_sink(a.sinks, hh, mx, wsum);
-                        factor[FEW_ROWS + wr] = (all > 0.f ? 1.0f / all : 0.f) * row_factor(a.gate, a.ld_gate, a.out_scale, q0 + tk, hh);
-                    }
-                }
-                __syncthreads();
-            }
-            if (g > 0)
-#pragma unroll
-                for (int p = 0; p < PB; ++p) {
-                    const float f = factor[at[p] / (HV / 2)];
-                    acc[p].x *= f; acc[p].y *= f;
-                }
-            for (int b = 0; b < n; b += U) {
-                if (b > 0) load(b);
-#pragma unroll
-                for (int p = 0; p < PB; ++p)
-                    if (p0 + p * 64 * FEW_WAVES < total) {
-                        const float* const w = weight + at[p] / (HV / 2) * FEW_TURN + b;
-#pragma unroll
-                        for (int u = 0; u < U; ++u) {         // (weights past the last range are 0)
-                            acc[p].x += w[u] * pv[p][u].x; acc[p].y += w[u] * pv[p][u].y;
-                        }
-                    }
-            }
+            compute(x, j);
+            __builtin_amdgcn_sched_barrier(0);
+            load(x, j + 2);
+            __builtin_amdgcn_sched_barrier(0);
+            compute(y, j + 1);
+            __builtin_amdgcn_sched_barrier(0);
         }
-#pragma unroll
-        for (int p = 0; p < PB; ++p) {
-            if (p0 + p * 64 * FEW_WAVES + tid >= total) continue;
-            const int r = at[p] / (HV / 2), d2 = (at[p] - r * (HV / 2)) * 2;
-            const int rr = row0 + r, tk = rr / G, hh = kvh * G + (rr - tk * G);
-            const float inv = factor[FEW_ROWS + r];
-            bf16_t* op = a.out + (size_t)(q0 + tk) * a.ld_out + hh * HV + d2;
-            *reinterpret_cast<uint32_t*>(op) = pack2(acc[p].x * inv, acc[p].y * inv);
+        if (j + 1 < n) {
+            load(y, j + 1);
+            __builtin_amdgcn_sched_barrier(0);
+            compute(x, j);
+            compute(y, j + 1);
+        } else {
+            compute(x, j);
         }
     }
+    l += __shfl_xor(l, 16, 64);
+    l += __shfl_xor(l, 32, 64);                          // the row's sum from its four lanes
+    if (row_ok) {
+        float* dst = mo + (wave * FEW_ROWS + lr) * FEW_MS + quad * 4 * FDB;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+            for (int d = 0; d < FDB; d += 2) *reinterpret_cast<float2*>(dst + e * FDB + d) = make_float2(o[d][e], o[d + 1][e]);
+        if (quad == 0) {
+            mml[(wave * FEW_ROWS + lr) * 2] = m;
+            mml[(wave * FEW_ROWS + lr) * 2 + 1] = l;
+        }
+    }
+    few_finish(a, it, kvh, row0, slot, q0, q_len, G, mo, mml, &last_one);
     }
 }
 
@@ -1620,7 +1930,7 @@ extern "C" int xr_attention_mfma(void* out, const void* q, const void* k_cache, 
                "attention: blocks of few rows need heads in steps of 32, pages of at least 32 positions, a positive scale and counters");
     XR_REQUIRE(n_few == 0 || (((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache) & 15) == 0, "attention: queries and cache must be 16-byte aligned");
     if (n_items + n_cta_items + n_few == 0) return XR_OK;
-    AttnArgs a;
+    AttnArgs a = {};
     a.few_items = few_items; a.n_few = n_few; a.counters = counters;
     a.q = (const bf16_t*)q; a.kc = (const bf16_t*)k_cache; a.vc = (const bf16_t*)v_cache; a.out = (bf16_t*)out;
     // the list begins with the items of the workgroup kernel
@@ -1636,4 +1946,35 @@ extern "C" int xr_attention_mfma(void* out, const void* q, const void* k_cache, 
     if (cap > 0.f) return launch_mode<MODE_CAP>(a, jobs, n_jobs, cu_q, stream);
     if (slopes) return launch_mode<MODE_SLOPES>(a, jobs, n_jobs, cu_q, stream);
     return launch_mode<MODE_PLAIN>(a, jobs, n_jobs, cu_q, stream);
+}
+
+// Requests of few rows over a cache held in 4 bits (``few_items`` as in xr_attention_mfma).
+extern "C" int xr_attention_few4(void* out, const void* q, const void* kc, const void* ks, const void* vc, const void* vs, const int* few_items, int n_few,
+                                 int* counters, const int* block_table, int table_stride, float* part_o, float* part_ml, int H, int Hk, int D, int Dv,
+                                 int page_size, float scale, int window, int chunk, const float* slopes, const float* sinks, float cap, const float* gate,
+                                 int ld_gate, float out_scale, int ld_out, hipStream_t stream) {
+    XR_REQUIRE(D == HD && Dv == HV, "attention: this library is compiled for head size %d and value size %d, got %d and %d", HD, HV, D, Dv);
+    XR_REQUIRE(FOUR_OK, "attention: rows over 4-bit pages need keys and values of whole blocks of 32 channels, not %d and %d", D, Dv);
+    XR_REQUIRE(H > 0 && Hk > 0 && H % Hk == 0, "attention: %d query heads are not a multiple of %d key/value heads", H, Hk);
+    const int shift = ilog2_exact(page_size);
+    XR_REQUIRE(shift >= 5, "attention: rows over 4-bit pages need pages of a power of two of at least 32 positions, got %d", page_size);
+    XR_REQUIRE(window >= 0 && chunk >= 0 && scale > 0.f, "attention: window %d, chunk %d or scale %g", window, chunk, (double)scale);
+    XR_REQUIRE(cap >= 0.f && !(cap > 0.f && slopes), "attention: a soft cap %g of the scores needs no slopes", (double)cap);
+    XR_REQUIRE(ld_out >= H * HV && ld_out % 2 == 0 && ((uintptr_t)out % 4) == 0 && (!gate || ld_gate >= H), "attention: output rows %d apart (a gate's %d)", ld_out, ld_gate);
+    XR_REQUIRE(n_few >= 0 && (long long)n_few * Hk < (1LL << 31), "attention: %d blocks of few rows of %d key/value heads", n_few, Hk);
+    if (n_few == 0) return XR_OK;
+    XR_REQUIRE(out && q && kc && ks && vc && vs && few_items && counters && block_table, "attention: a null operand");
+    XR_REQUIRE((((uintptr_t)q | (uintptr_t)kc | (uintptr_t)vc) & 15) == 0 && (((uintptr_t)ks | (uintptr_t)vs) & 7) == 0, "attention: queries and codes must be 16-byte aligned, scales 8-byte");
+    AttnArgs a = {};
+    a.q = (const bf16_t*)q; a.out = (bf16_t*)out; a.few_items = few_items; a.n_few = n_few; a.counters = counters;
+    a.four = Pages4{(uint8_t*)kc, (uint8_t*)ks, (uint8_t*)vc, (uint8_t*)vs};
+    a.block_table = block_table; a.table_stride = table_stride; a.part_o = part_o; a.part_ml = part_ml; a.H = H; a.Hk = Hk;
+    a.page_shift = shift; a.page_mask = page_size - 1; a.page_size = page_size; a.scale = scale; a.window = window; a.chunk = chunk;
+    a.slopes = slopes; a.sinks = sinks; a.cap = cap; a.gate = gate; a.ld_gate = ld_gate; a.out_scale = out_scale; a.ld_out = ld_out;
+    const dim3 grid((unsigned)n_few * (unsigned)Hk);
+    if (cap > 0.f) k_attn_few4<MODE_CAP><<<grid, 64 * FEW_WAVES, 0, stream>>>(a);
+    else if (slopes) k_attn_few4<MODE_SLOPES><<<grid, 64 * FEW_WAVES, 0, stream>>>(a);
+    else k_attn_few4<MODE_PLAIN><<<grid, 64 * FEW_WAVES, 0, stream>>>(a);
+    XR_CHECK_LAUNCH("attention_few4");
+    return XR_OK;
 }

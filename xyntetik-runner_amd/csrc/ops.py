@@ -1049,8 +1049,9 @@ class Ops:
 
         bfloat16 runs on the matrix cores (head and value sizes in steps of 16 up to 256, pages of at least
         16 positions, a cap or slopes; kept first keys only where values have the keys' size); float32, and what the MFMA kernel does not take, runs the 32-bit kernel.
-        Caches that are ``FourBitPages`` are read back first (``read_pages``), but for steps that are being recorded, which a
-        32-bit kernel serves from the codes themselves.
+        Caches that are ``FourBitPages``: requests of up to 16 rows a key/value head are read from the codes by a matrix-core kernel of their
+        own (bfloat16, sizes in whole blocks of 32, pages of at least 32 positions, no kept first keys); the pages of others are read back
+        first (``read_pages``), but in steps that are being recorded, which a 32-bit kernel then serves from the codes.
         """
         positions, req_of_token, block_table = ctx.positions, ctx.req_of_token, ctx.block_table(group)
         self._dev(q, k_cache, v_cache, positions, req_of_token, block_table)
@@ -1083,6 +1084,30 @@ class Ops:
         if chunk and window:
             raise KernelError("attention: a layer reads a window or its chunk, not both")
         if four:
+            if self._few4_ok(q, out, ctx, D, Dv, page_size, scale, keep_first, softcap, slopes):
+                mask = Chunked(int(chunk)) if chunk else window
+                plan = ctx.attention_plan(group, H // Hk, mask, Hk, page_size, few_rows=2 if D + Dv <= 256 else 1, few_channels=D + Dv)
+                lib = self.attention_lib(D, Dv)
+                part_o = part_ml = None
+                if plan.n_slots:
+                    part_o = torch.empty((plan.n_slots, Hk, 32, Dv), dtype=torch.float32, device=q.device)
+                    part_ml = torch.empty((plan.n_slots, Hk, 32, 2), dtype=torch.float32, device=q.device)
+                if plan.n_few:
+                    lib.check(lib.xr_attention_few4(
+                        out.data_ptr(), q.data_ptr(), *pages[:4], plan.few.data_ptr(), plan.n_few, plan.counters.data_ptr(), block_table.data_ptr(),
+                        block_table.stride(0), _ptr(part_o), _ptr(part_ml), H, Hk, D, Dv, page_size, float(scale), int(window or 0), int(chunk or 0),
+                        _ptr(slopes), _ptr(sinks), float(softcap), *gating, _stream()))
+                if not plan.n_items and not plan.n_cta_items:
+                    return out
+                if getattr(ctx, "knows_lengths", False) and out.stride(0) % 4 == 0 and out.data_ptr() % 8 == 0:
+                    # requests of many rows: their pages once as 16-bit ones, which every row block then reads
+                    k16, v16, table = self.read_pages(k_cache, v_cache, ctx, group, q.dtype, plan.rest, window, chunk)
+                    lib.check(lib.xr_attention_mfma(
+                        out.data_ptr(), q.data_ptr(), k16.data_ptr(), v16.data_ptr(), plan.items.data_ptr(), plan.n_items, plan.n_cta_items, None, 0,
+                        None, _ptr(plan.jobs), plan.n_jobs, ctx.cu_q.data_ptr(), ctx.starts_dev.data_ptr(), table.data_ptr(), table.stride(0),
+                        _ptr(part_o), _ptr(part_ml), H, Hk, D, Dv, page_size, float(scale), int(window or 0), int(chunk or 0), _ptr(slopes),
+                        _ptr(sinks), float(softcap), *gating, _stream()))
+                    return out
             if not getattr(ctx, "knows_lengths", False):
                 self.lib.check(self.lib.xr_attention_any4(
                     out.data_ptr(), q.data_ptr(), *pages, positions.data_ptr(), req_of_token.data_ptr(), block_table.data_ptr(), block_table.stride(0),
@@ -1139,6 +1164,12 @@ class Ops:
                and not (q.data_ptr() | k_cache.data_ptr() | v_cache.data_ptr()) & 15)
         more = {**({"extra_slot": True} if extra else {}), **({"few_rows": 2 if D + Dv <= 256 else 1, "few_channels": D + Dv} if few else {})}
         return ctx.attention_plan(group, H // Hk, mask, Hk, page_size, **more)
+
+    def _few4_ok(self, q, out, ctx, D: int, Dv: int, page_size: int, scale: float, keep_first: int, softcap: float, slopes) -> bool:
+        """Whether the matrix-core kernel for few rows over 4-bit pages takes a call's operands."""
+        return (self.use_mfma and q.dtype == torch.bfloat16 and D % 32 == 0 and Dv % 32 == 0 and page_size >= 32 and scale > 0.0 and not keep_first
+                and not (softcap and slopes is not None) and getattr(ctx, "plans_few_rows", False) and q.data_ptr() % 16 == 0
+                and out.stride(0) % 2 == 0 and out.data_ptr() % 4 == 0)
 
     def attention_on_matrix_cores(self, dtype: torch.dtype, D: int, Dv: int, page_size: int = 64) -> bool:
         """Whether keys of ``D`` and values of ``Dv`` channels have matrix-core attention kernels."""
@@ -1225,7 +1256,8 @@ class Ops:
             unit = f"attn_d{D}" if D == Dv else f"attn_d{D}v{Dv}"
             path = _build.find_built(unit) or _build.build_unit(unit)
             lib = _Lib(path, {"xr_attention_mfma": [_p, _p, _p, _p, _p, _i, _i, _p, _i, _p, _p, _i, _p, _p, _p, _i, _p, _p,
-                                                    _i, _i, _i, _i, _i, _f, _i, _i, _p, _p, _f, _p, _i, _f, _i, _p]})
+                                                    _i, _i, _i, _i, _i, _f, _i, _i, _p, _p, _f, _p, _i, _f, _i, _p],
+                              "xr_attention_few4": [_p] * 7 + [_i, _p, _p, _i, _p, _p] + [_i] * 5 + [_f, _i, _i, _p, _p, _f, _p, _i, _f, _i, _p]})
             self._attn_libs[(D, Dv)] = lib
         return lib
 

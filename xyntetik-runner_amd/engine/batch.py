@@ -47,6 +47,7 @@ class AttentionPlan:
     few: Optional[torch.Tensor] = None         # [n_few, 12]: blocks of up to 16 rows (see ``few_row_items``)
     n_few: int = 0
     counters: Optional[torch.Tensor] = None    # [row blocks of few rows x key/value heads], zero between launches
+    rest: tuple = ()                           # the step's requests that are not among those of few rows
 
 
 def first_key(mask, pos: int) -> int:
@@ -406,7 +407,8 @@ class StepContext:
             nf = nx + len(extras) * 8
             plan = AttentionPlan(dev[:nw], ni, dev[nw:nx] if nj else None, nj, n_slots, nc,
                                  dev[nx:nf] if extras else None, len(extras),
-                                 dev[nf:nf + n_few * FEW_INTS] if n_few else None, n_few, dev[nf + n_few * FEW_INTS:] if n_few else None)
+                                 dev[nf:nf + n_few * FEW_INTS] if n_few else None, n_few, dev[nf + n_few * FEW_INTS:] if n_few else None,
+                                 tuple(b for b in range(len(self.q_lens)) if b not in few))
             plan._host = host
             self._plans[key] = plan
         return plan
