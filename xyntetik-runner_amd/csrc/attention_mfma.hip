@@ -1113,7 +1113,7 @@ __device__ __forceinline__ float2 load_agent(const float* p) {
 // The end of a kernel for few rows: every wave has left its rows' unnormalised outputs in `mo`, their references and sums in `mml`; they are combined
 // here (sum_w 2^(m_w - max) O_w over sum_w 2^(m_w - max) l_w), and the row block's key ranges added up.
 constexpr int FEW_MS = HV + 4;                                // floats between rows of the combining buffer
-__device__ __forceinline__ void few_finish(const AttnArgs& a, const int* it, int kvh, int row0, int slot, int q0, int q_len, int G, float* mo, float* mml,
+template <int PB> __device__ __forceinline__ void few_finish(const AttnArgs& a, const int* it, int kvh, int row0, int slot, int q0, int q_len, int G, float* mo, float* mml,
                                            int* last_one) {
     constexpr int MS = FEW_MS;
     const int tid = threadIdx.x;
@@ -1211,7 +1211,7 @@ __device__ __forceinline__ void few_finish(const AttnArgs& a, const int* it, int
     const int wr = tid >> 4, wj = tid & 15;
     const float* const ml = a.part_ml + (((size_t)s0 * a.Hk + kvh) * ROWS + (wr < n_rows ? wr : 0)) * 2;
     const float* const po = a.part_o + ((size_t)s0 * a.Hk + kvh) * ROWS * HV;      // (a row block's rows lie one after the other)
-    constexpr int PB = FEW_PAIRS, U = 16;
+    constexpr int U = 16;
     for (int p0 = 0; p0 < total; p0 += PB * 64 * FEW_WAVES) {
         float2 acc[PB];
         int at[PB];
@@ -1490,7 +1490,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES, FEW_PER_CU) void k_attn_few(AttnArg
             mml[(wave * FEW_ROWS + lr) * 2 + 1] = l;
         }
     }
-    few_finish(a, it, kvh, row0, slot, q0, q_len, G, mo, mml, &last_one);
+    few_finish<FEW_PAIRS>(a, it, kvh, row0, slot, q0, q_len, G, mo, mml, &last_one);
     }
 }
 
@@ -1510,14 +1510,14 @@ constexpr int NB4K = HD / 32, NB4V = FOUR_OK ? HV / 32 : 1;              // bloc
 constexpr int KS4 = FKD % 4 == 0 ? FKD / 4 : 4 % FKD == 0 ? 1 : FKD;      // scales of a lane's share of a key: of whole blocks, of a part of one, or word by word
 constexpr int VP4 = FDB >= 2 ? FDB / 2 : 1;                               // pairs of channels of a lane
 constexpr int VS4 = 32 % FDB == 0 ? 1 : VP4;                              // scales of its values: one, or pair by pair
-constexpr int FOUR_SUBS = HD + HV <= 256 ? 2 : 1;
-constexpr int FOUR_STEP = 32 * FOUR_SUBS;
+constexpr int FOUR_PER_CU = HD + HV <= 256 ? 3 : 2;
+constexpr int FOUR_PAIRS = FEW_PAIRS < 2 ? FEW_PAIRS : 2;
 typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
 
 struct FourTile {
-    uint32_t k[FOUR_SUBS][2][FKD];
-    u32x2_t ks[FOUR_SUBS][KS4], v[FOUR_SUBS][VP4], vs[FOUR_SUBS][VS4];
-    int pg[FOUR_SUBS];
+    uint32_t k[2][FKD];
+    u32x2_t ks[KS4], v[VP4], vs[VS4];
+    int pg;
 };
 
 // N words from where they lie side by side, in as few loads as their alignment (a multiple of N * 4 bytes, or of 4) allows
@@ -1560,7 +1560,7 @@ __device__ __forceinline__ void values4(u32x2_t codes, u32x2_t s, u32x4_t& even,
 }
 
 template <int MODE, bool OK = FOUR_OK>
-__global__ __launch_bounds__(64 * FEW_WAVES, FEW_PER_CU) void k_attn_few4(AttnArgs a) {
+__global__ __launch_bounds__(64 * FEW_WAVES, FOUR_PER_CU) void k_attn_few4(AttnArgs a) {
     if constexpr (OK) {
     __shared__ float mo[FEW_WAVES * FEW_ROWS * FEW_MS];
     __shared__ float mml[FEW_WAVES * FEW_ROWS * 2];
@@ -1615,34 +1615,30 @@ __global__ __launch_bounds__(64 * FEW_WAVES, FEW_PER_CU) void k_attn_few4(AttnAr
     const uint32_t kturn = (uint32_t)((8 * (lr & 3) + 9) & 31);            // what brings the byte of the lane's key to a scale's exponent
 
     auto load = [&](FourTile& x, int j) __attribute__((always_inline)) {
-        const int k0 = kbeg + (wave + j * FEW_WAVES) * FOUR_STEP;
-        if (((k0 + FOUR_STEP - 1) >> a.page_shift) - pages_base >= 64) {
-            pages_base = k0 >> a.page_shift;
+        const int kt = kbeg + (wave + j * FEW_WAVES) * 32;
+        if ((kt >> a.page_shift) - pages_base >= 64) {
+            pages_base = kt >> a.page_shift;
             look_up();
         }
+        const int pg = __builtin_amdgcn_readlane(my_page, __builtin_amdgcn_readfirstlane((kt >> a.page_shift) - pages_base));
+        x.pg = pg;
+        const size_t pb = (size_t)(pg < 0 ? 0 : pg) * a.Hk + kvh;
+        const int ko = kt & a.page_mask;
+        const size_t octet = pb * (size_t)(a.page_size >> 3) + (ko >> 3);
+        const uint8_t* kb = a.four.kc + (pb * a.page_size + ko) * (size_t)(HD / 2);
+        const uint8_t* ksb = a.four.ks + octet * (NB4K * 8);
+        const uint8_t* vb = a.four.vc + octet * (HV / 2 * 8);
+        const uint8_t* vsb = a.four.vs + octet * (NB4V * 8);
 #pragma unroll
-        for (int u = 0; u < FOUR_SUBS; ++u) {
-            const int kt = k0 + 32 * u;
-            const int pg = __builtin_amdgcn_readlane(my_page, __builtin_amdgcn_readfirstlane((kt >> a.page_shift) - pages_base));
-            x.pg[u] = pg;
-            const size_t pb = (size_t)(pg < 0 ? 0 : pg) * a.Hk + kvh;
-            const int ko = kt & a.page_mask;
-            const size_t octet = pb * (size_t)(a.page_size >> 3) + (ko >> 3);
-            const uint8_t* kb = a.four.kc + (pb * a.page_size + ko) * (size_t)(HD / 2);
-            const uint8_t* ksb = a.four.ks + octet * (NB4K * 8);
-            const uint8_t* vb = a.four.vc + octet * (HV / 2 * 8);
-            const uint8_t* vsb = a.four.vs + octet * (NB4V * 8);
+        for (int b = 0; b < 2; ++b) load_words<FKD>(x.k[b], kb + (koff + (uint32_t)(b * 4 * (HD / 2))));
 #pragma unroll
-            for (int b = 0; b < 2; ++b) load_words<FKD>(x.k[u][b], kb + (koff + (uint32_t)(b * 4 * (HD / 2))));
+        for (int i = 0; i < KS4; ++i) x.ks[i] = *reinterpret_cast<const u32x2_t*>(ksb + ksoff[i]);
+        uint32_t w[2 * VP4];
+        load_words<2 * VP4>(w, vb + voff);
 #pragma unroll
-            for (int i = 0; i < KS4; ++i) x.ks[u][i] = *reinterpret_cast<const u32x2_t*>(ksb + ksoff[i]);
-            uint32_t w[2 * VP4];
-            load_words<2 * VP4>(w, vb + voff);
+        for (int p = 0; p < VP4; ++p) { x.v[p][0] = w[2 * p]; x.v[p][1] = w[2 * p + 1]; }
 #pragma unroll
-            for (int p = 0; p < VP4; ++p) { x.v[u][p][0] = w[2 * p]; x.v[u][p][1] = w[2 * p + 1]; }
-#pragma unroll
-            for (int i = 0; i < VS4; ++i) x.vs[u][i] = *reinterpret_cast<const u32x2_t*>(vsb + vsoff[i]);
-        }
+        for (int i = 0; i < VS4; ++i) x.vs[i] = *reinterpret_cast<const u32x2_t*>(vsb + vsoff[i]);
     };
 
     f32x4 o[FDB];
@@ -1655,102 +1651,98 @@ __global__ __launch_bounds__(64 * FEW_WAVES, FEW_PER_CU) void k_attn_few4(AttnAr
     const SoftCap cap(a.scale, a.cap);
 
     auto compute = [&](FourTile& x, int j) __attribute__((always_inline)) {
+        const int kt = kbeg + (wave + j * FEW_WAVES) * 32;
+        float s[8];
 #pragma unroll
-        for (int u = 0; u < FOUR_SUBS; ++u) {
-            const int kt = kbeg + (wave + j * FEW_WAVES) * FOUR_STEP + 32 * u;
-            if (FOUR_SUBS > 1 && u > 0 && kt >= kend) break;
-            float s[8];
+        for (int b = 0; b < 2; ++b) {
+            f32x4 z;
 #pragma unroll
-            for (int b = 0; b < 2; ++b) {
-                f32x4 z;
+            for (int e = 0; e < 4; ++e) z[e] = MODE == MODE_SLOPES ? sb * (float)(kt + 8 * quad + 4 * b + e - pos) : 0.f;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) z[e] = MODE == MODE_SLOPES ? sb * (float)(kt + 8 * quad + 4 * b + e - pos) : 0.f;
-#pragma unroll
-                for (int kd = 0; kd < FKD; ++kd) {
-                    const uint32_t c = x.k[u][b][kd], ss = x.ks[u][FKD % 4 == 0 ? kd / 4 : KS4 == 1 ? 0 : kd][b];
-                    const uint32_t sc = __builtin_amdgcn_alignbit(ss, ss, kturn);
-                    const bf16x8 kf = as_bf16x8(make_uint4(pair4_bf16<0>(c, sc), pair4_bf16<1>(c, sc), pair4_bf16<2>(c, sc), pair4_bf16<3>(c, sc)));
-                    z = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[kd], z, 0, 0, 0);
-                }
-#pragma unroll
-                for (int e = 0; e < 4; ++e) s[4 * b + e] = MODE == MODE_CAP ? cap.less(z[e], 0.f) : z[e];
+            for (int kd = 0; kd < FKD; ++kd) {
+                const uint32_t c = x.k[b][kd], ss = x.ks[FKD % 4 == 0 ? kd / 4 : KS4 == 1 ? 0 : kd][b];
+                const uint32_t sc = __builtin_amdgcn_alignbit(ss, ss, kturn);
+                const bf16x8 kf = as_bf16x8(make_uint4(pair4_bf16<0>(c, sc), pair4_bf16<1>(c, sc), pair4_bf16<2>(c, sc), pair4_bf16<3>(c, sc)));
+                z = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[kd], z, 0, 0, 0);
             }
-            const bool whole = kt + 32 <= kend && kt + 31 <= pos_min && kt >= lo_max;
-            if (!whole) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const int key = kt + 8 * quad + e;
-                    const bool ok = row_ok && key <= pos && key >= lo && key < kend;
-                    s[e] = ok ? s[e] : -INFINITY;
-                }
+            for (int e = 0; e < 4; ++e) s[4 * b + e] = MODE == MODE_CAP ? cap.less(z[e], 0.f) : z[e];
+        }
+        const bool whole = kt + 32 <= kend && kt + 31 <= pos_min && kt >= lo_max;
+        if (!whole) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int key = kt + 8 * quad + e;
+                const bool ok = row_ok && key <= pos && key >= lo && key < kend;
+                s[e] = ok ? s[e] : -INFINITY;
             }
-            if (kt + 32 > seq_len || x.pg[u] < 0) {        // the request's last tile: slots past its end hold old scales
-                const int k8 = kt + 8 * quad, end = x.pg[u] < 0 ? 0 : seq_len;
+        }
+        if (kt + 32 > seq_len || x.pg < 0) {        // the request's last tile: slots past its end hold old scales
+            const int k8 = kt + 8 * quad, end = x.pg < 0 ? 0 : seq_len;
 #pragma unroll
-                for (int w = 0; w < 2; ++w) {
-                    uint32_t mk = 0;
+            for (int w = 0; w < 2; ++w) {
+                uint32_t mk = 0;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) mk |= k8 + 4 * w + e < end ? 0xFFu << (8 * e) : 0u;
+                for (int e = 0; e < 4; ++e) mk |= k8 + 4 * w + e < end ? 0xFFu << (8 * e) : 0u;
 #pragma unroll
-                    for (int i = 0; i < VS4; ++i) x.vs[u][i][w] &= mk;
-                }
+                for (int i = 0; i < VS4; ++i) x.vs[i][w] &= mk;
             }
-            uint32_t none = 0;
+        }
+        uint32_t none = 0;
 #pragma unroll
-            for (int i = 0; i < VS4; ++i) none |= last_byte4(x.vs[u][i][0]) | last_byte4(x.vs[u][i][1]);
-            if (__any(none != 0)) {
-                // blocks that read as NaN: they become so in the rows that see them and in no other
+        for (int i = 0; i < VS4; ++i) none |= last_byte4(x.vs[i][0]) | last_byte4(x.vs[i][1]);
+        if (__any(none != 0)) {
+            // blocks that read as NaN: they become so in the rows that see them and in no other
 #pragma unroll
-                for (int i = 0; i < VS4; ++i)
+            for (int i = 0; i < VS4; ++i)
 #pragma unroll
-                    for (int w = 0; w < 2; ++w)
+                for (int w = 0; w < 2; ++w)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            if (((x.vs[u][i][w] >> (8 * e)) & 255u) == 255u) x.vs[u][i][w] &= ~(255u << (8 * e));
-                const uint8_t* vsb = a.four.vs + (((size_t)x.pg[u] * a.Hk + kvh) * (size_t)(a.page_size >> 3) + ((kt & a.page_mask) >> 3)) * (NB4V * 8);
-                for (int e = 0; e < 32; ++e) {
-                    const int key = kt + e;
-                    if (!(row_ok && key <= pos && key >= lo && key < kend)) continue;
-#pragma unroll
-                    for (int d = 0; d < FDB; ++d)
-#pragma unroll
-                        for (int r = 0; r < 4; ++r)
-                            if (vsb[((e >> 3) * NB4V + (((4 * quad + r) * FDB + d) >> 5)) * 8 + (e & 7)] == 255) o[d][r] = __builtin_nanf("");
-                }
-            }
-            float mt = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7]))) * c2;
-            // (the reference moves only where a maximum is more than 2^MAX_SLACK above it: no exchange between lanes otherwise)
-            if (__any(mt > m + MAX_SLACK)) {
-                mt = fmaxf(mt, __shfl_xor(mt, 16, 64));
-                mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
-                const float mn = mt > m + MAX_SLACK ? mt : m;
-                const float corr = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
-                m = mn;
-                l *= corr;
+                    for (int e = 0; e < 4; ++e)
+                        if (((x.vs[i][w] >> (8 * e)) & 255u) == 255u) x.vs[i][w] &= ~(255u << (8 * e));
+            const uint8_t* vsb = a.four.vs + (((size_t)x.pg * a.Hk + kvh) * (size_t)(a.page_size >> 3) + ((kt & a.page_mask) >> 3)) * (NB4V * 8);
+            for (int e = 0; e < 32; ++e) {
+                const int key = kt + e;
+                if (!(row_ok && key <= pos && key >= lo && key < kend)) continue;
 #pragma unroll
                 for (int d = 0; d < FDB; ++d)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) o[d][e] *= corr;
+                    for (int r = 0; r < 4; ++r)
+                        if (vsb[((e >> 3) * NB4V + (((4 * quad + r) * FDB + d) >> 5)) * 8 + (e & 7)] == 255) o[d][r] = __builtin_nanf("");
             }
-            const float mu = m == -INFINITY ? 0.f : m;
-            float p[8];
+        }
+        float mt = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7]))) * c2;
+        // (the reference moves only where a maximum is more than 2^MAX_SLACK above it: no exchange between lanes otherwise)
+        if (__any(mt > m + MAX_SLACK)) {
+            mt = fmaxf(mt, __shfl_xor(mt, 16, 64));
+            mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
+            const float mn = mt > m + MAX_SLACK ? mt : m;
+            const float corr = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
+            m = mn;
+            l *= corr;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                p[e] = __builtin_amdgcn_exp2f(fmaf(s[e], c2, -mu));
-                l += p[e];
-            }
-            const bf16x8 pf = as_bf16x8(make_uint4(pack2(p[0], p[1]), pack2(p[2], p[3]), pack2(p[4], p[5]), pack2(p[6], p[7])));
+            for (int d = 0; d < FDB; ++d)
 #pragma unroll
-            for (int i = 0; i < VP4; ++i) {
-                u32x4_t even, odd;
-                values4(x.v[u][i], x.vs[u][VS4 == 1 ? 0 : i], even, odd);
-                o[2 * i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(frag(even), pf, o[2 * i], 0, 0, 0);
-                o[2 * i + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(frag(odd), pf, o[2 * i + 1], 0, 0, 0);
-            }
+                for (int e = 0; e < 4; ++e) o[d][e] *= corr;
+        }
+        const float mu = m == -INFINITY ? 0.f : m;
+        float p[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            p[e] = __builtin_amdgcn_exp2f(fmaf(s[e], c2, -mu));
+            l += p[e];
+        }
+        const bf16x8 pf = as_bf16x8(make_uint4(pack2(p[0], p[1]), pack2(p[2], p[3]), pack2(p[4], p[5]), pack2(p[6], p[7])));
+#pragma unroll
+        for (int i = 0; i < VP4; ++i) {
+            u32x4_t even, odd;
+            values4(x.v[i], x.vs[VS4 == 1 ? 0 : i], even, odd);
+            o[2 * i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(frag(even), pf, o[2 * i], 0, 0, 0);
+            o[2 * i + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(frag(odd), pf, o[2 * i + 1], 0, 0, 0);
         }
     };
 
-    const int n_steps = (kend - kbeg + FOUR_STEP - 1) / FOUR_STEP;
+    const int n_steps = (kend - kbeg + 31) / 32;
     const int n = n_steps > wave ? (n_steps - wave + FEW_WAVES - 1) / FEW_WAVES : 0;
     if (n > 0) {
         FourTile x, y;
@@ -1788,7 +1780,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES, FEW_PER_CU) void k_attn_few4(AttnAr
             mml[(wave * FEW_ROWS + lr) * 2 + 1] = l;
         }
     }
-    few_finish(a, it, kvh, row0, slot, q0, q_len, G, mo, mml, &last_one);
+    few_finish<FOUR_PAIRS>(a, it, kvh, row0, slot, q0, q_len, G, mo, mml, &last_one);
     }
 }
 

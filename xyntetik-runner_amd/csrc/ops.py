@@ -1086,7 +1086,8 @@ class Ops:
         if four:
             if self._few4_ok(q, out, ctx, D, Dv, page_size, scale, keep_first, softcap, slopes):
                 mask = Chunked(int(chunk)) if chunk else window
-                plan = ctx.attention_plan(group, H // Hk, mask, Hk, page_size, few_rows=2 if D + Dv <= 256 else 1, few_channels=D + Dv)
+                plan = ctx.attention_plan(group, H // Hk, mask, Hk, page_size, few_rows=2 if D + Dv <= 256 else 1, few_channels=D + Dv,
+                                          most_rows=self.FOUR_ROWS)
                 lib = self.attention_lib(D, Dv)
                 part_o = part_ml = None
                 if plan.n_slots:
@@ -1164,6 +1165,8 @@ class Ops:
                and not (q.data_ptr() | k_cache.data_ptr() | v_cache.data_ptr()) & 15)
         more = {**({"extra_slot": True} if extra else {}), **({"few_rows": 2 if D + Dv <= 256 else 1, "few_channels": D + Dv} if few else {})}
         return ctx.attention_plan(group, H // Hk, mask, Hk, page_size, **more)
+
+    FOUR_ROWS = 64          # rows a key/value head that a request over 4-bit pages has at most to be served from the codes, 16 at a time
 
     def _few4_ok(self, q, out, ctx, D: int, Dv: int, page_size: int, scale: float, keep_first: int, softcap: float, slopes) -> bool:
         """Whether the matrix-core kernel for few rows over 4-bit pages takes a call's operands."""

@@ -222,9 +222,10 @@ def few_row_least(tiles: int, rows: int, channels: int = 256) -> int:
     return max(FEW_MIN_RANGE, -(-tiles // most))
 
 
-def few_row_items(req, starts, lens, q0s, mask, room: int, extra_slot: bool, first_slot: int = 0, pair_at: int = 0, least=None):
+def few_row_items(req, starts, lens, q0s, mask, room: int, extra_slot: bool, first_slot: int = 0, pair_at: int = 0, least=None,
+                  row0s=None, group_size: int = 1):
     """The work of the kernel for few rows: requests ``req`` of a step, each with one row block (its ``lens[i]`` tokens from row
-    ``q0s[i]`` and position ``starts[i]`` on), cut into at most ``room`` key ranges of about one length, so that a
+    ``q0s[i]`` and position ``starts[i]`` on; with ``row0s`` an entry is the block of 16 rows from ``row0s[i]`` on, tokens x heads of a group of ``group_size``), cut into at most ``room`` key ranges of about one length, so that a
     long request takes as many workgroups as its keys are worth: ``(items [n, 12], extras [len(req), 8], slots)`` as int64 arrays.
 
     An item: request, 0, first key, end key, partial slot (-1: all its keys), the request's first row, its tokens, its first
@@ -237,9 +238,12 @@ def few_row_items(req, starts, lens, q0s, mask, room: int, extra_slot: bool, fir
     a unit has a long and a short one (64 requests of 950 to 1,900 keys 71.3 us -> 68.8, of 100 to 4,000 117.8 -> 96.8; 48 of 950 to 1,900 65.6 -> 57.8)."""
     starts, lens = np.asarray(starts, dtype=np.int64), np.asarray(lens, dtype=np.int64)
     n = len(starts)
-    hi = starts + lens
+    hi, at = starts + lens, starts
+    if row0s is not None:
+        row0s = np.asarray(row0s, dtype=np.int64)
+        hi, at = starts + np.minimum(lens, (row0s + FEW_ROWS - 1) // group_size + 1), starts + row0s // group_size
     if mask:
-        lo = starts - starts % mask.size if isinstance(mask, Chunked) else np.maximum(0, starts - mask + 1)
+        lo = at - at % mask.size if isinstance(mask, Chunked) else np.maximum(0, at - mask + 1)
         lo = lo // ATTN_TILE * ATTN_TILE
     else:
         lo = 0
@@ -277,9 +281,11 @@ def few_row_items(req, starts, lens, q0s, mask, room: int, extra_slot: bool, fir
         items[:, 2] += k * items[:, 1]
         items[:, 3] = np.minimum(items[:, 3], items[:, 2] + items[:, 1])
         items[:, 4] = np.where(items[:, 9] > 0, items[:, 8] + k, -1)
-        items[:, 1] = 0
+        items[:, 1] = 0 if row0s is None else np.repeat(row0s[order], parts)
     else:
         rec[:, 4], rec[:, 11] = -1, 1
+        if row0s is not None:
+            rec[:, 1] = row0s
         items = rec[np.argsort(-tiles, kind="stable")]
     if 0 < pair_at < len(items) <= 2 * pair_at:
         items[pair_at:] = items[pair_at:][::-1].copy()
@@ -373,14 +379,14 @@ class StepContext:
         self.shared = {}        # what parts make once a step and share between layers (a rotation's table)
 
     def attention_plan(self, group: int, group_size: int, window, n_kv_heads: int,
-                       page_size: int = 64, extra_slot: bool = False, few_rows: int = 0, few_channels: int = 256) -> AttentionPlan:
+                       page_size: int = 64, extra_slot: bool = False, few_rows: int = 0, few_channels: int = 256, most_rows: int = FEW_ROWS) -> AttentionPlan:
         """The MFMA attention work list, made once per step and shared by all layers that can.  ``few_rows`` > 0:
-        requests of up to 16 rows a key/value head go to the kernel for few rows (where the page size allows), of which a compute unit
+        requests of up to ``most_rows`` rows a key/value head go to the kernel for few rows (where the page size allows), 16 of them a row block, of which a compute unit
         holds so many workgroups; ``few_channels``: those of a key and its value together."""
-        key = (group_size, window, n_kv_heads, page_size, extra_slot, few_rows, few_channels)
+        key = (group_size, window, n_kv_heads, page_size, extra_slot, few_rows, few_channels, most_rows)
         plan = self._plans.get(key)
         if plan is None:
-            few = [b for b, n in enumerate(self.q_lens) if few_rows and page_size >= FEW_PAGE and n * group_size <= FEW_ROWS]
+            few = [b for b, n in enumerate(self.q_lens) if few_rows and page_size >= FEW_PAGE and n * group_size <= most_rows]
             planned = plan_attention(self.starts, self.q_lens, group_size, window, n_kv_heads, page_size,
                                      extra_slot=extra_slot, skip=frozenset(few))
             cta_items, items, jobs, n_slots = planned[:4]
@@ -388,13 +394,17 @@ class StepContext:
             flat = [v for it in cta_items + items for v in it] + [v for j in jobs for v in j]
             n_few = n_count = 0
             if few:
-                q0s = np.concatenate([[0], np.cumsum(self.q_lens)])[few]
-                room = max(len(few), FEW_SLOTS // n_kv_heads)
-                few_items, few_extras, more = few_row_items(few, [self.starts[b] for b in few], [self.q_lens[b] for b in few], q0s,
+                blocks = [(b, row0) for b in few for row0 in range(0, self.q_lens[b] * group_size, FEW_ROWS)]
+                of = [b for b, _ in blocks]
+                q0s = np.concatenate([[0], np.cumsum(self.q_lens)])[of]
+                room = max(len(blocks), FEW_SLOTS // n_kv_heads)
+                rows = min(FEW_ROWS, group_size * max(self.q_lens[b] for b in few))
+                few_items, few_extras, more = few_row_items(of, [self.starts[b] for b in of], [self.q_lens[b] for b in of], q0s,
                                                             window, room, extra_slot, n_slots, ATTN_STREAM_SLOTS // n_kv_heads if few_rows == 2 else 0,
-                                                            least=lambda t: few_row_least(t, group_size * max(self.q_lens[b] for b in few), few_channels))
+                                                            least=lambda t: few_row_least(t, rows, few_channels),
+                                                            row0s=[r for _, r in blocks] if len(blocks) > len(few) else None, group_size=group_size)
                 n_slots += more
-                n_few, n_count = len(few_items), len(few) * n_kv_heads
+                n_few, n_count = len(few_items), len(blocks) * n_kv_heads
                 extras += few_extras.tolist()
             flat += [v for x in extras for v in x]
             if few:

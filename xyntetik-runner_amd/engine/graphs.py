@@ -60,6 +60,11 @@ def most_tiles(batch_cap: int, n_splits: int, n_kv_heads: int, table_tiles: int)
     return table_tiles if splits_for(batch_cap, end, n_kv_heads) == n_splits else min(end - 1, table_tiles)
 
 
+def few_blocks(group_size: int) -> int:
+    """Row blocks of the kernel for few rows that a request's one token fills."""
+    return -(-group_size // FEW_ROWS)
+
+
 def few_row_room(batch_cap: int, tiles: int, n_kv_heads: int) -> int:
     """Items that a recorded step keeps for the kernel for few rows: one a request, and as many key ranges as fill the kernel's workgroups beside the
     rows that pad the batch (fewer than half of it, an item each), but no more than ranges of the shortest length (and one for what the requests' last ranges lack).
@@ -108,7 +113,7 @@ class StaticDecodeContext:
 
     def _alloc(self) -> None:
         B = self.B
-        n_plan = sum((self._plan_splits[k] * FEW_INTS + B * k[2] if k[4] else B * self._plan_splits[k] * 8 + B * 7) + (B * 8 if k[3] else 0)
+        n_plan = sum((self._plan_splits[k] * FEW_INTS + B * few_blocks(k[0]) * k[2] if k[4] else B * self._plan_splits[k] * 8 + B * 7) + (B * 8 if k[3] else 0)
                      for k in self._plan_keys)
         offs = np.concatenate([[0], np.cumsum(self._sizes)]).astype(np.int64)
         total = int(offs[-1]) + n_plan
@@ -131,10 +136,10 @@ class StaticDecodeContext:
             S = self._plan_splits[k]
             self._plan_off[k] = base
             if k[4]:
-                n_items, n_count, n_extra = S * FEW_INTS, B * k[2], B * 8 if k[3] else 0
+                n_items, n_count, n_extra = S * FEW_INTS, B * few_blocks(k[0]) * k[2], B * 8 if k[3] else 0
                 few, counters = d[base:base + n_items], d[base + n_items:base + n_items + n_count]
                 extras = d[base + n_items + n_count:base + n_items + n_count + n_extra] if n_extra else None
-                self._plans[k] = AttentionPlan(few[:0], 0, None, 0, S + (B if n_extra else 0) if S > B or n_extra else 0, 0,
+                self._plans[k] = AttentionPlan(few[:0], 0, None, 0, S + (B if n_extra else 0) if S > B * few_blocks(k[0]) or n_extra else 0, 0,
                                                extras, B if n_extra else 0, few, S, counters)
                 base += n_items + n_count + n_extra
                 continue
@@ -158,8 +163,8 @@ class StaticDecodeContext:
                            "ctx.slots (on the device), or sets capturable = False to be run eagerly")
 
     def attention_plan(self, group: int, group_size: int, window, n_kv_heads: int,
-                       page_size: int = 64, extra_slot: bool = False, few_rows: int = 0, few_channels: int = 256) -> AttentionPlan:
-        few = few_rows if page_size >= FEW_PAGE and group_size <= FEW_ROWS else 0
+                       page_size: int = 64, extra_slot: bool = False, few_rows: int = 0, few_channels: int = 256, most_rows: int = FEW_ROWS) -> AttentionPlan:
+        few = few_rows if page_size >= FEW_PAGE and group_size <= most_rows else 0
         key = (group_size, window, n_kv_heads, bool(extra_slot), few, few_channels if few else 0)
         if key not in self._plans:
             if torch.cuda.is_current_stream_capturing():
@@ -168,7 +173,7 @@ class StaticDecodeContext:
             if tiles is not None and window:
                 tiles = min(tiles, -(-mask_reach(window) // ATTN_TILE) + 1)
             if few:
-                self._plan_splits[key] = few_row_room(self.B, tiles if tiles is not None else self.S * FEW_MIN_RANGE, n_kv_heads)
+                self._plan_splits[key] = few_row_room(self.B * few_blocks(group_size), tiles if tiles is not None else self.S * FEW_MIN_RANGE, n_kv_heads)
             else:
                 self._plan_splits[key] = self.S if tiles is None else min(self.S, splits_for(self.B, tiles, n_kv_heads))
             self._plan_keys.append(key)
@@ -242,13 +247,16 @@ class StaticDecodeContext:
         B, S = self.B, self._plan_splits[key]
         if few:
             # (rows that pad the batch have an item each, and leave the requests all the workgroups)
-            got, extras, _ = few_row_items(np.arange(B), starts, np.ones(B, dtype=np.int64), np.arange(B), window, min(S, max(B, FEW_SLOTS // n_kv_heads + B - n)), extra,
-                                           pair_at=ATTN_STREAM_SLOTS // n_kv_heads if few == 2 else 0, least=lambda t: few_row_least(t, group_size, few_channels))
+            nb = few_blocks(group_size)
+            of = np.repeat(np.arange(B), nb)
+            got, extras, _ = few_row_items(of, starts[of], np.ones(B * nb, dtype=np.int64), of, window, min(S, max(B * nb, FEW_SLOTS // n_kv_heads + (B - n) * nb)), extra,
+                                           pair_at=ATTN_STREAM_SLOTS // n_kv_heads if few == 2 else 0, least=lambda t: few_row_least(t, min(group_size, FEW_ROWS), few_channels),
+                                           row0s=np.tile(np.arange(nb) * FEW_ROWS, B) if nb > 1 else None, group_size=group_size)
             items = h[base:base + S * FEW_INTS].reshape(S, FEW_INTS)
             items[:len(got)] = got
             items[len(got):, 2:4] = 0              # (no keys: nothing to do)
             after = base + S * FEW_INTS
-            h[after:after + B * n_kv_heads] = 0
+            h[after:after + B * nb * n_kv_heads] = 0
             if extra:
                 h[after + B * n_kv_heads:after + B * n_kv_heads + B * 8] = extras.ravel()
             return
