@@ -106,3 +106,46 @@ def test_page_list(mask, keep, requests, monkeypatch):
             elif not positions or (requests is not None and b not in requests):
                 assert table[b][i] == -1
     assert seen == set(range(n))
+
+
+@pytest.mark.parametrize("mask", [None, 40, "chunk"])
+@pytest.mark.parametrize("room", [1, 9, 200])
+@pytest.mark.parametrize("G", [1, 4, 24])
+def test_row_blocks_cover_every_key_once(mask, room, G):
+    """Requests of many rows, 16 of them a block: every block sees its own rows' keys, cut into ranges that meet."""
+    from xyntetik_runner_amd.engine.batch import Chunked, few_row_items, first_key
+    mask = Chunked(48) if mask == "chunk" else mask
+    starts, lens, q0s = [100, 0, 37, 700], [9, 1, 70, 33], [0, 9, 10, 80]
+    blocks = [(b, r) for b in range(4) for r in range(0, lens[b] * G, 16)]
+    of = [b for b, _ in blocks]
+    seen = []
+
+    def ask(tiles):
+        seen.append(tiles)
+        return room + len(blocks)
+
+    items, _, n_slots = few_row_items(of, [starts[b] for b in of], [lens[b] for b in of], [q0s[b] for b in of], mask, ask, False, first_slot=3,
+                                      least=lambda t: 1, row0s=[r for _, r in blocks], group_size=G)
+    total, taken = 0, []
+    for i, (b, row0) in enumerate(blocks):
+        first, last = row0 // G, min(lens[b] - 1, (row0 + 15) // G)
+        mine = sorted((it for it in items.tolist() if it[10] == i), key=lambda it: it[2])
+        at = first_key(mask, starts[b] + first) // 32 * 32
+        total += -(-(starts[b] + last + 1 - at) // 32)
+        for it in mine:
+            assert it[:2] == [b, row0] and it[2] == at and it[3] > at and it[5:8] == [q0s[b], lens[b], starts[b]] and it[11] == len(mine)
+            at = it[3]
+        assert at == starts[b] + last + 1
+        taken += [it[4] for it in mine if it[4] >= 0]
+        assert len(mine) > 1 or mine[0][4] == -1
+    assert seen == [total] and sorted(taken) == list(range(3, 3 + n_slots)) and len(items) <= room + len(blocks)
+
+
+def test_which_requests_are_read_back():
+    from xyntetik_runner_amd.engine.batch import FOUR_ROWS, four_row_requests, four_row_slots
+    assert four_row_requests([8000] * 64, [1] * 64, 4, None, 8) == list(range(64))
+    assert four_row_requests([6144], [2048], 4, None, 8) == [] and four_row_requests([6144, 50], [2048, FOUR_ROWS // 4], 4, None, 8) == [1]
+    assert four_row_requests([3488], [512], 4, None, 8) == [0]                  # few blocks for the other kernel
+    assert four_row_requests([60000], [512], 4, None, 8) == [] and four_row_requests([60000], [512], 4, 1024, 8) == [0]      # a window leaves little to do
+    assert four_row_requests([0], [FOUR_ROWS + 1], 1, None, 32) == [0]
+    assert four_row_slots(1500, 8, 256) == 2 * four_row_slots(280, 8, 256) == 512 and four_row_slots(10 ** 6, 8, 512) == 256

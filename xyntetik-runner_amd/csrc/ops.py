@@ -1049,9 +1049,9 @@ class Ops:
 
         bfloat16 runs on the matrix cores (head and value sizes in steps of 16 up to 256, pages of at least
         16 positions, a cap or slopes; kept first keys only where values have the keys' size); float32, and what the MFMA kernel does not take, runs the 32-bit kernel.
-        Caches that are ``FourBitPages``: requests of up to 16 rows a key/value head are read from the codes by a matrix-core kernel of their
-        own (bfloat16, sizes in whole blocks of 32, pages of at least 32 positions, no kept first keys); the pages of others are read back
-        first (``read_pages``), but in steps that are being recorded, which a 32-bit kernel then serves from the codes.
+        Caches that are ``FourBitPages``: requests of up to some hundred rows a key/value head are read from the codes by a matrix-core kernel of
+        their own (bfloat16, sizes in whole blocks of 32, pages of at least 32 positions, no kept first keys); the pages of others are read
+        back first (``read_pages``), but in steps that are being recorded, which a 32-bit kernel then serves from the codes.
         """
         positions, req_of_token, block_table = ctx.positions, ctx.req_of_token, ctx.block_table(group)
         self._dev(q, k_cache, v_cache, positions, req_of_token, block_table)
@@ -1086,8 +1086,7 @@ class Ops:
         if four:
             if self._few4_ok(q, out, ctx, D, Dv, page_size, scale, keep_first, softcap, slopes):
                 mask = Chunked(int(chunk)) if chunk else window
-                plan = ctx.attention_plan(group, H // Hk, mask, Hk, page_size, few_rows=2 if D + Dv <= 256 else 1, few_channels=D + Dv,
-                                          most_rows=self.FOUR_ROWS)
+                plan = ctx.attention_plan(group, H // Hk, mask, Hk, page_size, few_rows=3, few_channels=D + Dv)      # (FEW_FOUR)
                 lib = self.attention_lib(D, Dv)
                 part_o = part_ml = None
                 if plan.n_slots:
@@ -1165,8 +1164,6 @@ class Ops:
                and not (q.data_ptr() | k_cache.data_ptr() | v_cache.data_ptr()) & 15)
         more = {**({"extra_slot": True} if extra else {}), **({"few_rows": 2 if D + Dv <= 256 else 1, "few_channels": D + Dv} if few else {})}
         return ctx.attention_plan(group, H // Hk, mask, Hk, page_size, **more)
-
-    FOUR_ROWS = 64          # rows a key/value head that a request over 4-bit pages has at most to be served from the codes, 16 at a time
 
     def _few4_ok(self, q, out, ctx, D: int, Dv: int, page_size: int, scale: float, keep_first: int, softcap: float, slopes) -> bool:
         """Whether the matrix-core kernel for few rows over 4-bit pages takes a call's operands."""

@@ -80,6 +80,8 @@ FEW_ROWS = 16           # rows of an item of the kernel for few rows (a request'
 FEW_PAGE = 32           # and the smallest page it takes
 FEW_INTS = 12           # numbers of such an item
 FEW_MIN_RANGE = 3       # tiles: its shortest key range
+FEW_FOUR = 3            # (a plan's ``few_rows``) the kernel for few rows over 4-bit pages
+FOUR_ROWS = 400         # rows of a request that it always takes, 16 at a time
 FEW_SLOTS = 256         # workgroups of it that a step's requests are cut into: one a compute unit (twice as many cost more than they gain:
                         # 8 requests of 1,000 to 2,000 keys 15.0 us -> 15.9, 16 of 330 9.4 -> 10.6, 32 of 1,000 to 2,000 with heads of 64 22.6 -> 23.3)
 
@@ -222,10 +224,36 @@ def few_row_least(tiles: int, rows: int, channels: int = 256) -> int:
     return max(FEW_MIN_RANGE, -(-tiles // most))
 
 
+def four_row_slots(tiles: int, n_kv_heads: int, channels: int) -> int:
+    """Workgroups that a step of ``tiles`` tiles of keys is cut into over 4-bit pages: one a compute unit, or two where that leaves each a dozen tiles of 256
+    channels.  us with one and with two: 16 requests of 4,000 keys, 8 heads over each of 8 17.3 and 15.3, 30 of 2,500 with heads of 64 14.1 and 12.3, 3 of
+    9,000 with 32 key/value heads 21.8 and 20.8, 130 tokens x 4 heads over 9,000 71 and 55; 8 of 1,500 9.1 and 10.6, 32 x 3 tokens in a window of 1,024 with heads of
+    64 9.7 and 11.6; 4 of 30,000 21.5 and 22.3."""
+    return FEW_SLOTS * (2 if channels <= 256 and tiles * n_kv_heads * channels >= 12 * 256 * 2 * FEW_SLOTS else 1)
+
+
+def four_row_requests(starts, q_lens, group_size: int, mask, n_kv_heads: int):
+    """The requests of a step that are served from the codes of 4-bit pages, 16 rows a block; the pages of the others are read back first, for the kernel that
+    takes 128 rows a workgroup.
+
+    Reading back costs a launch and 2.5 bytes a number, the codes 0.5 ns a block and tile of 256 channels where the other kernel takes 0.35: from about 400 rows on.
+    A step whose blocks of many rows have little to do in all, or fill the other kernel badly, is served from the codes whole (us, codes and pages): 8 x 9 tokens
+    x 4 heads over 3,000 keys 16.3 and 49.4, 200 x 1 over 1,500 (six requests, 32 key/value heads) 57 and 81, 130 x 4 over 9,000 55 and 72, 512 x 4 over 4,000 64 and 73,
+    1,024 x 4 over 1,024 29.3 and 30.8; 4 requests of 256 x 4 over 2,000 59 and 53, 256 x 4 over 16,000 129 and 102, 1,024 x 4 over 3,000 86 and 66."""
+    rows = [n * group_size for n in q_lens]
+    many = [b for b, r in enumerate(rows) if r > FOUR_ROWS]
+    if many:
+        work = sum(-(-rows[b] // FEW_ROWS) * -(-(starts[b] + q_lens[b] - first_key(mask, starts[b] + q_lens[b] // 2)) // ATTN_TILE) for b in many) * n_kv_heads
+        fill = sum(-(-rows[b] // ATTN_CTA_ROWS) for b in many) * n_kv_heads
+        if work > (128000 if fill < ATTN_CTA_FILL else 48000):
+            return [b for b, r in enumerate(rows) if r <= FOUR_ROWS]
+    return list(range(len(rows)))
+
+
 def few_row_items(req, starts, lens, q0s, mask, room: int, extra_slot: bool, first_slot: int = 0, pair_at: int = 0, least=None,
                   row0s=None, group_size: int = 1):
     """The work of the kernel for few rows: requests ``req`` of a step, each with one row block (its ``lens[i]`` tokens from row
-    ``q0s[i]`` and position ``starts[i]`` on; with ``row0s`` an entry is the block of 16 rows from ``row0s[i]`` on, tokens x heads of a group of ``group_size``), cut into at most ``room`` key ranges of about one length, so that a
+    ``q0s[i]`` and position ``starts[i]`` on; with ``row0s`` an entry is the block of 16 rows from ``row0s[i]`` on, tokens x heads of a group of ``group_size``), cut into at most ``room`` key ranges (a number, or a function of the tiles of all) of about one length, so that a
     long request takes as many workgroups as its keys are worth: ``(items [n, 12], extras [len(req), 8], slots)`` as int64 arrays.
 
     An item: request, 0, first key, end key, partial slot (-1: all its keys), the request's first row, its tokens, its first
@@ -248,6 +276,8 @@ def few_row_items(req, starts, lens, q0s, mask, room: int, extra_slot: bool, fir
     else:
         lo = 0
     tiles = (hi - lo + (ATTN_TILE - 1)) // ATTN_TILE
+    if callable(room):
+        room = room(int(tiles.sum()))
     # the shortest length c with at most ``room`` ranges: ceil(t / c) a request, which c >= total / (room - requests) has in any case
     t = tiles.tolist()
     longest = max(t)
@@ -379,14 +409,18 @@ class StepContext:
         self.shared = {}        # what parts make once a step and share between layers (a rotation's table)
 
     def attention_plan(self, group: int, group_size: int, window, n_kv_heads: int,
-                       page_size: int = 64, extra_slot: bool = False, few_rows: int = 0, few_channels: int = 256, most_rows: int = FEW_ROWS) -> AttentionPlan:
+                       page_size: int = 64, extra_slot: bool = False, few_rows: int = 0, few_channels: int = 256) -> AttentionPlan:
         """The MFMA attention work list, made once per step and shared by all layers that can.  ``few_rows`` > 0:
-        requests of up to ``most_rows`` rows a key/value head go to the kernel for few rows (where the page size allows), 16 of them a row block, of which a compute unit
-        holds so many workgroups; ``few_channels``: those of a key and its value together."""
-        key = (group_size, window, n_kv_heads, page_size, extra_slot, few_rows, few_channels, most_rows)
+        requests of up to 16 rows a key/value head go to the kernel for few rows (where the page size allows), of which a compute unit
+        holds so many workgroups; ``FEW_FOUR``: to the one over 4-bit pages, 16 rows a block (``four_row_requests``); ``few_channels``: those of a key and its
+        value together."""
+        key = (group_size, window, n_kv_heads, page_size, extra_slot, few_rows, few_channels)
         plan = self._plans.get(key)
         if plan is None:
-            few = [b for b, n in enumerate(self.q_lens) if few_rows and page_size >= FEW_PAGE and n * group_size <= most_rows]
+            if few_rows == FEW_FOUR and page_size >= FEW_PAGE:
+                few = four_row_requests(self.starts, self.q_lens, group_size, window, n_kv_heads)
+            else:
+                few = [b for b, n in enumerate(self.q_lens) if few_rows and page_size >= FEW_PAGE and n * group_size <= FEW_ROWS]
             planned = plan_attention(self.starts, self.q_lens, group_size, window, n_kv_heads, page_size,
                                      extra_slot=extra_slot, skip=frozenset(few))
             cta_items, items, jobs, n_slots = planned[:4]
@@ -397,10 +431,11 @@ class StepContext:
                 blocks = [(b, row0) for b in few for row0 in range(0, self.q_lens[b] * group_size, FEW_ROWS)]
                 of = [b for b, _ in blocks]
                 q0s = np.concatenate([[0], np.cumsum(self.q_lens)])[of]
-                room = max(len(blocks), FEW_SLOTS // n_kv_heads)
+                slots = (lambda tiles: four_row_slots(tiles, n_kv_heads, few_channels)) if few_rows == FEW_FOUR else (lambda tiles: FEW_SLOTS)
                 rows = min(FEW_ROWS, group_size * max(self.q_lens[b] for b in few))
                 few_items, few_extras, more = few_row_items(of, [self.starts[b] for b in of], [self.q_lens[b] for b in of], q0s,
-                                                            window, room, extra_slot, n_slots, ATTN_STREAM_SLOTS // n_kv_heads if few_rows == 2 else 0,
+                                                            window, lambda tiles: max(len(blocks), slots(tiles) // n_kv_heads), extra_slot, n_slots,
+                                                            ATTN_STREAM_SLOTS // n_kv_heads if few_rows >= 2 else 0,
                                                             least=lambda t: few_row_least(t, rows, few_channels),
                                                             row0s=[r for _, r in blocks] if len(blocks) > len(few) else None, group_size=group_size)
                 n_slots += more

@@ -22,8 +22,8 @@ import numpy as np
 import torch
 
 from ..cache import NULL_PAGE
-from .batch import (ATTN_MIN_RANGE, ATTN_STREAM_SLOTS, ATTN_TILE, FEW_INTS, FEW_MIN_RANGE, FEW_PAGE, FEW_ROWS, FEW_SLOTS, AttentionPlan,
-                    Chunked, StepEntry, few_row_items, few_row_least, mask_reach)
+from .batch import (ATTN_MIN_RANGE, ATTN_STREAM_SLOTS, ATTN_TILE, FEW_FOUR, FEW_INTS, FEW_MIN_RANGE, FEW_PAGE, FEW_ROWS, FEW_SLOTS, AttentionPlan,
+                    Chunked, StepEntry, few_row_items, few_row_least, four_row_slots, mask_reach)
 
 BUCKETS = (1, 2, 4, 8, 16, 32, 64, 128, 256, 512)
 SPLITS = (1, 2, 4, 8, 16, 32)
@@ -65,12 +65,12 @@ def few_blocks(group_size: int) -> int:
     return -(-group_size // FEW_ROWS)
 
 
-def few_row_room(batch_cap: int, tiles: int, n_kv_heads: int) -> int:
+def few_row_room(batch_cap: int, tiles: int, n_kv_heads: int, slots: int = FEW_SLOTS) -> int:
     """Items that a recorded step keeps for the kernel for few rows: one a request, and as many key ranges as fill the kernel's workgroups beside the
     rows that pad the batch (fewer than half of it, an item each), but no more than ranges of the shortest length (and one for what the requests' last ranges lack).
     ``tiles``: those of the longest request that the graph will serve, not of the one it is recorded with: ranges and the last bits of a result then
     do not hang on what ran before, and a request that grows gets as many as one that came long (items without keys return at once)."""
-    return max(batch_cap, min(FEW_SLOTS // n_kv_heads + batch_cap // 2, batch_cap * (-(-tiles // FEW_MIN_RANGE) + 1)))
+    return max(batch_cap, min(slots // n_kv_heads + batch_cap // 2, batch_cap * (-(-tiles // FEW_MIN_RANGE) + 1)))
 
 
 class StaticDecodeContext:
@@ -163,8 +163,8 @@ class StaticDecodeContext:
                            "ctx.slots (on the device), or sets capturable = False to be run eagerly")
 
     def attention_plan(self, group: int, group_size: int, window, n_kv_heads: int,
-                       page_size: int = 64, extra_slot: bool = False, few_rows: int = 0, few_channels: int = 256, most_rows: int = FEW_ROWS) -> AttentionPlan:
-        few = few_rows if page_size >= FEW_PAGE and group_size <= most_rows else 0
+                       page_size: int = 64, extra_slot: bool = False, few_rows: int = 0, few_channels: int = 256) -> AttentionPlan:
+        few = few_rows if page_size >= FEW_PAGE and (group_size <= FEW_ROWS or few_rows == FEW_FOUR) else 0
         key = (group_size, window, n_kv_heads, bool(extra_slot), few, few_channels if few else 0)
         if key not in self._plans:
             if torch.cuda.is_current_stream_capturing():
@@ -173,7 +173,8 @@ class StaticDecodeContext:
             if tiles is not None and window:
                 tiles = min(tiles, -(-mask_reach(window) // ATTN_TILE) + 1)
             if few:
-                self._plan_splits[key] = few_row_room(self.B * few_blocks(group_size), tiles if tiles is not None else self.S * FEW_MIN_RANGE, n_kv_heads)
+                self._plan_splits[key] = few_row_room(self.B * few_blocks(group_size), tiles if tiles is not None else self.S * FEW_MIN_RANGE, n_kv_heads,
+                                                      2 * FEW_SLOTS if few == FEW_FOUR else FEW_SLOTS)
             else:
                 self._plan_splits[key] = self.S if tiles is None else min(self.S, splits_for(self.B, tiles, n_kv_heads))
             self._plan_keys.append(key)
@@ -249,8 +250,10 @@ class StaticDecodeContext:
             # (rows that pad the batch have an item each, and leave the requests all the workgroups)
             nb = few_blocks(group_size)
             of = np.repeat(np.arange(B), nb)
-            got, extras, _ = few_row_items(of, starts[of], np.ones(B * nb, dtype=np.int64), of, window, min(S, max(B * nb, FEW_SLOTS // n_kv_heads + (B - n) * nb)), extra,
-                                           pair_at=ATTN_STREAM_SLOTS // n_kv_heads if few == 2 else 0, least=lambda t: few_row_least(t, min(group_size, FEW_ROWS), few_channels),
+            slots = (lambda tiles: four_row_slots(tiles, n_kv_heads, few_channels)) if few == FEW_FOUR else (lambda tiles: FEW_SLOTS)
+            got, extras, _ = few_row_items(of, starts[of], np.ones(B * nb, dtype=np.int64), of, window,
+                                           lambda tiles: min(S, max(B * nb, slots(tiles) // n_kv_heads + (B - n) * nb)), extra,
+                                           pair_at=ATTN_STREAM_SLOTS // n_kv_heads if few >= 2 else 0, least=lambda t: few_row_least(t, min(group_size, FEW_ROWS), few_channels),
                                            row0s=np.tile(np.arange(nb) * FEW_ROWS, B) if nb > 1 else None, group_size=group_size)
             items = h[base:base + S * FEW_INTS].reshape(S, FEW_INTS)
             items[:len(got)] = got
