@@ -7,7 +7,9 @@
 // lose nothing (a 32-bit product is off by 0.004 at 131,071).
 //
 // A thread takes 8 channels of a head of queries, keys or values; 4 neighbouring lanes are a block of 32 and share its largest
-// magnitude in two exchanges.  (A head's last block may be short: its missing lanes hold zeros.)
+// magnitude in two exchanges.  (A head's last block may be short: its missing lanes hold zeros.)  Where the rows are aligned it reads its channels and
+// their partners in the rotation as four pieces of 16 bytes, before the angles are made.  A page holds the bytes of 8 positions of a value side by side: where the
+// step brings such 8 positions whole, the workgroup of the first writes them all, 16 bytes at a time, and the other seven leave their values to it.
 struct Write4Args {
     const float* q_in;      // [T, in_stride] 32-bit
     const float* k_in;
@@ -24,9 +26,11 @@ struct Write4Args {
     float mscale;
     int page_shift, page_mask, page_size;
     int q_units, k_units, units, per_block;     // of a token: queries' end, keys' end, all; and those of a workgroup
-    int lanes_k, lanes_v;                       // threads of a head of queries or keys, and of values (a multiple of 4)
+    int lanes_k, lanes_v;                       // threads of a head of queries or keys, and of values (a multiple of 4, 32 at most)
+    uint32_t per_k, per_v;                      // 2^32 over these, rounded up: a division below 2^26 is one product
 };
 
+// (8 numbers of a row that begin at a multiple of 16 bytes)
 template <typename T> __device__ inline void store_row8(T* dst, const float* v);
 template <> __device__ inline void store_row8<float>(float* dst, const float* v) {
     *reinterpret_cast<float4*>(dst) = make_float4(v[0], v[1], v[2], v[3]);
@@ -36,72 +40,168 @@ template <> __device__ inline void store_row8<bf16_t>(bf16_t* dst, const float* 
     *reinterpret_cast<uint4*>(dst) = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
 }
 
-template <typename T>
+__device__ __forceinline__ void load_row8(const float* p, float* v) {
+    const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+}
+// the largest magnitude of a block of 32, of which the lane holds 8
+__device__ __forceinline__ uint32_t most_of_block(const float* x) {
+    uint32_t most = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) most = max(most, __float_as_uint(x[i]) & 0x7FFFFFFFu);
+    most = max(most, (uint32_t)__shfl_xor((int)most, 1, 64));
+    return max(most, (uint32_t)__shfl_xor((int)most, 2, 64));
+}
+// byte b of four words
+template <int B> __device__ __forceinline__ uint32_t bytes_of(uint32_t w0, uint32_t w1, uint32_t w2, uint32_t w3) {
+    const uint32_t lo = __builtin_amdgcn_perm(w1, w0, 0x0c0c0400u + 0x0101u * B), hi = __builtin_amdgcn_perm(w3, w2, 0x04000c0cu + 0x01010000u * B);
+    return lo | hi;
+}
+
+// VEC: rows of 16-byte pieces, and a rotation whose pairs lie in such pieces
+template <typename T, bool VEC>
 __global__ __launch_bounds__(256) void k_rope_kv_write4(Write4Args a) {
-    __shared__ float2 cs[128];
-    const int t = blockIdx.x, pos = a.positions[t];
+    __shared__ float2 cs[8][17];                // pair j at [j % 8][j / 8]: lanes that read the i-th of their 8 pairs read side by side
+    // (workgroups go to the eight dies in turn: 8 neighbouring tokens, whose codes share lines, to one of them)
+    const int b = blockIdx.x, t = b < ((int)gridDim.x & ~63) ? (b & ~63) | (b & 7) << 3 | (b >> 3 & 7) : b;
+    const int pos = a.positions[t];
     const int half = a.rot >> 1;
     const int u0 = blockIdx.y * a.per_block, u1 = min(a.units, u0 + a.per_block);
+    const int req = a.req_of_token ? a.req_of_token[t] : 0;
+    // a unit: what it is, its head, its first channel, and its numbers as they come
+    struct Unit { int h, c0, D; bool is_q, is_v; const float* src; float x[8], y[8]; };
+    auto unit = [&](int u) __attribute__((always_inline)) {
+        Unit w;
+        w.is_q = u < a.q_units;
+        w.is_v = u >= a.k_units;
+        const int n = w.is_q ? u : w.is_v ? u - a.k_units : u - a.q_units, lanes = w.is_v ? a.lanes_v : a.lanes_k;
+        w.D = w.is_v ? a.Dv : a.D;
+        w.h = (int)__umulhi((unsigned)n, w.is_v ? a.per_v : a.per_k);         // n / lanes
+        w.c0 = (n - w.h * lanes) * 8;
+        w.src = (w.is_q ? a.q_in : w.is_v ? a.v_in : a.k_in) + (size_t)t * a.in_stride + (size_t)w.h * w.D;
+        if constexpr (VEC) {
+            const bool turn = !w.is_v && w.c0 < a.rot && !a.interleaved;
+            int own = w.c0, other = w.c0;
+            if (turn) {
+                const bool second = w.c0 >= half;
+                own = a.paired ? (second ? 2 * (w.c0 - half) + 8 : 2 * w.c0) : w.c0;
+                other = a.paired ? (second ? own - 8 : own + 8) : second ? w.c0 - half : w.c0 + half;
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) w.x[i] = w.y[i] = 0.f;
+            if (w.c0 < w.D) load_row8(w.src + own, w.x);
+            if (turn) load_row8(w.src + other, w.y);
+        }
+        return w;
+    };
+    const int first = u0 + (int)threadIdx.x;
+    Unit ahead = unit(first < u1 ? first : u0);
     for (int j = threadIdx.x; j < half; j += 256) {
         double turns = (double)pos * (double)a.inv_freq[j] * 0.15915494309189533577;
         turns -= rint(turns);
         float s, c;
         sincospif((float)(2.0 * turns), &s, &c);
-        cs[j] = make_float2(c * a.mscale, s * a.mscale);
+        cs[j & 7][j >> 3] = make_float2(c * a.mscale, s * a.mscale);
     }
-    __syncthreads();
     const int bi = pos >> a.page_shift, off = pos & a.page_mask;
-    const int page = a.Hk > 0 && bi >= 0 && bi < a.table_stride ? a.block_table[(size_t)a.req_of_token[t] * a.table_stride + bi] : -1;
-    for (int u = u0 + (int)threadIdx.x; u < u1; u += 256) {
-        const bool is_q = u < a.q_units, is_v = u >= a.k_units;
-        const int w = is_q ? u : is_v ? u - a.k_units : u - a.q_units;
-        const int lanes = is_v ? a.lanes_v : a.lanes_k, D = is_v ? a.Dv : a.D;
-        const int h = w / lanes, c0 = (w - h * lanes) * 8;
-        const float* src = (is_q ? a.q_in : is_v ? a.v_in : a.k_in) + (size_t)t * a.in_stride + (size_t)h * D;
-        float x[8];
-        if (c0 >= D) {
+    const int page = bi >= 0 && bi < a.table_stride ? a.block_table[(size_t)req * a.table_stride + bi] : -1;
+    const bool there = (unsigned)page < (unsigned)a.n_pages;
+    // the 8 positions of a page that this one belongs to: whole in this step?  (A request's tokens of a step are consecutive rows at
+    // consecutive positions.)
+    const int lead = t - (pos & 7);
+    const bool whole = lead >= 0 && lead + 7 < (int)gridDim.x && a.req_of_token[lead] == req && a.req_of_token[lead + 7] == req &&
+                       a.positions[lead] == pos - (pos & 7) && a.positions[lead + 7] == pos - (pos & 7) + 7;
+    __syncthreads();
+    for (int u = first; u < u1; u += 256) {
+        Unit w = u == first ? ahead : unit(u);
+        float* x = w.x;
+        if (w.is_v && whole) {
+            if (pos & 7) continue;
+            // 8 positions, all on their way at once: a word of codes each, then their bytes side by side
+            uint32_t c[8], sc[2] = {0, 0};
+            float v[8][8];
+            const float* src = w.src + (w.c0 < w.D ? w.c0 : 0);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = 0.f;
-        } else if (is_v || c0 >= a.rot) {
+            for (int i = 0; i < 8; ++i) {
+                if constexpr (VEC) load_row8(src + (size_t)i * a.in_stride, v[i]);
+                else
 #pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = src[c0 + i];
+                    for (int e = 0; e < 8; ++e) v[i][e] = src[(size_t)i * a.in_stride + e];
+            }
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                if (w.c0 >= w.D)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[i][e] = 0.f;
+                const uint32_t byte = scale_byte4(most_of_block(v[i]));
+                c[i] = codes4(v[i], byte);
+                sc[i >> 2] |= byte << (8 * (i & 3));
+            }
+            if (w.c0 >= w.D || !there) continue;
+            const size_t pb = (size_t)page * a.Hk + w.h;
+            if ((w.c0 & 31) == 0) *reinterpret_cast<uint2*>(a.pages.vs + scale_at4(pb, a.page_size, blocks4(w.D), off, w.c0 >> 5)) = make_uint2(sc[0], sc[1]);
+            uint4* dst = reinterpret_cast<uint4*>(a.pages.vc + value_at4(pb, a.page_size, w.D, off, w.c0 >> 1));
+            dst[0] = make_uint4(bytes_of<0>(c[0], c[1], c[2], c[3]), bytes_of<0>(c[4], c[5], c[6], c[7]), bytes_of<1>(c[0], c[1], c[2], c[3]), bytes_of<1>(c[4], c[5], c[6], c[7]));
+            dst[1] = make_uint4(bytes_of<2>(c[0], c[1], c[2], c[3]), bytes_of<2>(c[4], c[5], c[6], c[7]), bytes_of<3>(c[0], c[1], c[2], c[3]), bytes_of<3>(c[4], c[5], c[6], c[7]));
+            continue;
+        }
+        if constexpr (VEC) {
+            if (!w.is_v && w.c0 < a.rot) {
+                if (a.interleaved) {
+#pragma unroll
+                    for (int i = 0; i < 8; i += 2) {
+                        const int j = (w.c0 + i) >> 1;
+                        const float2 r = cs[j & 7][j >> 3];
+                        const float x0 = x[i], x1 = x[i + 1];
+                        x[i] = x0 * r.x - x1 * r.y;
+                        x[i + 1] = x0 * r.y + x1 * r.x;
+                    }
+                } else {
+                    const bool second = w.c0 >= half;
+                    const int j = second ? w.c0 - half : w.c0;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const float2 r = cs[i][j >> 3];
+                        x[i] = second ? w.y[i] * r.y + x[i] * r.x : x[i] * r.x - w.y[i] * r.y;
+                    }
+                }
+            }
         } else {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const int c = c0 + i;
-                if (c >= a.rot) {
-                    x[i] = src[c];
+                const int c = w.c0 + i;
+                if (w.c0 >= w.D) {
+                    x[i] = 0.f;
+                } else if (w.is_v || c >= a.rot) {
+                    x[i] = w.src[c];
                 } else {
                     const int j = a.interleaved ? c >> 1 : c < half ? c : c - half;
                     const bool second = a.interleaved ? (c & 1) : c >= half;
                     int i0 = a.interleaved ? 2 * j : j, i1 = a.interleaved ? 2 * j + 1 : j + half;
                     if (a.paired) { i0 = paired_col(i0, a.rot); i1 = paired_col(i1, a.rot); }
-                    const float x0 = src[i0], x1 = src[i1];
-                    const float2 r = cs[j];
+                    const float x0 = w.src[i0], x1 = w.src[i1];
+                    const float2 r = cs[j & 7][j >> 3];
                     x[i] = second ? x0 * r.y + x1 * r.x : x0 * r.x - x1 * r.y;
                 }
             }
         }
-        if (is_q) {
-            if (c0 < D) store_row8<T>((T*)a.q_out + ((size_t)t * a.H + h) * D + c0, x);
+        if (w.is_q) {
+            if (w.c0 < w.D) store_row8<T>((T*)a.q_out + ((size_t)t * a.H + w.h) * w.D + w.c0, x);
             continue;
         }
-        uint32_t most = 0;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) most = max(most, __float_as_uint(x[i]) & 0x7FFFFFFFu);
-        most = max(most, (uint32_t)__shfl_xor((int)most, 1, 64));
-        most = max(most, (uint32_t)__shfl_xor((int)most, 2, 64));
-        if (c0 >= D || (unsigned)page >= (unsigned)a.n_pages) continue;
+        const uint32_t most = most_of_block(x);
+        if (w.c0 >= w.D || !there) continue;
         const uint32_t byte = scale_byte4(most), codes = codes4(x, byte);
-        const size_t pb = (size_t)page * a.Hk + h;
-        uint8_t* scales = is_v ? a.pages.vs : a.pages.ks;
-        if ((c0 & 31) == 0) scales[scale_at4(pb, a.page_size, blocks4(D), off, c0 >> 5)] = (uint8_t)byte;
-        if (is_v) {
-            uint8_t* dst = a.pages.vc + value_at4(pb, a.page_size, D, off, c0 >> 1);
+        const size_t pb = (size_t)page * a.Hk + w.h;
+        uint8_t* scales = w.is_v ? a.pages.vs : a.pages.ks;
+        if ((w.c0 & 31) == 0) scales[scale_at4(pb, a.page_size, blocks4(w.D), off, w.c0 >> 5)] = (uint8_t)byte;
+        if (w.is_v) {
+            uint8_t* dst = a.pages.vc + value_at4(pb, a.page_size, w.D, off, w.c0 >> 1);
 #pragma unroll
             for (int i = 0; i < 4; ++i) dst[8 * i] = (uint8_t)(codes >> (8 * i));
         } else {
-            *reinterpret_cast<uint32_t*>(a.pages.kc + key_at4(pb, a.page_size, D, off) + (c0 >> 1)) = codes;
+            *reinterpret_cast<uint32_t*>(a.pages.kc + key_at4(pb, a.page_size, w.D, off) + (w.c0 >> 1)) = codes;
         }
     }
 }
@@ -124,7 +224,7 @@ extern "C" int xr_rope_kv_write4(const float* q_in, const float* k_in, const flo
     a.pages = Pages4{(uint8_t*)kc, (uint8_t*)ks, (uint8_t*)vc, (uint8_t*)vs};
     const int rc = check_pages4("rope_kv_write", a.pages, Hk, D, Dv, page_size, n_pages);
     if (rc != XR_OK) return rc;
-    XR_REQUIRE(T >= 0 && H >= 0 && table_stride > 0, "rope_kv_write: bad sizes T=%d H=%d, block tables of %d pages", T, H, table_stride);
+    XR_REQUIRE(T >= 0 && H >= 0 && H < (1 << 20) && Hk < (1 << 20) && table_stride > 0, "rope_kv_write: bad sizes T=%d H=%d, block tables of %d pages", T, H, table_stride);
     XR_REQUIRE(rot >= 0 && rot <= D && rot % 2 == 0, "rope_kv_write: rotary width %d must be even and at most head_dim %d", rot, D);
     XR_REQUIRE(rot == 0 || inv_freq, "rope_kv_write: rotary width %d without a frequency table", rot);
     XR_REQUIRE(q_dtype == XR_F32 || q_dtype == XR_BF16, "rope_kv_write: bad dtype %d", q_dtype);
@@ -137,6 +237,7 @@ extern "C" int xr_rope_kv_write4(const float* q_in, const float* k_in, const flo
     a.inv_freq = inv_freq; a.H = H; a.Hk = Hk; a.D = D; a.Dv = Dv; a.rot = rot; a.interleaved = interleaved; a.paired = paired ? 1 : 0;
     a.mscale = mscale; a.page_shift = ilog2_exact(page_size); a.page_mask = page_size - 1; a.page_size = page_size;
     a.lanes_k = blocks4(D) * 4; a.lanes_v = blocks4(Dv) * 4;
+    a.per_k = (uint32_t)(((1ull << 32) + a.lanes_k - 1) / a.lanes_k); a.per_v = (uint32_t)(((1ull << 32) + a.lanes_v - 1) / a.lanes_v);
     a.q_units = H * a.lanes_k; a.k_units = a.q_units + Hk * a.lanes_k; a.units = a.k_units + Hk * a.lanes_v;
     // a token a workgroup where there are tokens enough for the chip, else a round of threads each
     int groups = (1024 + T - 1) / T;
@@ -144,8 +245,12 @@ extern "C" int xr_rope_kv_write4(const float* q_in, const float* k_in, const flo
     groups = groups < 1 ? 1 : groups > most ? most : groups;
     a.per_block = ((a.units + groups - 1) / groups + 255) / 256 * 256;
     const dim3 grid(T, (a.units + a.per_block - 1) / a.per_block);
-    if (q_dtype == XR_F32) k_rope_kv_write4<float><<<grid, 256, 0, stream>>>(a);
-    else k_rope_kv_write4<bf16_t><<<grid, 256, 0, stream>>>(a);
+    const bool vec = in_stride % 4 == 0 && (((uintptr_t)(H ? q_in : k_in) | (uintptr_t)k_in | (uintptr_t)v_in) & 15) == 0 && (interleaved ? rot % 8 == 0 : rot % 16 == 0);
+    if (q_dtype == XR_F32) {
+        if (vec) k_rope_kv_write4<float, true><<<grid, 256, 0, stream>>>(a);
+        else k_rope_kv_write4<float, false><<<grid, 256, 0, stream>>>(a);
+    } else if (vec) k_rope_kv_write4<bf16_t, true><<<grid, 256, 0, stream>>>(a);
+    else k_rope_kv_write4<bf16_t, false><<<grid, 256, 0, stream>>>(a);
     XR_CHECK_LAUNCH("rope_kv_write4");
     return XR_OK;
 }
