@@ -196,6 +196,10 @@ class FourBitPages:
             raise KernelError("4-bit pages: codes and scales must be uint8 on one device")
         if not codes.is_contiguous() or not scales.is_contiguous() or codes.data_ptr() % 16 or scales.data_ptr() % 8:
             raise KernelError("4-bit pages: codes and scales must be contiguous, 16 and 8 bytes aligned")
+        self.device, self.is_cuda = codes.device, codes.is_cuda
+        # what a pair of keys and values has in common, and where the bytes are (the tensors are never replaced)
+        self.layout = (self.num_pages, self.heads, self.page_size, self.device)
+        self.pointers = (codes.data_ptr(), scales.data_ptr())
 
     @staticmethod
     def shapes(pages: int, heads: int, page_size: int, dim: int, values: bool):
@@ -211,14 +215,6 @@ class FourBitPages:
     def zeros(cls, pages: int, heads: int, page_size: int, dim: int, values: bool, device) -> "FourBitPages":
         codes, scales = cls.shapes(pages, heads, page_size, dim, values)
         return cls(torch.zeros(codes, dtype=torch.uint8, device=device), torch.zeros(scales, dtype=torch.uint8, device=device), dim)
-
-    @property
-    def device(self):
-        return self.codes.device
-
-    @property
-    def is_cuda(self):
-        return self.codes.is_cuda
 
     @property
     def dtype(self):            # (what takes 16- or 32-bit caches refuses these by it)
@@ -806,20 +802,20 @@ class Ops:
     @staticmethod
     def _pages4(what: str, k_pages, v_pages, Hk: Optional[int] = None, D: Optional[int] = None, page_size: Optional[int] = None):
         """The operands of a pair of 4-bit caches for the library."""
+        if (type(k_pages) is FourBitPages and type(v_pages) is FourBitPages and k_pages.layout == v_pages.layout and v_pages.values and not k_pages.values
+                and (Hk is None or (Hk == k_pages.heads and D == k_pages.dim and page_size == k_pages.page_size))):
+            return k_pages.pointers + v_pages.pointers + (k_pages.num_pages,)
         if not (isinstance(k_pages, FourBitPages) and isinstance(v_pages, FourBitPages)) or k_pages.values or not v_pages.values:
             raise KernelError(f"{what}: keys and values must both be in 4-bit pages, keys in a key's and values in a value's")
-        if (k_pages.num_pages, k_pages.heads, k_pages.page_size) != (v_pages.num_pages, v_pages.heads, v_pages.page_size) or k_pages.device != v_pages.device:
+        if k_pages.layout != v_pages.layout:
             raise KernelError(f"{what}: keys and values differ in pages, heads or device")
-        if ((Hk is not None and Hk != k_pages.heads) or (D is not None and D != k_pages.dim)
-                or (page_size is not None and page_size != k_pages.page_size)):
-            raise KernelError(f"{what}: 4-bit pages of {k_pages.heads} heads of {k_pages.dim} channels in pages of {k_pages.page_size} do not fit "
-                              f"{Hk} heads of {D} in pages of {page_size}")
-        return (k_pages.codes.data_ptr(), k_pages.scales.data_ptr(), v_pages.codes.data_ptr(), v_pages.scales.data_ptr(), k_pages.num_pages)
+        raise KernelError(f"{what}: 4-bit pages of {k_pages.heads} heads of {k_pages.dim} channels in pages of {k_pages.page_size} do not fit "
+                          f"{Hk} heads of {D} in pages of {page_size}")
 
     @staticmethod
-    def _ints(what: str, n: Optional[int], *ts: torch.Tensor) -> None:
+    def _ints(what: str, n: int, *ts: torch.Tensor) -> None:
         for t in ts:
-            if t.dtype != torch.int32 or t.dim() != 1 or (t.numel() > 1 and t.stride(0) != 1) or (n is not None and t.numel() != n):
+            if t.dtype is not torch.int32 or t.shape != (n,) or not t.is_contiguous():
                 raise KernelError(f"{what}: positions and requests must be int32, contiguous and of one length")
 
     @staticmethod
@@ -836,17 +832,19 @@ class Ops:
         self._ints("rope_kv_write", T, positions, req_of_token)
         self._table("rope_kv_write", block_table)
         H = H if q_in is not None else 0
+        stride = k_in.stride(0)
         for t, width in ((q_in, H * D), (k_in, Hk * D), (v_in, Hk * Dv)):
-            if t is not None and (t.dtype != torch.float32 or tuple(t.shape) != (T, width) or (width > 1 and t.stride(1) != 1)):
-                raise KernelError(f"rope_kv_write: inputs must be float32 [{T}, heads x channels] with unit column stride")
-        if T > 1 and len({t.stride(0) for t in (q_in, k_in, v_in) if t is not None}) > 1:
-            raise KernelError("rope_kv_write: q, k and v inputs must share a row stride")
-        if q_out is not None and (tuple(q_out.shape) != (T, H * D) or not q_out.is_contiguous() or q_out.data_ptr() % 16):
+            if t is not None:
+                if t.dtype is not torch.float32 or t.shape != (T, width) or (width > 1 and t.stride(1) != 1):
+                    raise KernelError(f"rope_kv_write: inputs must be float32 [{T}, heads x channels] with unit column stride")
+                if T > 1 and t.stride(0) != stride:
+                    raise KernelError("rope_kv_write: q, k and v inputs must share a row stride")
+        if q_out is not None and (q_out.shape != (T, H * D) or not q_out.is_contiguous() or q_out.data_ptr() % 16):
             raise KernelError(f"rope_kv_write: the queries' place must be contiguous [{T}, {H * D}] and 16-byte aligned")
         if rot and (inv_freq is None or inv_freq.dtype != torch.float32 or inv_freq.numel() != rot // 2 or not inv_freq.is_contiguous()):
             raise KernelError(f"rope_kv_write: {rot // 2} 32-bit frequencies are needed")
         self.lib.check(self.lib.xr_rope_kv_write4(
-            _ptr(q_in), k_in.data_ptr(), v_in.data_ptr(), k_in.stride(0), _ptr(q_out), *pages, positions.data_ptr(), req_of_token.data_ptr(),
+            _ptr(q_in), k_in.data_ptr(), v_in.data_ptr(), stride, _ptr(q_out), *pages, positions.data_ptr(), req_of_token.data_ptr(),
             block_table.data_ptr(), block_table.stride(0), _ptr(inv_freq) if rot else None, T, H, Hk, D, Dv, rot, 1 if interleaved else 0,
             float(mscale), page_size, dtype_code(q_out.dtype) if q_out is not None else XR_F32, 1 if paired else 0, _stream()))
 
@@ -1060,7 +1058,7 @@ class Ops:
         four = isinstance(k_cache, FourBitPages) or isinstance(v_cache, FourBitPages)
         if four:
             pages = self._pages4("attention", k_cache, v_cache, Hk, D, page_size)
-            if tuple(q.shape) != (T, H * D) or v_cache.dim != (int(v_head_dim) if v_head_dim is not None else D):
+            if q.shape != (T, H * D) or v_cache.dim != (int(v_head_dim) if v_head_dim is not None else D):
                 raise KernelError(f"attention: queries {tuple(q.shape)} or values of {v_cache.dim} do not fit {T} rows of {H} heads of {D}")
             dtype_code(q.dtype)
         elif q.dtype != k_cache.dtype or q.dtype != v_cache.dtype:
@@ -1089,13 +1087,14 @@ class Ops:
                 plan = ctx.attention_plan(group, H // Hk, mask, Hk, page_size, few_rows=3, few_channels=D + Dv)      # (FEW_FOUR)
                 lib = self.attention_lib(D, Dv)
                 part_o = part_ml = None
-                if plan.n_slots:
-                    part_o = torch.empty((plan.n_slots, Hk, 32, Dv), dtype=torch.float32, device=q.device)
-                    part_ml = torch.empty((plan.n_slots, Hk, 32, 2), dtype=torch.float32, device=q.device)
+                if plan.n_slots:        # partial results, and behind them their maxima and sums
+                    parts = torch.empty((plan.n_slots * Hk * 32, Dv + 2), dtype=torch.float32, device=q.device)
+                    part_o = parts.data_ptr()
+                    part_ml = part_o + plan.n_slots * Hk * 32 * Dv * 4
                 if plan.n_few:
                     lib.check(lib.xr_attention_few4(
                         out.data_ptr(), q.data_ptr(), *pages[:4], plan.few.data_ptr(), plan.n_few, plan.counters.data_ptr(), block_table.data_ptr(),
-                        block_table.stride(0), _ptr(part_o), _ptr(part_ml), H, Hk, D, Dv, page_size, float(scale), int(window or 0), int(chunk or 0),
+                        block_table.stride(0), part_o, part_ml, H, Hk, D, Dv, page_size, float(scale), int(window or 0), int(chunk or 0),
                         _ptr(slopes), _ptr(sinks), float(softcap), *gating, _stream()))
                 if not plan.n_items and not plan.n_cta_items:
                     return out
@@ -1105,7 +1104,7 @@ class Ops:
                     lib.check(lib.xr_attention_mfma(
                         out.data_ptr(), q.data_ptr(), k16.data_ptr(), v16.data_ptr(), plan.items.data_ptr(), plan.n_items, plan.n_cta_items, None, 0,
                         None, _ptr(plan.jobs), plan.n_jobs, ctx.cu_q.data_ptr(), ctx.starts_dev.data_ptr(), table.data_ptr(), table.stride(0),
-                        _ptr(part_o), _ptr(part_ml), H, Hk, D, Dv, page_size, float(scale), int(window or 0), int(chunk or 0), _ptr(slopes),
+                        part_o, part_ml, H, Hk, D, Dv, page_size, float(scale), int(window or 0), int(chunk or 0), _ptr(slopes),
                         _ptr(sinks), float(softcap), *gating, _stream()))
                     return out
             if not getattr(ctx, "knows_lengths", False):
