@@ -45,7 +45,7 @@ def log(msg):
     sys.stderr.flush()
 
 
-def build_runner(cfg, dtype, max_tokens, max_requests, seed=0):
+def build_runner(cfg, dtype, max_tokens, max_requests, seed=0, cache_dtype=None):
     import torch
     from xyntetik_runner_amd.config import config_from_dict
     from xyntetik_runner_amd.engine import ModelRunner
@@ -56,7 +56,7 @@ def build_runner(cfg, dtype, max_tokens, max_requests, seed=0):
     t0 = time.time()
     state = random_state(Model.expected_tensors(spec), seed, device=torch.device("cuda:0"))
     runner = ModelRunner(spec, state, dtype, max_tokens=max_tokens, page_size=64, max_requests=max_requests,
-                         consume_state=True)      # the 70B shape is half the card: it must not stand there twice
+                         cache_dtype=cache_dtype, consume_state=True)      # the 70B shape is half the card: it must not stand there twice
     del state
     torch.cuda.synchronize()
     log(f"model with {len(spec.layers)} layers on the GPU in {time.time() - t0:.1f} s")
@@ -70,13 +70,18 @@ def matmul_params(cfg, layers):
     return per_layer * layers, V * E
 
 
-def decode_bytes(cfg, layers, batch, ctx_tokens, elt=2):
+def kv_bytes(cfg, layers, elt, cache_dtype=None):
+    """Bytes of a cached token: in 4 bits half a byte a channel and one for every 32."""
+    D = cfg["head_dim"]
+    return 2 * cfg["num_key_value_heads"] * layers * (D // 2 + -(-D // 32) if cache_dtype == "mxfp4" else D * elt)
+
+
+def decode_bytes(cfg, layers, batch, ctx_tokens, elt=2, cache_dtype=None):
     """Bytes one decode step has to read: every weight it uses once, and the cache of the live requests."""
     body, head = matmul_params(cfg, layers)
     norms = (2 * layers + 1) * cfg["hidden_size"]
     weights = (body + head + norms) * elt + batch * cfg["hidden_size"] * elt     # + one embedding row per request
-    kv = ctx_tokens * 2 * cfg["num_key_value_heads"] * cfg["head_dim"] * layers * elt
-    return weights + kv
+    return weights + ctx_tokens * kv_bytes(cfg, layers, elt, cache_dtype)
 
 
 def prefill_flops(cfg, layers, T):
@@ -508,6 +513,7 @@ def main():
     ap.add_argument("--prompt-len", type=int, default=2048)
     ap.add_argument("--no-points", action="store_true", help="skip decode at batch 1 and 64")
     ap.add_argument("--dtype", default="bfloat16")
+    ap.add_argument("--cache-dtype", default="auto", choices=["auto", "mxfp4"], help="keys and values in the engine's dtype (auto) or in 4 bits")
     ap.add_argument("--shape", default="llama-3.1-8b", choices=sorted(SHAPES), help="sizes of the model (same architecture)")
     ap.add_argument("--max-context", type=int, default=0, metavar="N",
                     help="the model's context length (max_position_embeddings) instead of the shape's own")
@@ -550,7 +556,7 @@ def main():
     # The points away from the tuned one: (context, batch) pairs.  By default the model's limit at
     # batch 8 and, if the card has room for 64 requests of that length beside the weights, at batch 64.
     import torch
-    kv_per_token = 2 * cfg["num_key_value_heads"] * cfg["head_dim"] * layers * elt
+    kv_per_token = kv_bytes(cfg, layers, elt, args.cache_dtype)
     body, head = matmul_params(cfg, layers)
     weight_bytes = (body + (1 if cfg.get("tie_word_embeddings") else 2) * head) * elt
     total_mem = torch.cuda.get_device_properties(0).total_memory
@@ -566,7 +572,7 @@ def main():
     long_T = args.long_prefill or min(ctx_max, 32768)
     if not args.no_points:
         pool = max([pool, long_T + 4096] + [pool_for(*cb) for cb in ctx_points])
-    spec, runner = build_runner(cfg, args.dtype, max_tokens=pool, max_requests=max(64, args.mixed))
+    spec, runner = build_runner(cfg, args.dtype, max_tokens=pool, max_requests=max(64, args.mixed), cache_dtype=args.cache_dtype)
 
     read_gbs, mm_flops = measure_achievable(runner) if args.dtype == "bfloat16" else (None, None)
     if read_gbs:
@@ -585,16 +591,16 @@ def main():
         tps, step_s, ctx, _ = measure_decode(runner, cfg, B, P, args.steps, args.warmup, seed=2 + 100 * rep)
         runs.append((step_s, tps, ctx))
         log(f"decode batch {B}, repetition {rep + 1}: {tps:.1f} tok/s, {step_s * 1e3:.3f} ms/step, "
-            f"{decode_bytes(cfg, layers, B, ctx, elt) / step_s / 1e9:.0f} GB/s")
+            f"{decode_bytes(cfg, layers, B, ctx, elt, args.cache_dtype) / step_s / 1e9:.0f} GB/s")
     runs.sort()
     step_s, tps, ctx = runs[1]
-    achieved = decode_bytes(cfg, layers, B, ctx, elt) / step_s / 1e9
+    achieved = decode_bytes(cfg, layers, B, ctx, elt, args.cache_dtype) / step_s / 1e9
     points, checks = {}, {}
     if not args.no_points:
         def point(name, b, prompt_len, n, warm, seed, alone=False):
             t, sec, c, chk = measure_decode(runner, cfg, b, prompt_len, n, warm, seed=seed, alone=alone)
             points[name] = round(t, 1)
-            log(f"{name}: {t:.1f} tok/s, {sec * 1e3:.3f} ms/step, {decode_bytes(cfg, layers, b, c, elt) / sec / 1e9:.0f} GB/s")
+            log(f"{name}: {t:.1f} tok/s, {sec * 1e3:.3f} ms/step, {decode_bytes(cfg, layers, b, c, elt, args.cache_dtype) / sec / 1e9:.0f} GB/s")
             if chk is not None:
                 # One request's logits must not depend on the 63 beside it beyond the rounding of bfloat16
                 # operands summed in another order.  That rounding grows with the root of the depth:
@@ -605,7 +611,8 @@ def main():
                 checks[f"{name}_row0_vs_alone"] = chk
                 log(f"{name}: the first request's logits against the same request alone: {chk}")
                 bound = 5e-3 * (max(layers, 2) / 32.0) ** 0.5
-                if args.dtype == "bfloat16" and not (chk["mean"] <= bound and chk["max"] <= 10 * bound):
+                # (over a cache in 4 bits a key whose rounding falls the other way moves by a whole step: reported only)
+                if args.dtype == "bfloat16" and args.cache_dtype == "auto" and not (chk["mean"] <= bound and chk["max"] <= 10 * bound):
                     raise RuntimeError(f"{name}: a request's logits in the batch differ from the same request alone: {chk} "
                                        f"(allowed: mean {bound:.1e}, max {10 * bound:.1e} of the logit range)")
         for b in (1, 64):
@@ -654,6 +661,8 @@ def main():
         "points": points, "checks": checks,
         "repetitions_ms_per_step": [round(r[0] * 1e3, 4) for r in runs],
     }
+    if args.cache_dtype != "auto":
+        line["config"]["cache_dtype"] = args.cache_dtype
     if read_gbs:
         # the same two figures against what this GPU gave a kernel that only reads, and the matrix
         # kernel on one large product, in this very run
