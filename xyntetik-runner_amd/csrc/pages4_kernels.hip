@@ -397,8 +397,9 @@ extern "C" int xr_read_pages4(void* k_out, void* v_out, void* kc, void* ks, void
 }
 
 // ---------------------------------------------------------------- attention, any head size
-// k_attention_ref over 4-bit pages: a wave a token and query head, 64 keys a turn, a key a lane for the scores and channels a lane for the
-// values; the same options.  For what the matrix-core kernel does not take and a recorded step cannot read back first.
+// k_attention_ref over 4-bit pages: a workgroup a token and query head, its waves 64 keys a turn each, a key a lane for the scores and channels a
+// lane for the values; the same options.  For what the matrix-core kernel does not take and a recorded step cannot read back first.
+#define ANY4_WAVES 8
 struct Any4Args {
     Pages4 pages;
     const void* q;              // [T, H * D]
@@ -414,13 +415,13 @@ struct Any4Args {
 };
 
 template <typename T>
-__global__ __launch_bounds__(64) void k_attention_any4(Any4Args a) {
-    __shared__ float qs[256];
-    const int t = blockIdx.x, h = blockIdx.y, lane = threadIdx.x;
+__global__ __launch_bounds__(64 * ANY4_WAVES) void k_attention_any4(Any4Args a) {
+    __shared__ float qs[256], sums[ANY4_WAVES][256], ml[ANY4_WAVES][2];
+    const int t = blockIdx.x, h = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int pos = a.positions[t], kvh = h / (a.H / a.Hk);
     const int lo = a.chunk > 0 ? pos - pos % a.chunk : (a.window > 0 && pos - a.window + 1 > 0) ? pos - a.window + 1 : 0;
     const int kept = a.keep < lo ? a.keep : lo;
-    for (int d = lane; d < a.D; d += 64) qs[d] = ld<T>((const T*)a.q, ((size_t)t * a.H + h) * a.D + d);
+    for (int d = threadIdx.x; d < a.D; d += 64 * ANY4_WAVES) qs[d] = ld<T>((const T*)a.q, ((size_t)t * a.H + h) * a.D + d);
     __syncthreads();
     const int* bt = a.block_table + (size_t)a.req_of_token[t] * a.table_stride;
     const float slope = a.slopes ? a.slopes[h] : 0.f;
@@ -431,7 +432,7 @@ __global__ __launch_bounds__(64) void k_attention_any4(Any4Args a) {
     };
     float m = -INFINITY, l = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
     for (int seg = kept > 0 ? 0 : 1; seg < 2; ++seg)
-        for (int k0 = seg ? lo : 0, last = seg ? pos : kept - 1; k0 <= last; k0 += 64) {
+        for (int k0 = (seg ? lo : 0) + 64 * wave, last = seg ? pos : kept - 1; k0 <= last; k0 += 64 * ANY4_WAVES) {
             const int key = k0 + lane;
             const int page = key <= last ? page_at(key) : -1;
             float s = -INFINITY;
@@ -471,18 +472,24 @@ __global__ __launch_bounds__(64) void k_attention_any4(Any4Args a) {
             }
             m = mn;
         }
-    if (a.sinks) {
-        const float sk = a.sinks[h], mn = fmaxf(m, sk), corr = m == -INFINITY ? 0.f : expf(m - mn);
-        l = l * corr + expf(sk - mn);
+    // the waves' shares in one scale (a wave without keys has the sum 0)
 #pragma unroll
-        for (int dd = 0; dd < 4; ++dd) acc[dd] *= corr;
+    for (int dd = 0; dd < 4; ++dd) sums[wave][lane + 64 * dd] = acc[dd];
+    if (lane == 0) {
+        ml[wave][0] = m;
+        ml[wave][1] = l;
     }
+    __syncthreads();
+    float most = a.sinks ? a.sinks[h] : -INFINITY;
+    for (int w = 0; w < ANY4_WAVES; ++w) most = fmaxf(most, ml[w][0]);
+    float all = a.sinks ? expf(a.sinks[h] - most) : 0.f;
+    for (int w = 0; w < ANY4_WAVES; ++w) all += ml[w][1] == 0.f ? 0.f : ml[w][1] * expf(ml[w][0] - most);
     const float f = a.gate ? a.out_scale / (1.0f + expf(-a.gate[(size_t)t * a.ld_gate + h])) : a.out_scale;
     T* orow = (T*)a.out + (size_t)t * a.ld_out + (size_t)h * a.Dv;
-#pragma unroll
-    for (int dd = 0; dd < 4; ++dd) {
-        const int d = lane + 64 * dd;
-        if (d < a.Dv) st<T>(orow, d, l == 0.f ? 0.f : acc[dd] / l * f);      // (0: no key that exists and no sink)
+    for (int d = threadIdx.x; d < a.Dv; d += 64 * ANY4_WAVES) {
+        float o = 0.f;
+        for (int w = 0; w < ANY4_WAVES; ++w) o += ml[w][1] == 0.f ? 0.f : sums[w][d] * expf(ml[w][0] - most);
+        st<T>(orow, d, all == 0.f ? 0.f : o / all * f);      // (0: no key that exists and no sink)
     }
 }
 
@@ -506,8 +513,8 @@ extern "C" int xr_attention_any4(void* out, const void* q, void* kc, void* ks, v
     a.slopes = slopes; a.sinks = sinks; a.gate = gate; a.table_stride = table_stride; a.n_pages = n_pages; a.H = H; a.Hk = Hk;
     a.D = D; a.Dv = Dv; a.page_shift = ilog2_exact(page_size); a.page_size = page_size; a.window = window; a.chunk = chunk; a.keep = keep;
     a.ld_gate = ld_gate; a.ld_out = ld_out; a.scale = scale; a.cap = cap; a.out_scale = out_scale;
-    if (dtype == XR_F32) k_attention_any4<float><<<dim3(T, H), 64, 0, stream>>>(a);
-    else k_attention_any4<bf16_t><<<dim3(T, H), 64, 0, stream>>>(a);
+    if (dtype == XR_F32) k_attention_any4<float><<<dim3(T, H), 64 * ANY4_WAVES, 0, stream>>>(a);
+    else k_attention_any4<bf16_t><<<dim3(T, H), 64 * ANY4_WAVES, 0, stream>>>(a);
     XR_CHECK_LAUNCH("attention_any4");
     return XR_OK;
 }
