@@ -147,6 +147,27 @@ def test_write(ops, case, dt):
                         assert np.array_equal(c0[p, :, off], c1[p, :, off])
 
 
+def test_rows_in_any_order_and_without_a_page(ops):
+    """Rows of a request that are not one after the other, with first and last as if they were; positions past the table, requests past its rows,
+    pages given back or past the pool: written nowhere, read as zeros."""
+    from xyntetik_runner_amd.csrc.ops import FourBitPages
+    rng = np.random.default_rng(8)
+    kp, vp = (FourBitPages.zeros(4, 2, 16, 32, values, DEV) for values in (False, True))
+    pos = [0, 5, 2, 3, 4, 1, 6, 7, 16, 17, 18, 19, 20, 21, 22, 23, 40, 33, 9, 10, 47]
+    req = [0] * 8 + [1] * 4 + [0] * 4 + [0, 1, 2, -1, 0]
+    table = torch.tensor([[1, 2], [3, 9]], dtype=torch.int32, device=DEV)      # (request 0: two pages; 1: one, and one that is none)
+    x = torch.tensor(rng.normal(size=(len(pos), 2 * 32)), dtype=torch.float32, device=DEV)
+    p, r = (torch.tensor(v, dtype=torch.int32, device=DEV) for v in (pos, req))
+    ops.rope_kv_write(None, x, x, None, kp, vp, p, r, table, None, 0, 2, 32, 0, False, 1.0, 16)
+    want = F.rounded(x.double().cpu().numpy().reshape(-1, 2, 32))[2]
+    for i, (a, b) in enumerate(zip(pos, req)):
+        if b not in (0, 1) or a >= 32 or (b == 1 and a >= 16):
+            want[i] = 0.0
+    for got in ops.read_rows(kp, vp, p, r, table, torch.float32):
+        assert np.array_equal(got.double().cpu().numpy().reshape(want.shape), want)
+    assert int((kp.scales != 0).sum()) == 2 * sum(1 for i in range(len(pos)) if want[i].any()) and not kp.codes[0].any()
+
+
 def test_write_of_special_numbers(ops):
     """Blocks of zeros, of one sign, with ties, at both ends of the scales, with a NaN or an infinity: the oracle's bytes."""
     rng = np.random.default_rng(5)
@@ -482,6 +503,11 @@ def test_refusals(ops):
         with pytest.raises(KernelError):
             call()
             pytest.fail(f"call {i} was not refused")
+    for cpu in (lambda: ops.read_rows(kp, vp, ctx.positions.cpu(), ctx.req_of_token, ctx.block_table(0), torch.bfloat16),
+                lambda: ops.attention(q.cpu(), kp, vp, ctx, 0, 4, 2, 64, 16, 1.0),
+                lambda: ops.rope_kv_write(None, x.cpu(), x, None, kp, vp, ctx.positions, ctx.req_of_token, ctx.block_table(0), None, 0, 2, 64, 0, False, 1.0, 16)):
+        with pytest.raises(KernelError):
+            cpu()
     # and the smallest calls that are allowed
     none = torch.zeros((0,), dtype=torch.int32, device=DEV)
     assert [t.shape for t in ops.read_rows(kp, vp, none, none, ctx.block_table(0), torch.bfloat16)] == [(0, 128), (0, 128)]

@@ -120,8 +120,8 @@ _PROTOS = {
     "xr_qkv_store": [_p, _p, _p, _p, _p, _p, _i, _p, _p, _p, _i, _i, _i, _i, _i, _i, _i, _i, _p],
     "xr_pool_blocks": [_p, _p, _p, _p, _p, _p, _p, _i, _p, _i, _i, _i, _i, _i, _i, _i, _i, _i, _p],
     "xr_attention_pool_partial": [_p, _p, _p, _p, _p, _p, _i, _p, _i, _i, _i, _i, _i, _i, _f, _i, _i, _i, _p],
-    "xr_rope_kv_write4": [_p, _p, _p, _i, _p] + [_p] * 4 + [_i] + [_p] * 3 + [_i, _p] + [_i] * 7 + [_f, _i, _i, _i, _p],
-    "xr_read_rows4": [_p, _p] + [_p] * 4 + [_i] + [_p] * 3 + [_i] * 7 + [_p],
+    "xr_rope_kv_write4": [_p, _p, _p, _i, _p] + [_p] * 4 + [_i] + [_p] * 3 + [_i, _i, _p] + [_i] * 7 + [_f, _i, _i, _i, _p],
+    "xr_read_rows4": [_p, _p] + [_p] * 4 + [_i] + [_p] * 3 + [_i] * 8 + [_p],
     "xr_read_pages4": [_p, _p] + [_p] * 4 + [_i, _p, _i, _p] + [_i] * 6 + [_p],
     "xr_attention_any4": [_p, _p] + [_p] * 4 + [_i] + [_p] * 3 + [_i] * 7 + [_f] + [_i] * 4 + [_p, _p, _f, _p, _i, _f, _i, _p],
     "xr_attention_pooled": [_p, _p, _p, _p, _p, _p, _p, _p, _p, _i, _p, _i, _i, _i, _i, _i, _i, _i, _f, _i, _i, _i, _p],
@@ -215,6 +215,9 @@ class FourBitPages:
     def zeros(cls, pages: int, heads: int, page_size: int, dim: int, values: bool, device) -> "FourBitPages":
         codes, scales = cls.shapes(pages, heads, page_size, dim, values)
         return cls(torch.zeros(codes, dtype=torch.uint8, device=device), torch.zeros(scales, dtype=torch.uint8, device=device), dim)
+
+    def get_device(self) -> int:
+        return self.codes.get_device()
 
     @property
     def dtype(self):            # (what takes 16- or 32-bit caches refuses these by it)
@@ -777,10 +780,10 @@ class Ops:
         channels of every query and key head come in ``paired_order``.  Caches that are ``FourBitPages`` take their
         blocks' codes and scales (values may have another size than keys there: as the cache says).
         """
-        self._dev(q_in, k_in, v_in, q_out, k_cache, v_cache, positions, req_of_token, block_table, inv_freq)
         if isinstance(k_cache, FourBitPages) or isinstance(v_cache, FourBitPages):
             return self._rope_kv_write4(q_in, k_in, v_in, q_out, k_cache, v_cache, positions, req_of_token, block_table, inv_freq, H, Hk, D, rot,
                                         interleaved, mscale, page_size, paired)
+        self._dev(q_in, k_in, v_in, q_out, k_cache, v_cache, positions, req_of_token, block_table, inv_freq)
         T = positions.numel()
         ins = [t for t in (q_in, k_in, v_in) if t is not None]
         if any(t.dtype != torch.float32 or t.stride(-1) != 1 for t in ins):
@@ -813,6 +816,14 @@ class Ops:
                           f"{Hk} heads of {D} in pages of {page_size}")
 
     @staticmethod
+    def _here(what: str, *ts) -> None:
+        """Every operand must be on the current device, whose stream the kernels are queued on."""
+        here = torch._C._cuda_getDevice()
+        for t in ts:
+            if t is not None and t.get_device() != here:
+                raise KernelError(f"{what}: an operand is not on the current GPU (there is no CPU path)")
+
+    @staticmethod
     def _ints(what: str, n: int, *ts: torch.Tensor) -> None:
         for t in ts:
             if t.dtype is not torch.int32 or t.shape != (n,) or not t.is_contiguous():
@@ -825,6 +836,7 @@ class Ops:
 
     def _rope_kv_write4(self, q_in, k_in, v_in, q_out, k_pages, v_pages, positions, req_of_token, block_table, inv_freq, H: int, Hk: int,
                         D: int, rot: int, interleaved: bool, mscale: float, page_size: int, paired: bool) -> None:
+        self._here("rope_kv_write", q_in, k_in, v_in, q_out, k_pages, v_pages, positions, req_of_token, block_table, inv_freq)
         pages = self._pages4("rope_kv_write", k_pages, v_pages, Hk, D, page_size)
         T, Dv = positions.numel(), v_pages.dim
         if k_in is None or v_in is None or req_of_token is None or (q_in is None) != (q_out is None):
@@ -845,7 +857,7 @@ class Ops:
             raise KernelError(f"rope_kv_write: {rot // 2} 32-bit frequencies are needed")
         self.lib.check(self.lib.xr_rope_kv_write4(
             _ptr(q_in), k_in.data_ptr(), v_in.data_ptr(), stride, _ptr(q_out), *pages, positions.data_ptr(), req_of_token.data_ptr(),
-            block_table.data_ptr(), block_table.stride(0), _ptr(inv_freq) if rot else None, T, H, Hk, D, Dv, rot, 1 if interleaved else 0,
+            block_table.data_ptr(), block_table.stride(0), block_table.shape[0], _ptr(inv_freq) if rot else None, T, H, Hk, D, Dv, rot, 1 if interleaved else 0,
             float(mscale), page_size, dtype_code(q_out.dtype) if q_out is not None else XR_F32, 1 if paired else 0, _stream()))
 
     def read_rows(self, k_pages: "FourBitPages", v_pages: "FourBitPages", positions: torch.Tensor, req_of_row: torch.Tensor,
@@ -853,7 +865,7 @@ class Ops:
         """Cached keys ``[n, heads * dim]`` and values of any list of (request, position), as ``dtype`` numbers; a row whose position
         has no page in ``block_table`` reads as zeros."""
         pages = self._pages4("read_rows", k_pages, v_pages)
-        self._dev(k_pages, positions, req_of_row, block_table)
+        self._here("read_rows", k_pages, positions, req_of_row, block_table)
         n = positions.numel()
         self._ints("read_rows", n, positions, req_of_row)
         self._table("read_rows", block_table)
@@ -861,7 +873,7 @@ class Ops:
         k = torch.empty((n, Hk * D), dtype=dtype, device=k_pages.device)
         v = torch.empty((n, Hk * Dv), dtype=dtype, device=k_pages.device)
         self.lib.check(self.lib.xr_read_rows4(k.data_ptr(), v.data_ptr(), *pages, positions.data_ptr(), req_of_row.data_ptr(),
-                                              block_table.data_ptr(), block_table.stride(0), n, Hk, D, Dv, k_pages.page_size, dtype_code(dtype),
+                                              block_table.data_ptr(), block_table.stride(0), block_table.shape[0], n, Hk, D, Dv, k_pages.page_size, dtype_code(dtype),
                                               _stream()))
         return k, v
 
@@ -878,7 +890,7 @@ class Ops:
         if window and chunk:
             raise KernelError("read_pages: a layer reads a window or its chunk, not both")
         block_table = ctx.block_table(group)
-        self._dev(k_pages, block_table)
+        self._here("read_pages", k_pages, block_table)
         self._table("read_pages", block_table)
         Hk, D, Dv, P = k_pages.heads, k_pages.dim, v_pages.dim, k_pages.page_size
         mask = Chunked(int(chunk)) if chunk else window
@@ -1057,6 +1069,7 @@ class Ops:
         self._contig(q, "attention queries")
         four = isinstance(k_cache, FourBitPages) or isinstance(v_cache, FourBitPages)
         if four:
+            self._here("attention", q, k_cache, v_cache, positions, req_of_token, block_table, slopes, sinks, gate, out)
             pages = self._pages4("attention", k_cache, v_cache, Hk, D, page_size)
             if q.shape != (T, H * D) or v_cache.dim != (int(v_head_dim) if v_head_dim is not None else D):
                 raise KernelError(f"attention: queries {tuple(q.shape)} or values of {v_cache.dim} do not fit {T} rows of {H} heads of {D}")

@@ -20,7 +20,7 @@ struct Write4Args {
     const int* positions;   // [T]
     const int* req_of_token;
     const int* block_table; // [B, table_stride]
-    int table_stride, n_pages;
+    int table_stride, n_requests, n_pages;
     const float* inv_freq;  // [rot / 2] or null
     int H, Hk, D, Dv, rot, interleaved, paired;
     float mscale;
@@ -67,7 +67,7 @@ __global__ __launch_bounds__(256) void k_rope_kv_write4(Write4Args a) {
     const int pos = a.positions[t];
     const int half = a.rot >> 1;
     const int u0 = blockIdx.y * a.per_block, u1 = min(a.units, u0 + a.per_block);
-    const int req = a.req_of_token ? a.req_of_token[t] : 0;
+    const int req = a.req_of_token[t];
     // a unit: what it is, its head, its first channel, and its numbers as they come
     struct Unit { int h, c0, D; bool is_q, is_v; const float* src; float x[8], y[8]; };
     auto unit = [&](int u) __attribute__((always_inline)) {
@@ -104,13 +104,14 @@ __global__ __launch_bounds__(256) void k_rope_kv_write4(Write4Args a) {
         cs[j & 7][j >> 3] = make_float2(c * a.mscale, s * a.mscale);
     }
     const int bi = pos >> a.page_shift, off = pos & a.page_mask;
-    const int page = bi >= 0 && bi < a.table_stride ? a.block_table[(size_t)req * a.table_stride + bi] : -1;
-    const bool there = (unsigned)page < (unsigned)a.n_pages;
-    // the 8 positions of a page that this one belongs to: whole in this step?  (A request's tokens of a step are consecutive rows at
-    // consecutive positions.)
+    const int page = bi >= 0 && bi < a.table_stride && (unsigned)req < (unsigned)a.n_requests ? a.block_table[(size_t)req * a.table_stride + bi] : -1;
+    const bool there = (unsigned)page < (unsigned)a.n_pages;          // (what has no page is written nowhere)
+    // the 8 positions of a page that this one belongs to: whole in this step, row by row?
     const int lead = t - (pos & 7);
-    const bool whole = lead >= 0 && lead + 7 < (int)gridDim.x && a.req_of_token[lead] == req && a.req_of_token[lead + 7] == req &&
-                       a.positions[lead] == pos - (pos & 7) && a.positions[lead + 7] == pos - (pos & 7) + 7;
+    bool whole = lead >= 0 && lead + 7 < (int)gridDim.x;
+    if (whole)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) whole &= a.req_of_token[lead + i] == req && a.positions[lead + i] == pos - (pos & 7) + i;
     __syncthreads();
     for (int u = first; u < u1; u += 256) {
         Unit w = u == first ? ahead : unit(u);
@@ -218,8 +219,9 @@ static int check_pages4(const char* what, const Pages4& p, int Hk, int D, int Dv
 
 extern "C" int xr_rope_kv_write4(const float* q_in, const float* k_in, const float* v_in, int in_stride, void* q_out,
                                  void* kc, void* ks, void* vc, void* vs, int n_pages, const int* positions, const int* req_of_token,
-                                 const int* block_table, int table_stride, const float* inv_freq, int T, int H, int Hk, int D, int Dv,
-                                 int rot, int interleaved, float mscale, int page_size, int q_dtype, int paired, hipStream_t stream) {
+                                 const int* block_table, int table_stride, int n_requests, const float* inv_freq, int T, int H, int Hk,
+                                 int D, int Dv, int rot, int interleaved, float mscale, int page_size, int q_dtype, int paired,
+                                 hipStream_t stream) {
     Write4Args a;
     a.pages = Pages4{(uint8_t*)kc, (uint8_t*)ks, (uint8_t*)vc, (uint8_t*)vs};
     const int rc = check_pages4("rope_kv_write", a.pages, Hk, D, Dv, page_size, n_pages);
@@ -233,7 +235,7 @@ extern "C" int xr_rope_kv_write4(const float* q_in, const float* k_in, const flo
     XR_REQUIRE(k_in && v_in && block_table && req_of_token && positions, "rope_kv_write: keys and values to cache but a null operand");
     XR_REQUIRE(H == 0 || (q_in && q_out && ((uintptr_t)q_out & 15) == 0), "rope_kv_write: queries but a null operand, or rows that are not 16-byte aligned");
     a.q_in = q_in; a.k_in = k_in; a.v_in = v_in; a.in_stride = in_stride; a.q_out = q_out;
-    a.positions = positions; a.req_of_token = req_of_token; a.block_table = block_table; a.table_stride = table_stride; a.n_pages = n_pages;
+    a.positions = positions; a.req_of_token = req_of_token; a.block_table = block_table; a.table_stride = table_stride; a.n_requests = n_requests; a.n_pages = n_pages;
     a.inv_freq = inv_freq; a.H = H; a.Hk = Hk; a.D = D; a.Dv = Dv; a.rot = rot; a.interleaved = interleaved; a.paired = paired ? 1 : 0;
     a.mscale = mscale; a.page_shift = ilog2_exact(page_size); a.page_mask = page_size - 1; a.page_size = page_size;
     a.lanes_k = blocks4(D) * 4; a.lanes_v = blocks4(Dv) * 4;
@@ -282,7 +284,7 @@ struct Read4Args {
     const int* slots;           // pages: [n, 3] request, place in its table, positions of the page that are the request's
     void* k_out;                // rows: [n, Hk * D]; pages: [n, Hk, page_size, D]
     void* v_out;                // rows: [n, Hk * Dv]; pages: [n, Hk, Dv, page_size]
-    int table_stride, n_pages, Hk, D, Dv, page_shift, page_size;
+    int table_stride, n_requests, n_pages, Hk, D, Dv, page_shift, page_size;
     size_t total;               // threads of all rows, keys' first
     size_t k_total;
 };
@@ -297,7 +299,8 @@ __global__ __launch_bounds__(256) void k_read_rows4(Read4Args a) {
         const size_t r = j / per;
         const int w = (int)(j - r * per), h = w / (D >> 3), c0 = (w - h * (D >> 3)) * 8;
         const int pos = a.positions[r], bi = pos >> a.page_shift, off = pos & (a.page_size - 1);
-        const int page = bi >= 0 && bi < a.table_stride ? a.block_table[(size_t)a.req_of_row[r] * a.table_stride + bi] : -1;
+        const int req = a.req_of_row[r];
+        const int page = bi >= 0 && bi < a.table_stride && (unsigned)req < (unsigned)a.n_requests ? a.block_table[(size_t)req * a.table_stride + bi] : -1;
         float x[8];
         if ((unsigned)page >= (unsigned)a.n_pages) {
 #pragma unroll
@@ -352,8 +355,8 @@ __global__ __launch_bounds__(256) void k_read_pages4(Read4Args a) {
 }
 
 extern "C" int xr_read_rows4(void* k_out, void* v_out, void* kc, void* ks, void* vc, void* vs, int n_pages, const int* positions,
-                             const int* req_of_row, const int* block_table, int table_stride, int n, int Hk, int D, int Dv,
-                             int page_size, int dtype, hipStream_t stream) {
+                             const int* req_of_row, const int* block_table, int table_stride, int n_requests, int n, int Hk, int D,
+                             int Dv, int page_size, int dtype, hipStream_t stream) {
     Read4Args a;
     a.pages = Pages4{(uint8_t*)kc, (uint8_t*)ks, (uint8_t*)vc, (uint8_t*)vs};
     const int rc = check_pages4("read_rows", a.pages, Hk, D, Dv, page_size, n_pages);
@@ -363,7 +366,7 @@ extern "C" int xr_read_rows4(void* k_out, void* v_out, void* kc, void* ks, void*
     XR_REQUIRE(k_out && v_out && positions && req_of_row && block_table, "read_rows: a null operand");
     XR_REQUIRE((((uintptr_t)k_out | (uintptr_t)v_out) & 15) == 0, "read_rows: outputs must be 16-byte aligned");
     a.positions = positions; a.req_of_row = req_of_row; a.block_table = block_table; a.slots = nullptr;
-    a.k_out = k_out; a.v_out = v_out; a.table_stride = table_stride; a.n_pages = n_pages; a.Hk = Hk; a.D = D; a.Dv = Dv;
+    a.k_out = k_out; a.v_out = v_out; a.table_stride = table_stride; a.n_requests = n_requests; a.n_pages = n_pages; a.Hk = Hk; a.D = D; a.Dv = Dv;
     a.page_shift = ilog2_exact(page_size); a.page_size = page_size;
     a.k_total = (size_t)n * Hk * (D >> 3);
     a.total = a.k_total + (size_t)n * Hk * (Dv >> 3);
@@ -387,7 +390,7 @@ extern "C" int xr_read_pages4(void* k_out, void* v_out, void* kc, void* ks, void
     XR_REQUIRE(k_out && v_out && slots && block_table, "read_pages: a null operand");
     XR_REQUIRE((((uintptr_t)k_out | (uintptr_t)v_out) & 15) == 0, "read_pages: outputs must be 16-byte aligned");
     a.positions = nullptr; a.req_of_row = nullptr; a.block_table = block_table; a.slots = slots;
-    a.k_out = k_out; a.v_out = v_out; a.table_stride = table_stride; a.n_pages = n_pages; a.Hk = Hk; a.D = D; a.Dv = Dv;
+    a.k_out = k_out; a.v_out = v_out; a.table_stride = table_stride; a.n_requests = 0; a.n_pages = n_pages; a.Hk = Hk; a.D = D; a.Dv = Dv;
     a.page_shift = ilog2_exact(page_size); a.page_size = page_size; a.total = a.k_total = 0;
     const unsigned grid = (unsigned)n * (unsigned)Hk;
     if (dtype == XR_F32) k_read_pages4<float><<<grid, 256, 0, stream>>>(a);
