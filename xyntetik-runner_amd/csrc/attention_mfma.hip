@@ -1670,6 +1670,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES, FOUR_PER_CU) void k_attn_few4(AttnA
         }
         const bool whole = kt + 32 <= kend && kt + 31 <= pos_min && kt >= lo_max;
         if (!whole) {
+            asm volatile("; hidden keys");      // (a branch: as a selection its 40 instructions were every tile's)
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 const int key = kt + 8 * quad + e;

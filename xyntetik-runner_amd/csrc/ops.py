@@ -1064,10 +1064,11 @@ class Ops:
         back first (``read_pages``), but in steps that are being recorded, which a 32-bit kernel then serves from the codes.
         """
         positions, req_of_token, block_table = ctx.positions, ctx.req_of_token, ctx.block_table(group)
-        self._dev(q, k_cache, v_cache, positions, req_of_token, block_table)
         T = positions.numel()
-        self._contig(q, "attention queries")
         four = isinstance(k_cache, FourBitPages) or isinstance(v_cache, FourBitPages)
+        if not four:
+            self._dev(q, k_cache, v_cache, positions, req_of_token, block_table)
+        self._contig(q, "attention queries")
         if four:
             self._here("attention", q, k_cache, v_cache, positions, req_of_token, block_table, slopes, sinks, gate, out)
             pages = self._pages4("attention", k_cache, v_cache, Hk, D, page_size)
@@ -1101,7 +1102,7 @@ class Ops:
                 lib = self.attention_lib(D, Dv)
                 part_o = part_ml = None
                 if plan.n_slots:        # partial results, and behind them their maxima and sums
-                    parts = torch.empty((plan.n_slots * Hk * 32, Dv + 2), dtype=torch.float32, device=q.device)
+                    parts = q.new_empty((plan.n_slots * Hk * 32, Dv + 2), dtype=torch.float32)
                     part_o = parts.data_ptr()
                     part_ml = part_o + plan.n_slots * Hk * 32 * Dv * 4
                 if plan.n_few:
