@@ -196,7 +196,7 @@ class FourBitPages:
             raise KernelError("4-bit pages: codes and scales must be uint8 on one device")
         if not codes.is_contiguous() or not scales.is_contiguous() or codes.data_ptr() % 16 or scales.data_ptr() % 8:
             raise KernelError("4-bit pages: codes and scales must be contiguous, 16 and 8 bytes aligned")
-        self.device, self.is_cuda = codes.device, codes.is_cuda
+        self.device, self.is_cuda, self.index = codes.device, codes.is_cuda, codes.get_device()
         # what a pair of keys and values has in common, and where the bytes are (the tensors are never replaced)
         self.layout = (self.num_pages, self.heads, self.page_size, self.device)
         self.pointers = (codes.data_ptr(), scales.data_ptr())
@@ -217,7 +217,7 @@ class FourBitPages:
         return cls(torch.zeros(codes, dtype=torch.uint8, device=device), torch.zeros(scales, dtype=torch.uint8, device=device), dim)
 
     def get_device(self) -> int:
-        return self.codes.get_device()
+        return self.index
 
     @property
     def dtype(self):            # (what takes 16- or 32-bit caches refuses these by it)
@@ -230,6 +230,19 @@ class FourBitPages:
     @property
     def nbytes(self) -> int:
         return self.codes.numel() + self.scales.numel()
+
+
+class _PagesOf:
+    """A step's context with another block table: that of pages read back."""
+
+    def __init__(self, ctx, table: torch.Tensor):
+        self._ctx, self._table = ctx, table
+
+    def block_table(self, group: int) -> torch.Tensor:
+        return self._table
+
+    def __getattr__(self, name):
+        return getattr(self._ctx, name)
 
 
 class F32Weight(torch.Tensor):
@@ -889,11 +902,12 @@ class Ops:
             raise KernelError("read_pages: the lengths of a recorded step's requests change from replay to replay")
         if window and chunk:
             raise KernelError("read_pages: a layer reads a window or its chunk, not both")
+        dtype_code(dtype)
         block_table = ctx.block_table(group)
         self._here("read_pages", k_pages, block_table)
         self._table("read_pages", block_table)
         Hk, D, Dv, P = k_pages.heads, k_pages.dim, v_pages.dim, k_pages.page_size
-        mask = Chunked(int(chunk)) if chunk else window
+        mask = Chunked(int(chunk)) if chunk else window or None
         key = ("read_pages", group, P, None if requests is None else tuple(requests), mask, keep_first if mask else 0)
         made = ctx.shared.get(key)
         if made is None:
@@ -1063,19 +1077,14 @@ class Ops:
         their own (bfloat16, sizes in whole blocks of 32, pages of at least 32 positions, no kept first keys); the pages of others are read
         back first (``read_pages``), but in steps that are being recorded, which a 32-bit kernel then serves from the codes.
         """
+        if isinstance(k_cache, FourBitPages) or isinstance(v_cache, FourBitPages):
+            return self._attention4(q, k_cache, v_cache, ctx, group, H, Hk, D, page_size, scale, window, slopes, chunk, keep_first, sinks,
+                                    v_head_dim, softcap, gate, out_scale, out)
         positions, req_of_token, block_table = ctx.positions, ctx.req_of_token, ctx.block_table(group)
+        self._dev(q, k_cache, v_cache, positions, req_of_token, block_table)
         T = positions.numel()
-        four = isinstance(k_cache, FourBitPages) or isinstance(v_cache, FourBitPages)
-        if not four:
-            self._dev(q, k_cache, v_cache, positions, req_of_token, block_table)
         self._contig(q, "attention queries")
-        if four:
-            self._here("attention", q, k_cache, v_cache, positions, req_of_token, block_table, slopes, sinks, gate, out)
-            pages = self._pages4("attention", k_cache, v_cache, Hk, D, page_size)
-            if q.shape != (T, H * D) or v_cache.dim != (int(v_head_dim) if v_head_dim is not None else D):
-                raise KernelError(f"attention: queries {tuple(q.shape)} or values of {v_cache.dim} do not fit {T} rows of {H} heads of {D}")
-            dtype_code(q.dtype)
-        elif q.dtype != k_cache.dtype or q.dtype != v_cache.dtype:
+        if q.dtype != k_cache.dtype or q.dtype != v_cache.dtype:
             raise KernelError("attention: queries and cache differ in dtype")
         if H % Hk:
             raise KernelError(f"attention: {H} query heads are not a multiple of {Hk} key/value heads")
@@ -1095,39 +1104,6 @@ class Ops:
                     raise KernelError(f"attention: the {name} must be float32 [{H}]")
         if chunk and window:
             raise KernelError("attention: a layer reads a window or its chunk, not both")
-        if four:
-            if self._few4_ok(q, out, ctx, D, Dv, page_size, scale, keep_first, softcap, slopes):
-                mask = Chunked(int(chunk)) if chunk else window
-                plan = ctx.attention_plan(group, H // Hk, mask, Hk, page_size, few_rows=3, few_channels=D + Dv)      # (FEW_FOUR)
-                lib = self.attention_lib(D, Dv)
-                part_o = part_ml = None
-                if plan.n_slots:        # partial results, and behind them their maxima and sums
-                    parts = q.new_empty((plan.n_slots * Hk * 32, Dv + 2), dtype=torch.float32)
-                    part_o = parts.data_ptr()
-                    part_ml = part_o + plan.n_slots * Hk * 32 * Dv * 4
-                if plan.n_few:
-                    lib.check(lib.xr_attention_few4(
-                        out.data_ptr(), q.data_ptr(), *pages[:4], plan.few.data_ptr(), plan.n_few, plan.counters.data_ptr(), block_table.data_ptr(),
-                        block_table.stride(0), part_o, part_ml, H, Hk, D, Dv, page_size, float(scale), int(window or 0), int(chunk or 0),
-                        _ptr(slopes), _ptr(sinks), float(softcap), *gating, _stream()))
-                if not plan.n_items and not plan.n_cta_items:
-                    return out
-                if getattr(ctx, "knows_lengths", False) and out.stride(0) % 4 == 0 and out.data_ptr() % 8 == 0:
-                    # requests of many rows: their pages once as 16-bit ones, which every row block then reads
-                    k16, v16, table = self.read_pages(k_cache, v_cache, ctx, group, q.dtype, plan.rest, window, chunk)
-                    lib.check(lib.xr_attention_mfma(
-                        out.data_ptr(), q.data_ptr(), k16.data_ptr(), v16.data_ptr(), plan.items.data_ptr(), plan.n_items, plan.n_cta_items, None, 0,
-                        None, _ptr(plan.jobs), plan.n_jobs, ctx.cu_q.data_ptr(), ctx.starts_dev.data_ptr(), table.data_ptr(), table.stride(0),
-                        part_o, part_ml, H, Hk, D, Dv, page_size, float(scale), int(window or 0), int(chunk or 0), _ptr(slopes),
-                        _ptr(sinks), float(softcap), *gating, _stream()))
-                    return out
-            if not getattr(ctx, "knows_lengths", False):
-                self.lib.check(self.lib.xr_attention_any4(
-                    out.data_ptr(), q.data_ptr(), *pages, positions.data_ptr(), req_of_token.data_ptr(), block_table.data_ptr(), block_table.stride(0),
-                    T, H, Hk, D, Dv, page_size, float(scale), int(window or 0), int(chunk or 0), int(keep_first), dtype_code(q.dtype), _ptr(slopes),
-                    _ptr(sinks), float(softcap), *gating, _stream()))
-                return out
-            k_cache, v_cache, block_table = self.read_pages(k_cache, v_cache, ctx, group, q.dtype, window=window, chunk=chunk, keep_first=keep_first)
         if (self.attention_on_matrix_cores(q.dtype, D, Dv, page_size) and not (softcap and slopes is not None)
                 and (D == Dv or not keep_first) and out.stride(0) % 4 == 0 and out.data_ptr() % 8 == 0):
             # The first keys that a window has passed enter the same softmax as a partial result of its own, which
@@ -1178,11 +1154,63 @@ class Ops:
         more = {**({"extra_slot": True} if extra else {}), **({"few_rows": 2 if D + Dv <= 256 else 1, "few_channels": D + Dv} if few else {})}
         return ctx.attention_plan(group, H // Hk, mask, Hk, page_size, **more)
 
-    def _few4_ok(self, q, out, ctx, D: int, Dv: int, page_size: int, scale: float, keep_first: int, softcap: float, slopes) -> bool:
-        """Whether the matrix-core kernel for few rows over 4-bit pages takes a call's operands."""
-        return (self.use_mfma and q.dtype == torch.bfloat16 and D % 32 == 0 and Dv % 32 == 0 and page_size >= 32 and scale > 0.0 and not keep_first
-                and not (softcap and slopes is not None) and getattr(ctx, "plans_few_rows", False) and q.data_ptr() % 16 == 0
-                and out.stride(0) % 2 == 0 and out.data_ptr() % 4 == 0)
+    def _attention4(self, q, k_pages, v_pages, ctx, group: int, H: int, Hk: int, D: int, page_size: int, scale: float, window, slopes, chunk, keep_first: int,
+                    sinks, v_head_dim, softcap: float, gate, out_scale: float, out) -> torch.Tensor:
+        """``attention`` over 4-bit pages."""
+        pages = self._pages4("attention", k_pages, v_pages, Hk, D, page_size)
+        positions, req_of_token, block_table, Dv = ctx.positions, ctx.req_of_token, ctx.block_table(group), v_pages.dim
+        self._here("attention", q, k_pages, positions, req_of_token, block_table, slopes, sinks, gate, out)
+        T = positions.numel()
+        dtype = q.dtype
+        if q.shape != (T, H * D) or not q.is_contiguous() or H % Hk or (v_head_dim is not None and v_head_dim != Dv) or (v_head_dim is None and Dv != D):
+            raise KernelError(f"attention: queries {tuple(q.shape)} (contiguous), values of {Dv} channels and {Hk} key/value heads do not fit "
+                              f"{T} rows of {H} heads of {D} and {v_head_dim if v_head_dim is not None else D}")
+        if chunk and window:
+            raise KernelError("attention: a layer reads a window or its chunk, not both")
+        if out is None:
+            out = q.new_empty((T, H * Dv))
+        elif out.dtype != dtype or out.shape != (T, H * Dv) or out.stride(1) != 1:
+            raise KernelError(f"attention: the output must be a {dtype} view [{T}, {H * Dv}] with unit column stride")
+        if gate is not None and (gate.dtype != torch.float32 or gate.shape != (T, H) or gate.stride(1) != 1):
+            raise KernelError(f"attention: the gate must be a float32 view [{T}, {H}]")
+        for t in (slopes, sinks):
+            if t is not None and (t.dtype != torch.float32 or t.numel() != H or not t.is_contiguous()):
+                raise KernelError(f"attention: slopes and sinks must be float32 [{H}]")
+        window, chunk, ld_out, at = int(window or 0), int(chunk or 0), out.stride(0), out.data_ptr()
+        gating = (_ptr(gate), gate.stride(0) if gate is not None else 0, float(out_scale), ld_out, _stream())
+        knows = getattr(ctx, "knows_lengths", False)
+        if (dtype is torch.bfloat16 and self.use_mfma and D % 32 == 0 and Dv % 32 == 0 and page_size >= 32 and scale > 0.0 and not keep_first
+                and not (softcap and slopes is not None) and getattr(ctx, "plans_few_rows", False) and q.data_ptr() % 16 == 0 and ld_out % 4 == 0 and at % 8 == 0):
+            plan = ctx.attention_plan(group, H // Hk, Chunked(chunk) if chunk else window or None, Hk, page_size, few_rows=3, few_channels=D + Dv)   # (FEW_FOUR)
+            rest = plan.n_items or plan.n_cta_items
+            if not rest or knows:
+                lib = self.attention_lib(D, Dv)
+                part_o = part_ml = None
+                if plan.n_slots:        # partial results, and behind them their maxima and sums
+                    parts = q.new_empty((plan.n_slots * Hk * 32, Dv + 2), dtype=torch.float32)
+                    part_o = parts.data_ptr()
+                    part_ml = part_o + plan.n_slots * Hk * 32 * Dv * 4
+                if plan.n_few:
+                    lib.check(lib.xr_attention_few4(
+                        at, q.data_ptr(), *pages[:4], plan.few.data_ptr(), plan.n_few, plan.counters.data_ptr(), block_table.data_ptr(),
+                        block_table.stride(0), part_o, part_ml, H, Hk, D, Dv, page_size, float(scale), window, chunk, _ptr(slopes), _ptr(sinks),
+                        float(softcap), *gating))
+                if rest:
+                    # requests of many rows: their pages once as 16-bit ones, which every row block then reads
+                    k16, v16, table = self.read_pages(k_pages, v_pages, ctx, group, dtype, plan.rest, window, chunk)
+                    lib.check(lib.xr_attention_mfma(
+                        at, q.data_ptr(), k16.data_ptr(), v16.data_ptr(), plan.items.data_ptr(), plan.n_items, plan.n_cta_items, None, 0, None,
+                        _ptr(plan.jobs), plan.n_jobs, ctx.cu_q.data_ptr(), ctx.starts_dev.data_ptr(), table.data_ptr(), table.stride(0), part_o, part_ml,
+                        H, Hk, D, Dv, page_size, float(scale), window, chunk, _ptr(slopes), _ptr(sinks), float(softcap), *gating))
+                return out
+        if knows:
+            k16, v16, table = self.read_pages(k_pages, v_pages, ctx, group, dtype, None, window, chunk, keep_first)
+            return self.attention(q, k16, v16, _PagesOf(ctx, table), group, H, Hk, D, page_size, scale, window or None, slopes, chunk or None, keep_first, sinks, Dv,
+                                     softcap, gate, out_scale, out)
+        self.lib.check(self.lib.xr_attention_any4(
+            at, q.data_ptr(), *pages, positions.data_ptr(), req_of_token.data_ptr(), block_table.data_ptr(), block_table.stride(0), T, H, Hk, D, Dv,
+            page_size, float(scale), window, chunk, int(keep_first), dtype_code(dtype), _ptr(slopes), _ptr(sinks), float(softcap), *gating))
+        return out
 
     def attention_on_matrix_cores(self, dtype: torch.dtype, D: int, Dv: int, page_size: int = 64) -> bool:
         """Whether keys of ``D`` and values of ``Dv`` channels have matrix-core attention kernels."""
