@@ -400,8 +400,9 @@ extern "C" int xr_read_pages4(void* k_out, void* v_out, void* kc, void* ks, void
 }
 
 // ---------------------------------------------------------------- attention, any head size
-// k_attention_ref over 4-bit pages: a workgroup a token and query head, its waves 64 keys a turn each, a key a lane for the scores and channels a
-// lane for the values; the same options.  For what the matrix-core kernel does not take and a recorded step cannot read back first.
+// Attention over 4-bit pages in 32 bits: a workgroup a token and query head, its waves 64 keys a turn each; a key a lane for the scores, a pair of channels a
+// lane for the values, 8 positions at a time as they lie side by side; the options of k_attention_ref.  For what the matrix-core kernel does not take: 32-bit
+// queries, and in recorded steps, whose pages cannot be read back first, other head sizes and kept first keys.
 #define ANY4_WAVES 8
 struct Any4Args {
     Pages4 pages;
@@ -417,10 +418,12 @@ struct Any4Args {
     float scale, cap, out_scale;
 };
 
-template <typename T>
+// WIDE: keys in whole blocks, a block's codes in one load
+template <typename T, bool WIDE>
 __global__ __launch_bounds__(64 * ANY4_WAVES) void k_attention_any4(Any4Args a) {
-    __shared__ float qs[256], sums[ANY4_WAVES][256], ml[ANY4_WAVES][2];
-    const int t = blockIdx.x, h = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    __shared__ __align__(16) float qs[256];
+    __shared__ float sums[ANY4_WAVES][256], ml[ANY4_WAVES][2];
+    const int t = blockIdx.x, h = blockIdx.y, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int pos = a.positions[t], kvh = h / (a.H / a.Hk);
     const int lo = a.chunk > 0 ? pos - pos % a.chunk : (a.window > 0 && pos - a.window + 1 > 0) ? pos - a.window + 1 : 0;
     const int kept = a.keep < lo ? a.keep : lo;
@@ -428,56 +431,99 @@ __global__ __launch_bounds__(64 * ANY4_WAVES) void k_attention_any4(Any4Args a) 
     __syncthreads();
     const int* bt = a.block_table + (size_t)a.req_of_token[t] * a.table_stride;
     const float slope = a.slopes ? a.slopes[h] : 0.f;
-    auto page_at = [&](int key) {           // (a place past the table, or a page that was given back: none)
-        const int bi = key >> a.page_shift;
-        const int p = bi < a.table_stride ? bt[bi] : -1;
-        return (unsigned)p < (unsigned)a.n_pages ? p : -1;
-    };
-    float m = -INFINITY, l = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int seg = kept > 0 ? 0 : 1; seg < 2; ++seg)
-        for (int k0 = (seg ? lo : 0) + 64 * wave, last = seg ? pos : kept - 1; k0 <= last; k0 += 64 * ANY4_WAVES) {
-            const int key = k0 + lane;
-            const int page = key <= last ? page_at(key) : -1;
+    const int P = a.page_size, nbk = blocks4(a.D), nbv = blocks4(a.Dv), pairs = a.Dv >> 1;
+    const bool both = pairs <= 32;                  // few pairs: the halves of a wave take turns with the eights of positions
+    const int pair = both ? lane & 31 : lane;
+    float m = -INFINITY, l = 0.f;
+    float2 acc[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+    for (int seg = kept > 0 ? 0 : 1; seg < 2; ++seg) {
+        const int begin = seg ? lo : 0, last = seg ? pos : kept - 1;
+        for (int k0 = (begin & ~7) + 64 * wave; k0 <= last; k0 += 64 * ANY4_WAVES) {
+            const int key = k0 + lane, bi = key >> a.page_shift;
+            int page = key <= last && bi < a.table_stride ? bt[bi] : -1;       // (a place past the table, or a page that was given back: none)
+            page = (unsigned)page < (unsigned)a.n_pages ? page : -1;
+            const bool seen = page >= 0 && key >= begin;
             float s = -INFINITY;
-            if (page >= 0) {
-                float dot = 0.f, x[8];
-                for (int c0 = 0; c0 < a.D; c0 += 8) {
-                    key_row8(a.pages, (size_t)page * a.Hk + kvh, a.page_size, a.D, key & (a.page_size - 1), c0, x);
+            if (seen) {
+                const size_t pb = (size_t)page * a.Hk + kvh;
+                const int off = key & (P - 1);
+                const uint8_t* codes = a.pages.kc + key_at4(pb, P, a.D, off);
+                const uint8_t* scales = a.pages.ks + scale_at4(pb, P, nbk, off, 0);
+                float dot = 0.f;
+                for (int b = 0; b < nbk; ++b) {
+                    const uint32_t sc = (uint32_t)scales[8 * b] << 23;
+                    uint32_t w[4];
+                    const int n = WIDE ? 4 : min(4, (a.D - 32 * b) >> 3);
+                    if constexpr (WIDE) {
+                        const uint4 v = *reinterpret_cast<const uint4*>(codes + 16 * b);
+                        w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+                    } else {
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) dot = fmaf(qs[c0 + i], x[i], dot);
+                        for (int i = 0; i < 4; ++i) w[i] = i < n ? *reinterpret_cast<const uint32_t*>(codes + 16 * b + 4 * i) : 0u;
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        if (!WIDE && i >= n) break;
+                        const float4 qa = *reinterpret_cast<const float4*>(qs + 32 * b + 8 * i), qb = *reinterpret_cast<const float4*>(qs + 32 * b + 8 * i + 4);
+                        const float2 v0 = pair4_f32<0>(w[i], sc), v1 = pair4_f32<1>(w[i], sc), v2 = pair4_f32<2>(w[i], sc), v3 = pair4_f32<3>(w[i], sc);
+                        dot = fmaf(qa.x, v0.x, dot); dot = fmaf(qa.y, v0.y, dot); dot = fmaf(qa.z, v1.x, dot); dot = fmaf(qa.w, v1.y, dot);
+                        dot = fmaf(qb.x, v2.x, dot); dot = fmaf(qb.y, v2.y, dot); dot = fmaf(qb.z, v3.x, dot); dot = fmaf(qb.w, v3.y, dot);
+                    }
                 }
                 s = dot * a.scale;
                 if (a.cap > 0.f) s = a.cap * tanhf(s / a.cap);
                 s -= slope * (float)(pos - key);
             }
             const float mn = fmaxf(m, wave_max(s));
-            const float p = page >= 0 ? expf(s - mn) : 0.f;
+            const float p = seen ? expf(s - mn) : 0.f;
             const float corr = m == -INFINITY ? 0.f : expf(m - mn);
             l = l * corr + wave_sum(p);
+            m = mn;
 #pragma unroll
-            for (int dd = 0; dd < 4; ++dd) acc[dd] *= corr;
-            const int nk = min(64, last - k0 + 1);
-            for (int j = 0; j < nk; ++j) {
-                const float pj = __shfl(p, j, 64);
-                const int pg = __shfl(page, j, 64);
-                if (pg < 0) continue;
+            for (int i = 0; i < 2; ++i) { acc[i].x *= corr; acc[i].y *= corr; }
+            const unsigned long long mask = __ballot(seen);
+            if (!mask) continue;
+            for (int o = 0; o < 8; o += both ? 2 : 1) {
+                const int mine = both ? o + (lane >> 5) : o;
+                const uint32_t some = (uint32_t)(mask >> (8 * mine)) & 255u;
+                const int pg = __shfl(page, 8 * mine + (some ? __ffs((int)some) - 1 : 0), 64);
+                float pj[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) pj[e] = __shfl(p, 8 * mine + e, 64);
+                if (!some) continue;
                 const size_t pb = (size_t)pg * a.Hk + kvh;
-                const int off = (k0 + j) & (a.page_size - 1);
+                const int off = (k0 + 8 * mine) & (P - 1);
 #pragma unroll
-                for (int dd = 0; dd < 4; ++dd) {
-                    const int d = lane + 64 * dd;
-                    if (d < a.Dv) {
-                        const uint32_t sc = (uint32_t)a.pages.vs[scale_at4(pb, a.page_size, blocks4(a.Dv), off, d >> 5)] << 23;
-                        const float2 v = pair4_f32<0>((uint32_t)a.pages.vc[value_at4(pb, a.page_size, a.Dv, off, d >> 1)], sc);
-                        acc[dd] = fmaf(pj, d & 1 ? v.y : v.x, acc[dd]);
+                for (int i = 0; i < 2; ++i) {
+                    const int pr = pair + 64 * i;
+                    if (pr >= pairs || (i > 0 && both)) break;
+                    const uint2 c = *reinterpret_cast<const uint2*>(a.pages.vc + value_at4(pb, P, a.Dv, off, pr));
+                    const uint2 sc = *reinterpret_cast<const uint2*>(a.pages.vs + scale_at4(pb, P, nbv, off, pr >> 4));
+                    // (a position that is not seen is no number's: its scale becomes the smallest, its weight is 0)
+                    const float2 v[8] = {pair4_f32<0>(c.x, some & 1 ? sc.x << 23 : 0u), pair4_f32<1>(c.x, some & 2 ? sc.x << 15 : 0u),
+                                         pair4_f32<2>(c.x, some & 4 ? sc.x << 7 : 0u), pair4_f32<3>(c.x, some & 8 ? sc.x >> 1 : 0u),
+                                         pair4_f32<0>(c.y, some & 16 ? sc.y << 23 : 0u), pair4_f32<1>(c.y, some & 32 ? sc.y << 15 : 0u),
+                                         pair4_f32<2>(c.y, some & 64 ? sc.y << 7 : 0u), pair4_f32<3>(c.y, some & 128 ? sc.y >> 1 : 0u)};
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        acc[i].x = fmaf(pj[e], v[e].x, acc[i].x);
+                        acc[i].y = fmaf(pj[e], v[e].y, acc[i].y);
                     }
                 }
             }
-            m = mn;
         }
+    }
+    if (both) {
+        acc[0].x += __shfl_xor(acc[0].x, 32, 64);
+        acc[0].y += __shfl_xor(acc[0].y, 32, 64);
+    }
     // the waves' shares in one scale (a wave without keys has the sum 0)
 #pragma unroll
-    for (int dd = 0; dd < 4; ++dd) sums[wave][lane + 64 * dd] = acc[dd];
+    for (int i = 0; i < 2; ++i)
+        if (pair + 64 * i < pairs && !(both && (i > 0 || lane > 31))) {
+            sums[wave][2 * (pair + 64 * i)] = acc[i].x;
+            sums[wave][2 * (pair + 64 * i) + 1] = acc[i].y;
+        }
     if (lane == 0) {
         ml[wave][0] = m;
         ml[wave][1] = l;
@@ -516,8 +562,12 @@ extern "C" int xr_attention_any4(void* out, const void* q, void* kc, void* ks, v
     a.slopes = slopes; a.sinks = sinks; a.gate = gate; a.table_stride = table_stride; a.n_pages = n_pages; a.H = H; a.Hk = Hk;
     a.D = D; a.Dv = Dv; a.page_shift = ilog2_exact(page_size); a.page_size = page_size; a.window = window; a.chunk = chunk; a.keep = keep;
     a.ld_gate = ld_gate; a.ld_out = ld_out; a.scale = scale; a.cap = cap; a.out_scale = out_scale;
-    if (dtype == XR_F32) k_attention_any4<float><<<dim3(T, H), 64 * ANY4_WAVES, 0, stream>>>(a);
-    else k_attention_any4<bf16_t><<<dim3(T, H), 64 * ANY4_WAVES, 0, stream>>>(a);
+    const dim3 grid(T, H);
+    if (dtype == XR_F32) {
+        if (D % 32 == 0) k_attention_any4<float, true><<<grid, 64 * ANY4_WAVES, 0, stream>>>(a);
+        else k_attention_any4<float, false><<<grid, 64 * ANY4_WAVES, 0, stream>>>(a);
+    } else if (D % 32 == 0) k_attention_any4<bf16_t, true><<<grid, 64 * ANY4_WAVES, 0, stream>>>(a);
+    else k_attention_any4<bf16_t, false><<<grid, 64 * ANY4_WAVES, 0, stream>>>(a);
     XR_CHECK_LAUNCH("attention_any4");
     return XR_OK;
 }
