@@ -346,6 +346,16 @@ def test_attention_with(ops, what, shape, recorded, dt):
     attend(ops, (H, Hk, D, D, page, mask, [0, 37, 129, 300, 1500, 64], [1, 2, 1, 40, 1, 1]), dt, 100 + len(what), recorded, **opt)
 
 
+@pytest.mark.parametrize("what", ["", *OPTIONS])
+@pytest.mark.parametrize("shape", [(6, 2, 72, 40, 16), (3, 1, 200, 136, 8), (4, 2, 256, 256, 64), (4, 4, 24, 64, 32)])
+@pytest.mark.parametrize("mask", [None, 13, Chunked(20)])
+@pytest.mark.parametrize("dt", ["bfloat16", "float32"])
+def test_other_head_sizes(ops, what, shape, mask, dt):
+    """Heads that end inside a block, more than 64 pairs of channels, masks that begin inside 8 positions."""
+    H, Hk, D, Dv, page = shape
+    attend(ops, (H, Hk, D, Dv, page, mask, [0, 6, 129, 61, 530], [1, 2, 9, 1, 1]), dt, 200 + D + len(what), **OPTIONS.get(what, {}))
+
+
 MANY = [
     # H, Hk, D, Dv, page, mask, starts, q_lens: more than 16 rows a key/value head
     (8, 2, 128, 128, 64, None, [0, 61, 700], [5, 33, 17]),

@@ -1074,8 +1074,10 @@ class Ops:
         bfloat16 runs on the matrix cores (head and value sizes in steps of 16 up to 256, pages of at least
         16 positions, a cap or slopes; kept first keys only where values have the keys' size); float32, and what the MFMA kernel does not take, runs the 32-bit kernel.
         Caches that are ``FourBitPages``: requests of up to some hundred rows a key/value head are read from the codes by a matrix-core kernel of
-        their own (bfloat16, sizes in whole blocks of 32, pages of at least 32 positions, no kept first keys); the pages of others are read
-        back first (``read_pages``), but in steps that are being recorded, which a 32-bit kernel then serves from the codes.
+        their own (bfloat16, sizes in whole blocks of 32, pages of at least 32 positions, no kept first keys).  The pages of others are read
+        back first (``read_pages``) where matrix cores then have enough rows; what is left, and what a step that is being recorded cannot read back,
+        a 32-bit kernel serves from the codes.  Calls that share a step's context follow one another (they share its counters): on one stream, or
+        behind an event.
         """
         if isinstance(k_cache, FourBitPages) or isinstance(v_cache, FourBitPages):
             return self._attention4(q, k_cache, v_cache, ctx, group, H, Hk, D, page_size, scale, window, slopes, chunk, keep_first, sinks,
@@ -1203,7 +1205,12 @@ class Ops:
                         _ptr(plan.jobs), plan.n_jobs, ctx.cu_q.data_ptr(), ctx.starts_dev.data_ptr(), table.data_ptr(), table.stride(0), part_o, part_ml,
                         H, Hk, D, Dv, page_size, float(scale), window, chunk, _ptr(slopes), _ptr(sinks), float(softcap), *gating))
                 return out
-        if knows:
+        # Pages are read back for what then runs on matrix cores: 16-bit queries, and 32-bit ones of more than 16 rows a request (8 requests of 4,000 keys, 32 heads
+        # over 8, codes and pages: 1 row 59 us and 441, 8 rows 282 and 540, 16 rows 517 and 540, 64 rows 1,904 and 1,002).  What is left for the kernel that takes a
+        # row and head at a time reads the codes itself (8 requests of 2,000 keys, heads of 72: 1 row 29 us and 769, 64 rows 834 and 15,227).
+        cores = (self.attention_on_matrix_cores(dtype, D, Dv, page_size) and not (softcap and slopes is not None) and (D == Dv or not keep_first)
+                 and ld_out % 4 == 0 and at % 8 == 0)
+        if knows and (cores or (dtype is torch.float32 and max(D, Dv) <= 128 and max(ctx.q_lens) > 16)):
             k16, v16, table = self.read_pages(k_pages, v_pages, ctx, group, dtype, None, window, chunk, keep_first)
             return self.attention(q, k16, v16, _PagesOf(ctx, table), group, H, Hk, D, page_size, scale, window or None, slopes, chunk or None, keep_first, sinks, Dv,
                                      softcap, gate, out_scale, out)
