@@ -147,6 +147,72 @@ def test_write(ops, case, dt):
                         assert np.array_equal(c0[p, :, off], c1[p, :, off])
 
 
+PROJECTIONS = [
+    # H, Hk, D, K, rot, interleaved, page, packed, bias, starts, q_lens
+    (8, 2, 64, 512, 64, False, 64, True, False, [0] * 10 + [63, 1000, 64, 7, 8, 9, 130], [1] * 17),        # decoded tokens
+    (4, 4, 128, 1024, 128, False, 32, False, True, [5, 131000], [40, 24]),
+    (6, 2, 96, 256, 64, False, 64, False, True, [0, 250], [90, 10]),
+    (4, 1, 64, 2048, 64, True, 128, True, True, [3], [137]),
+    (2, 2, 48, 320, 48, False, 16, False, False, [16, 3, 0], [200, 100, 1]),
+    (9, 3, 80, 576, 16, False, 8, False, True, [0], [320]),
+    (3, 3, 32, 256, 0, False, 64, False, False, [100], [33]),
+]
+
+
+@pytest.mark.parametrize("case", PROJECTIONS)
+def test_projection(ops, case):
+    """The kernel that adds a product's ranges up against the product and ``rope_kv_write`` one after the other."""
+    from xyntetik_runner_amd.csrc.ops import FourBitPages
+    H, Hk, D, K, rot, interleaved, page, packed, biased, starts, q_lens = case
+    rng = np.random.default_rng(D + K)
+    T, N = sum(q_lens), (H + 2 * Hk) * D
+    tables, n_pages = scattered(rng, [s + n for s, n in zip(starts, q_lens)], page)
+    tables[-1][-1] = -1                          # a page that was given back: its rows' queries come back all the same
+    ctx = step(starts, q_lens, tables)
+    inv = torch.tensor(1e4 ** -(np.arange(rot // 2) / max(1, rot // 2)), dtype=torch.float32, device=DEV)
+    h = torch.tensor(rng.normal(size=(T, K)), device=DEV).bfloat16()
+    w = torch.tensor(rng.normal(size=(N, K)) * K ** -0.5, device=DEV).bfloat16()
+    bias = torch.tensor(rng.normal(size=N), dtype=torch.float32, device=DEV) if biased else None
+    both = []
+    for fuse in (True, False):
+        kp, vp = (FourBitPages.zeros(n_pages, Hk, page, D, values, DEV) for values in (False, True))
+        before, ops.fuse_rope = ops.fuse_rope, fuse
+        try:
+            q = ops.project_rope_kv_write(h, ops.pack_weight(w) if packed else w, bias, kp, vp, ctx.positions, ctx.req_of_token, ctx.block_table(0),
+                                          inv, H, Hk, D, rot, interleaved, 1.25, page, paired=rot > 0 and not interleaved)
+        finally:
+            ops.fuse_rope = before
+        both.append((q.cpu().double().numpy(), host(kp), host(vp)))
+    (q0, k0, v0), (q1, k1, v1) = both
+    # Both add the same products up in 32 bits, in ranges that may differ: numbers of about 1 are off by 2^-20, sums of K = 2,048 products included.  A rounding
+    # that this turns over moves a query by a step, a code by one, of at most two units; fewer than one in a thousand lies that near to a tie (2^-20 of 2^-9 a step: one in 2,000).
+    assert (np.abs(q0 - q1) <= 2.0 ** -7 * np.abs(q1) + 2.0 ** -18).all() and np.mean(q0 != q1) < 1e-3
+    for (c0, s0), (c1, s1), values in ((k0, k1, False), (v0, v1, True)):
+        assert c1.any() and np.mean(c0 != c1) < 1e-3 and np.mean(s0 != s1) < 1e-3
+        for b, n in enumerate(q_lens):
+            at = [p for p in range(starts[b], starts[b] + n) if tables[b][p // page] >= 0]
+            if not at:
+                continue
+            x0, x1 = (F.pages_rows(c, s, tables[b], at, page, values) for c, s in ((c0, s0), (c1, s1)))
+            blocks = [np.abs(x1[..., i:i + 32]).max(-1, keepdims=True) for i in range(0, D, 32)]
+            largest = np.concatenate([np.repeat(m, min(32, D - 32 * i), -1) for i, m in enumerate(blocks)], -1)
+            assert (np.abs(x0 - x1) <= largest).all()
+
+
+def test_a_projection_that_pages_do_not_fit(ops):
+    from xyntetik_runner_amd.csrc.ops import FourBitPages, KernelError
+    ctx = step([0], [20], [[1]])
+    h, w = torch.zeros((20, 64), dtype=torch.bfloat16, device=DEV), torch.zeros((4 * 32, 64), dtype=torch.bfloat16, device=DEV)
+    kp, vp, wide = FourBitPages.zeros(3, 1, 32, 32, False, DEV), FourBitPages.zeros(3, 1, 32, 32, True, DEV), FourBitPages.zeros(3, 1, 32, 64, True, DEV)
+    inv = torch.ones(16, device=DEV)
+    call = lambda *a, **k: ops.project_rope_kv_write(h, w, None, *a, ctx.block_table(0), inv, 2, 1, 32, 32, True, 1.0, k.get("page", 32))
+    call(kp, vp, ctx.positions, ctx.req_of_token)
+    for a, k in (((kp, wide, ctx.positions, ctx.req_of_token), {}), ((kp, vp, ctx.positions, ctx.req_of_token), {"page": 64}),
+                 ((kp, vp, ctx.positions.long(), ctx.req_of_token), {}), ((kp, vp, ctx.positions, ctx.req_of_token[:4]), {})):
+        with pytest.raises(KernelError):
+            call(*a, **k)
+
+
 def test_rows_in_any_order_and_without_a_page(ops):
     """Rows of a request that are not one after the other, with first and last as if they were; positions past the table, requests past its rows,
     pages given back or past the pool: written nowhere, read as zeros."""

@@ -1505,6 +1505,13 @@ __global__ __launch_bounds__(64 * FEW_WAVES, FEW_PER_CU) void k_attn_few(AttnArg
 // neighbouring channels; a pair of channels is converted position by position and two positions' words change halves (32 conversions and 32 exchanges of
 // halves for 32 keys x 128 channels).  Row m of output block d so stands for channel m * HV / 16 + d.
 // Scales past a request's end are taken as zeros' and codes there are any numbers: no operand has to be masked.
+//
+// What bounds it: with one row block a request and head memory, 64 requests of 4,000 to 8,000 keys (8 heads of 128, 4 query heads each) take 65.6 us for 424 MB, 6.5
+// TB/s of the 7.05 that a kernel here reaches that only reads (pages read back first: 715); the 64 conversions and 32 exchanges of a tile, 4.65 cycles each, take
+// half of that time beside it.  Blocks of many rows are bound by instructions, 197 a tile of 32 keys (512 rows of 4 heads over 4,000 keys 64 us).  A lone request of 131,072
+// keys takes 31 us (143 MB, 4.5 TB/s): eight tiles a wave, then the sum over 64 ranges.
+// Three workgroups a compute unit with a tile on its way while one is multiplied, streaming loads (23 requests of 900 keys, 32 heads: 16 us; two workgroups and two
+// tiles 18; four do not fit the registers of heads of 128; ordinary loads 64 of 8,000 66 us -> 76).  32 rows a block would halve the conversions a row, but leaves two workgroups a unit (8 x 9 tokens of 4 heads over 3,000 keys 17 us -> 28).
 constexpr bool FOUR_OK = HD % 32 == 0 && HV % 32 == 0;
 constexpr int NB4K = HD / 32, NB4V = FOUR_OK ? HV / 32 : 1;              // blocks of a key and of a value
 constexpr int KS4 = FKD % 4 == 0 ? FKD / 4 : 4 % FKD == 0 ? 1 : FKD;      // scales of a lane's share of a key: of whole blocks, of a part of one, or word by word
@@ -1670,7 +1677,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES, FOUR_PER_CU) void k_attn_few4(AttnA
         }
         const bool whole = kt + 32 <= kend && kt + 31 <= pos_min && kt >= lo_max;
         if (!whole) {
-            asm volatile("; hidden keys");      // (a branch: as a selection its 40 instructions were every tile's)
+            asm volatile("; hidden keys");      // (stays a branch: whole tiles, nearly all, skip the selection's 40 instructions)
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 const int key = kt + 8 * quad + e;

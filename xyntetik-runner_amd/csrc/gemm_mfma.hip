@@ -31,6 +31,7 @@
 
 #include "common.h"
 #include "async_copy.h"
+#include "pages4.h"
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -101,6 +102,7 @@ struct GemmArgs {
     int post_ld;
     float post_alpha;
     RopeFuse rope;     // rotation and cache write in place of the output (on: rope.q_out not null)
+    const Write4Sums* four;     // the same with 4-bit pages: its kernel takes the raw sums (the host's memory; for the launcher alone)
 };
 
 // what a caller passes to have the product's row rotated and cached (see RopeFuse)
@@ -117,6 +119,7 @@ struct XrGemmRope {
     void* k_cache;
     void* v_cache;
     const void* cs_table;   // [M][rot/2] (cosine, sine) pairs made by xr_rope_table for these rows, or null: the product makes its own
+    const XrGemmPages4* four;   // 4-bit pages in place of the caches (17 to XR_ROPE_TILE_ROWS - 1 rows), or null
 };
 
 // what a caller passes to fold a norm into a product of at most 16 rows (see GemmArgs)
@@ -1361,6 +1364,12 @@ static int launch_tile_async(GemmArgs g, hipStream_t stream) {
     else
         k_gemm_tile_async<BM, BN, WM_, WN_, ST, PIPE, BK><<<groups, 64 * WM_ * WN_, smem, stream>>>(g);
     XR_CHECK_LAUNCH("gemm_tile_async");
+    if (g.four) {
+        Write4Sums w = *g.four;
+        w.sums = g.partial;
+        w.ranges = g.splits;
+        return rope_kv_write4_sums(w, stream);
+    }
     if (g.norm_whole) {
         if (g.N <= 4096) k_gemm_finish_norm<1><<<(unsigned)g.M, 1024, 0, stream>>>(g);
         else if (g.N <= 8192) k_gemm_finish_norm<2><<<(unsigned)g.M, 1024, 0, stream>>>(g);
@@ -1873,6 +1882,8 @@ extern "C" int xr_gemm_bf16(void* out, const void* a, const void* w, const float
         }
     }
     g.rope.q_out = nullptr; g.rope.cs = g.rope.table = nullptr;
+    g.four = nullptr;
+    Write4Sums four;
     // many rows: the tile kernel rotates and caches its own result, with the rows' cosines and
     // sines from a table that a small kernel writes into the workspace first; K is then not split
     // from XR_ROPE_TILE_ROWS rows on; below, the kernel that adds up the K ranges rotates and caches
@@ -1897,8 +1908,14 @@ extern "C" int xr_gemm_bf16(void* out, const void* a, const void* w, const float
         XR_REQUIRE(rope->rot == 0 || rope->inv_freq, "gemm: rotary width %d without a frequency table", rope->rot);
         const int shift = ilog2_exact(rope->page_size);
         XR_REQUIRE(rope->Hk == 0 || shift >= 0, "gemm: page size %d is not a power of two", rope->page_size);
-        XR_REQUIRE(rope->positions && rope->q_out && (rope->Hk == 0 || (rope->k_cache && rope->v_cache && rope->block_table && rope->req_of_token)),
+        XR_REQUIRE(rope->positions && rope->q_out && (rope->Hk == 0 || ((rope->four || (rope->k_cache && rope->v_cache)) && rope->block_table && rope->req_of_token)),
                    "gemm: rotation and cache write with a null operand");
+        if (rope->four) {
+            XR_REQUIRE(!rope_direct && M > 16 && rope->Hk > 0, "gemm: a product of %d rows does not write to 4-bit pages by itself (17 to %d do)", M, XR_ROPE_TILE_ROWS - 1);
+            four = Write4Sums{nullptr, bias, 0, rope->four, rope->positions, rope->req_of_token, rope->block_table, rope->table_stride, rope->inv_freq,
+                              rope->q_out, M, rope->H, rope->Hk, rope->D, rope->rot, rope->interleaved, rope->mscale, rope->page_size};
+            g.four = &four;
+        }
         g.rope.positions = rope->positions; g.rope.req_of_token = rope->req_of_token; g.rope.block_table = rope->block_table;
         g.rope.table_stride = rope->table_stride; g.rope.inv_freq = rope->inv_freq;
         g.rope.H = rope->H; g.rope.Hk = rope->Hk; g.rope.D = rope->D; g.rope.rot = rope->rot; g.rope.interleaved = rope->interleaved;

@@ -330,7 +330,12 @@ class _GemmRope(C.Structure):
     """XrGemmRope of the library."""
     _fields_ = [("positions", _p), ("req_of_token", _p), ("block_table", _p), ("table_stride", _i),
                 ("inv_freq", _p), ("H", _i), ("Hk", _i), ("D", _i), ("rot", _i), ("interleaved", _i),
-                ("mscale", _f), ("page_size", _i), ("q_out", _p), ("k_cache", _p), ("v_cache", _p), ("cs_table", _p)]
+                ("mscale", _f), ("page_size", _i), ("q_out", _p), ("k_cache", _p), ("v_cache", _p), ("cs_table", _p), ("four", _p)]
+
+
+class _GemmPages4(C.Structure):
+    """XrGemmPages4 of the library."""
+    _fields_ = [("kc", _p), ("ks", _p), ("vc", _p), ("vs", _p), ("n_pages", _i), ("n_requests", _i)]
 
 
 def paired_order(D: int, rot: int) -> list:
@@ -504,6 +509,9 @@ class Ops:
     GEMM_WORKSPACE_BYTES = 96 << 20
     ROPE_TILE_ROWS = 512    # from here the q/k/v product has tiles enough with K whole, and its tile kernel rotates and caches
     FINISH_ROWS = 511       # up to here the kernel that adds a product's K ranges up rotates and caches (the library's own number)
+    # With 4-bit pages up to here: a product whose ranges stay to be added up is one launch of one tile, which costs more rows more than the other kernel saves
+    # (32 + 2 * 8 heads of 128, 8 of 64, 32 of 128, one kernel and two, us: 256 rows 32.8, 37.7; 19.8, 23.5; 49.1, 51.8; 300 37.7, 39.4; 22.7, 25.0; 58.1, 56.4; 450 44.7, 43.4; 26.4, 25.0; 72.6, 68.1).
+    FOUR_FINISH_ROWS = 320
 
     def _gemm_workspace(self, device):
         """Room for the sums of K ranges when a product with few rows is split (one buffer per process;
@@ -1008,7 +1016,8 @@ class Ops:
         Up to 16 bfloat16 rows (``h`` may be an ``UnscaledRows``) the product's kernel rotates and
         stores its own result, up to 511 the kernel that adds the product's K ranges up does, from
         512 the tile kernel (with the rows' cosines and sines from a table made first), which
-        saves a kernel; in float32, and where the kernels' conditions on sizes do not hold, the
+        saves a kernel; in float32, where the kernels' conditions on sizes do not hold, and with
+        4-bit pages but for 17 to 320 rows, whose ranges its kernel adds up, the
         product and ``rope_kv_write`` run one after the other.  ``cs_table``: a callable that returns the
         step's ``rope_table`` (asked for only where the tile kernel rotates); ``finish_table``: the same for 17 to 511 rows,
         where the kernel that adds the ranges up makes its own without one.  (Eight layers and their table, us more or less than without: 17 rows
@@ -1020,12 +1029,24 @@ class Ops:
         if w.shape[0] != Q + 2 * KV:
             raise KernelError(f"projection has {w.shape[0]} rows, {H} query and 2 x {Hk} key/value heads of {D} need {Q + 2 * KV}")
         q = torch.empty((T, Q), dtype=rows.dtype, device=rows.device)
+        four = isinstance(k_cache, FourBitPages)
         if (self.fuse_rope and (T <= self.FINISH_ROWS or T >= self.ROPE_TILE_ROWS) and self._mfma_ok(rows, wt) and D % 16 == 0
                 and (T * w.shape[0] * 4 if T <= self.FINISH_ROWS else T * (rot // 2 + 1) * 8) <= self.GEMM_WORKSPACE_BYTES
-                and (Hk == 0 or (k_cache.dtype == torch.bfloat16 and v_cache.dtype == torch.bfloat16))
+                and (Hk == 0 or (k_cache.dtype == torch.bfloat16 and v_cache.dtype == torch.bfloat16) or
+                     (four and UnscaledRows.MAX_ROWS < T <= self.FOUR_FINISH_ROWS and (rot % 8 == 0 if interleaved else rot % 16 == 0) and (bias is None or bias.data_ptr() % 16 == 0)))
                 and (T < self.ROPE_TILE_ROWS or Hk == 0 or k_cache.data_ptr() % 16 == 0)       # (tiles store 8 channels at a time)
                 and (rot == 0 or interleaved or (paired and rot % 16 == 0))):
-            self._dev(rows, wt, bias, k_cache, v_cache, positions, req_of_token, block_table, inv_freq)
+            pages = None
+            if four:
+                self._here("projection", rows, wt, bias, k_cache, v_cache, positions, req_of_token, block_table, inv_freq)
+                pages = _GemmPages4(*self._pages4("projection", k_cache, v_cache, Hk, D, page_size), 0)
+                if v_cache.dim != D or (rot and (inv_freq is None or inv_freq.dtype != torch.float32 or inv_freq.numel() != rot // 2 or not inv_freq.is_contiguous())):
+                    raise KernelError(f"projection: values of {D} channels and {rot // 2} 32-bit frequencies are needed")
+                self._ints("projection", T, positions, req_of_token)
+                self._table("projection", block_table)
+                pages.n_requests = block_table.shape[0]
+            else:
+                self._dev(rows, wt, bias, k_cache, v_cache, positions, req_of_token, block_table, inv_freq)
             self._contig(wt, "projection weight")
             if rows.shape[1] != w.shape[1] or rows.stride(1) != 1:
                 raise KernelError(f"projection: shapes {tuple(rows.shape)} x {tuple(w.shape)}^T do not fit")
@@ -1037,8 +1058,9 @@ class Ops:
             rp.table_stride = block_table.stride(0) if block_table is not None else 0
             rp.inv_freq, rp.H, rp.Hk, rp.D, rp.rot = _ptr(inv_freq), H, Hk, D, rot
             rp.interleaved, rp.mscale, rp.page_size = 1 if interleaved else 0, float(mscale), page_size
-            rp.q_out, rp.k_cache, rp.v_cache = q.data_ptr(), _ptr(k_cache) if Hk else None, _ptr(v_cache) if Hk else None
-            ask = cs_table if T >= self.ROPE_TILE_ROWS else finish_table if T > UnscaledRows.MAX_ROWS else None
+            rp.q_out, rp.k_cache, rp.v_cache = q.data_ptr(), _ptr(k_cache) if Hk and not four else None, _ptr(v_cache) if Hk and not four else None
+            rp.four = C.addressof(pages) if four else None
+            ask = None if four else cs_table if T >= self.ROPE_TILE_ROWS else finish_table if T > UnscaledRows.MAX_ROWS else None
             table = ask() if (ask is not None and rot > 0) else None
             rp.cs_table = _ptr(table)
             self.lib.check(self.lib.xr_gemm_bf16(None, rows.data_ptr(), wt.data_ptr(), _ptr(bias), T, w.shape[0],

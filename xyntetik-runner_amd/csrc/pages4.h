@@ -30,6 +30,30 @@ struct Pages4 {
     uint8_t* vs;
 };
 
+// what a product's caller passes beside its rotation to have keys and values go to 4-bit pages
+struct XrGemmPages4 {
+    void *kc, *ks, *vc, *vs;
+    int n_pages, n_requests;
+};
+
+struct Write4Sums {
+    const float* sums;      // [ranges][T][(H + 2 Hk) * D], 32-bit
+    const float* bias;      // [(H + 2 Hk) * D] or null
+    int ranges;
+    const XrGemmPages4* pages;
+    const int* positions;
+    const int* req_of_token;
+    const int* block_table;
+    int table_stride;
+    const float* inv_freq;
+    void* q_out;            // [T, H * D] bfloat16
+    int T, H, Hk, D, rot, interleaved;     // (pairs that are not neighbours: in paired order)
+    float mscale;
+    int page_size;
+};
+// xr_rope_kv_write4 behind a product whose K ranges are still to be added up
+int rope_kv_write4_sums(const Write4Sums& w, hipStream_t stream);
+
 __host__ __device__ inline int blocks4(int channels) { return (channels + XR_BLOCK4 - 1) / XR_BLOCK4; }
 
 // byte of a page's scale: `pb` = page * heads + head

@@ -10,6 +10,10 @@
 // magnitude in two exchanges.  (A head's last block may be short: its missing lanes hold zeros.)  Where the rows are aligned it reads its channels and
 // their partners in the rotation as four pieces of 16 bytes, before the angles are made.  A page holds the bytes of 8 positions of a value side by side: where the
 // step brings such 8 positions whole, the workgroup of the first writes them all, 16 bytes at a time, and the other seven leave their values to it.
+//
+// Bound by memory: 2,048 tokens of 32 + 2 * 8 heads of 128 (50 MB of 32-bit rows in, 17 MB of queries and 2 MB of codes out) take 15.4 us, 4.5 TB/s where a
+// large copy reaches 5.06 (channel by channel, a byte at a time and tokens in the order of their numbers 30.9); one token takes 2.8, the latency of its two
+// dependent reads (position, page) and of the rows.
 struct Write4Args {
     const float* q_in;      // [T, in_stride] 32-bit
     const float* k_in;
@@ -28,6 +32,9 @@ struct Write4Args {
     int q_units, k_units, units, per_block;     // of a token: queries' end, keys' end, all; and those of a workgroup
     int lanes_k, lanes_v;                       // threads of a head of queries or keys, and of values (a multiple of 4, 32 at most)
     uint32_t per_k, per_v;                      // 2^32 over these, rounded up: a division below 2^26 is one product
+    const float* bias;                          // SUMS: [columns of a row] or null
+    size_t range_step;                          // SUMS: from a range's rows to the next's
+    int ranges;
 };
 
 // (8 numbers of a row that begin at a multiple of 16 bytes)
@@ -44,6 +51,24 @@ __device__ __forceinline__ void load_row8(const float* p, float* v) {
     const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
     v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
 }
+// 8 sums of a product's K ranges, four ranges on their way at a time
+__device__ __forceinline__ void load_sums8(const Write4Args& a, const float* p, const float* bias, float* v) {
+    float b[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = b[i] = 0.f;
+    if (bias) load_row8(bias, b);
+    for (int s0 = 0; s0 < a.ranges; s0 += 4) {
+        float part[4][8];
+#pragma unroll
+        for (int s = 0; s < 4; ++s) load_row8(p + (size_t)(s0 + s < a.ranges ? s0 + s : s0) * a.range_step, part[s]);
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] += s0 + s < a.ranges ? part[s][i] : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] += b[i];
+}
 // the largest magnitude of a block of 32, of which the lane holds 8
 __device__ __forceinline__ uint32_t most_of_block(const float* x) {
     uint32_t most = 0;
@@ -59,7 +84,9 @@ template <int B> __device__ __forceinline__ uint32_t bytes_of(uint32_t w0, uint3
 }
 
 // VEC: rows of 16-byte pieces, and a rotation whose pairs lie in such pieces
-template <typename T, bool VEC>
+// SUMS: a number is the sum of a product's K ranges, added in their order, and its column's bias: a kernel and a trip of the rows to memory less.  With the product,
+// 32 + 2 * 8 heads of 128 behind 4,096 columns: 64 decoded tokens 20.3 us, in two kernels 21.3; 256 32.8 and 37.7; a prompt's 137 tokens 28.7 and 30.6.
+template <typename T, bool VEC, bool SUMS>
 __global__ __launch_bounds__(256) void k_rope_kv_write4(Write4Args a) {
     __shared__ float2 cs[8][17];                // pair j at [j % 8][j / 8]: lanes that read the i-th of their 8 pairs read side by side
     // (workgroups go to the eight dies in turn: 8 neighbouring tokens, whose codes share lines, to one of them)
@@ -89,8 +116,14 @@ __global__ __launch_bounds__(256) void k_rope_kv_write4(Write4Args a) {
             }
 #pragma unroll
             for (int i = 0; i < 8; ++i) w.x[i] = w.y[i] = 0.f;
-            if (w.c0 < w.D) load_row8(w.src + own, w.x);
-            if (turn) load_row8(w.src + other, w.y);
+            if constexpr (SUMS) {
+                const float* bias = a.bias ? a.bias + (w.src - a.q_in - (size_t)t * a.in_stride) : nullptr;
+                if (w.c0 < w.D) load_sums8(a, w.src + own, bias ? bias + own : nullptr, w.x);
+                if (turn) load_sums8(a, w.src + other, bias ? bias + other : nullptr, w.y);
+            } else {
+                if (w.c0 < w.D) load_row8(w.src + own, w.x);
+                if (turn) load_row8(w.src + other, w.y);
+            }
         }
         return w;
     };
@@ -128,6 +161,26 @@ __global__ __launch_bounds__(256) void k_rope_kv_write4(Write4Args a) {
                 else
 #pragma unroll
                     for (int e = 0; e < 8; ++e) v[i][e] = src[(size_t)i * a.in_stride + e];
+            }
+            if constexpr (SUMS) {
+                for (int s = 1; s < a.ranges; ++s) {
+                    float more[8][8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) load_row8(src + (size_t)s * a.range_step + (size_t)i * a.in_stride, more[i]);
+                    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) v[i][e] += more[i][e];
+                }
+                if (a.bias) {
+                    float bias[8];
+                    load_row8(a.bias + (src - a.q_in - (size_t)t * a.in_stride), bias);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) v[i][e] += bias[e];
+                }
             }
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -217,6 +270,39 @@ static int check_pages4(const char* what, const Pages4& p, int Hk, int D, int Dv
     return XR_OK;
 }
 
+// the work of a token in workgroups: one where there are tokens enough for the chip, else a round of threads each
+static dim3 deal_units(Write4Args& a, int T) {
+    a.lanes_k = blocks4(a.D) * 4; a.lanes_v = blocks4(a.Dv) * 4;
+    a.per_k = (uint32_t)(((1ull << 32) + a.lanes_k - 1) / a.lanes_k); a.per_v = (uint32_t)(((1ull << 32) + a.lanes_v - 1) / a.lanes_v);
+    a.q_units = a.H * a.lanes_k; a.k_units = a.q_units + a.Hk * a.lanes_k; a.units = a.k_units + a.Hk * a.lanes_v;
+    int groups = (1024 + T - 1) / T;
+    const int most = (a.units + 255) / 256;
+    groups = groups < 1 ? 1 : groups > most ? most : groups;
+    a.per_block = ((a.units + groups - 1) / groups + 255) / 256 * 256;
+    return dim3(T, (a.units + a.per_block - 1) / a.per_block);
+}
+
+int rope_kv_write4_sums(const Write4Sums& w, hipStream_t stream) {
+    const XrGemmPages4& p = *w.pages;
+    Write4Args a;
+    a.pages = Pages4{(uint8_t*)p.kc, (uint8_t*)p.ks, (uint8_t*)p.vc, (uint8_t*)p.vs};
+    const int rc = check_pages4("gemm", a.pages, w.Hk, w.D, w.D, w.page_size, p.n_pages);
+    if (rc != XR_OK) return rc;
+    a.in_stride = (w.H + 2 * w.Hk) * w.D;
+    XR_REQUIRE(a.in_stride % 4 == 0 && (((uintptr_t)w.sums | (uintptr_t)w.bias | (uintptr_t)w.q_out) & 15) == 0 && (w.interleaved ? w.rot % 8 == 0 : w.rot % 16 == 0),
+               "gemm: rows that go to 4-bit pages must be 16-byte aligned, their rotary width (%d) a multiple of 16 (pairs of neighbours: 8)", w.rot);
+    a.q_in = w.sums; a.k_in = w.sums + (size_t)w.H * w.D; a.v_in = a.k_in + (size_t)w.Hk * w.D; a.q_out = w.q_out;
+    a.bias = w.bias; a.range_step = (size_t)w.T * a.in_stride; a.ranges = w.ranges;
+    a.positions = w.positions; a.req_of_token = w.req_of_token; a.block_table = w.block_table; a.table_stride = w.table_stride;
+    a.n_requests = p.n_requests; a.n_pages = p.n_pages; a.inv_freq = w.inv_freq; a.H = w.H; a.Hk = w.Hk; a.D = a.Dv = w.D; a.rot = w.rot;
+    a.interleaved = w.interleaved; a.paired = !w.interleaved && w.rot > 0; a.mscale = w.mscale;
+    a.page_shift = ilog2_exact(w.page_size); a.page_mask = w.page_size - 1; a.page_size = w.page_size;
+    const dim3 grid = deal_units(a, w.T);
+    k_rope_kv_write4<bf16_t, true, true><<<grid, 256, 0, stream>>>(a);
+    XR_CHECK_LAUNCH("rope_kv_write4_sums");
+    return XR_OK;
+}
+
 extern "C" int xr_rope_kv_write4(const float* q_in, const float* k_in, const float* v_in, int in_stride, void* q_out,
                                  void* kc, void* ks, void* vc, void* vs, int n_pages, const int* positions, const int* req_of_token,
                                  const int* block_table, int table_stride, int n_requests, const float* inv_freq, int T, int H, int Hk,
@@ -234,25 +320,17 @@ extern "C" int xr_rope_kv_write4(const float* q_in, const float* k_in, const flo
     if (T == 0) return XR_OK;
     XR_REQUIRE(k_in && v_in && block_table && req_of_token && positions, "rope_kv_write: keys and values to cache but a null operand");
     XR_REQUIRE(H == 0 || (q_in && q_out && ((uintptr_t)q_out & 15) == 0), "rope_kv_write: queries but a null operand, or rows that are not 16-byte aligned");
-    a.q_in = q_in; a.k_in = k_in; a.v_in = v_in; a.in_stride = in_stride; a.q_out = q_out;
+    a.q_in = q_in; a.k_in = k_in; a.v_in = v_in; a.in_stride = in_stride; a.q_out = q_out; a.bias = nullptr; a.range_step = 0; a.ranges = 1;
     a.positions = positions; a.req_of_token = req_of_token; a.block_table = block_table; a.table_stride = table_stride; a.n_requests = n_requests; a.n_pages = n_pages;
     a.inv_freq = inv_freq; a.H = H; a.Hk = Hk; a.D = D; a.Dv = Dv; a.rot = rot; a.interleaved = interleaved; a.paired = paired ? 1 : 0;
     a.mscale = mscale; a.page_shift = ilog2_exact(page_size); a.page_mask = page_size - 1; a.page_size = page_size;
-    a.lanes_k = blocks4(D) * 4; a.lanes_v = blocks4(Dv) * 4;
-    a.per_k = (uint32_t)(((1ull << 32) + a.lanes_k - 1) / a.lanes_k); a.per_v = (uint32_t)(((1ull << 32) + a.lanes_v - 1) / a.lanes_v);
-    a.q_units = H * a.lanes_k; a.k_units = a.q_units + Hk * a.lanes_k; a.units = a.k_units + Hk * a.lanes_v;
-    // a token a workgroup where there are tokens enough for the chip, else a round of threads each
-    int groups = (1024 + T - 1) / T;
-    const int most = (a.units + 255) / 256;
-    groups = groups < 1 ? 1 : groups > most ? most : groups;
-    a.per_block = ((a.units + groups - 1) / groups + 255) / 256 * 256;
-    const dim3 grid(T, (a.units + a.per_block - 1) / a.per_block);
+    const dim3 grid = deal_units(a, T);
     const bool vec = in_stride % 4 == 0 && (((uintptr_t)(H ? q_in : k_in) | (uintptr_t)k_in | (uintptr_t)v_in) & 15) == 0 && (interleaved ? rot % 8 == 0 : rot % 16 == 0);
     if (q_dtype == XR_F32) {
-        if (vec) k_rope_kv_write4<float, true><<<grid, 256, 0, stream>>>(a);
-        else k_rope_kv_write4<float, false><<<grid, 256, 0, stream>>>(a);
-    } else if (vec) k_rope_kv_write4<bf16_t, true><<<grid, 256, 0, stream>>>(a);
-    else k_rope_kv_write4<bf16_t, false><<<grid, 256, 0, stream>>>(a);
+        if (vec) k_rope_kv_write4<float, true, false><<<grid, 256, 0, stream>>>(a);
+        else k_rope_kv_write4<float, false, false><<<grid, 256, 0, stream>>>(a);
+    } else if (vec) k_rope_kv_write4<bf16_t, true, false><<<grid, 256, 0, stream>>>(a);
+    else k_rope_kv_write4<bf16_t, false, false><<<grid, 256, 0, stream>>>(a);
     XR_CHECK_LAUNCH("rope_kv_write4");
     return XR_OK;
 }
@@ -289,7 +367,8 @@ struct Read4Args {
     size_t k_total;
 };
 
-// Rows of a list of (request, position): a thread 8 channels of a head.  Rows without a page read as zeros.
+// Rows of a list of (request, position): a thread 8 channels of a head, whose codes are one word (of a value: 4 bytes 8 apart, in lines that the row's neighbours
+// share).  Rows without a page read as zeros.  Bound by what it writes: 2,048 rows of 8 heads of 128, 16 bits, take 7.2 us (8.4 MB out; the neighbours' lines come from L2), one 2.5.
 template <typename T>
 __global__ __launch_bounds__(256) void k_read_rows4(Read4Args a) {
     for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < a.total; i += (size_t)gridDim.x * 256) {
@@ -315,7 +394,8 @@ __global__ __launch_bounds__(256) void k_read_rows4(Read4Args a) {
 }
 
 // Whole pages in the layout of 16- and 32-bit caches (values transposed), a workgroup a page and head.  What lies behind a request's
-// end becomes zero, so that readers may multiply it.
+// end becomes zero, so that readers may multiply it.  Bound by memory: 32,768 positions of 8 heads of 128 (36 MB in, 134 MB out, 16 bits) take 27.4 us, 6.2 TB/s;
+// 13,300 of 8 heads of 64 in 32 bits (7 MB in, 55 MB out) 13.5, 4.6 TB/s.
 template <typename T>
 __global__ __launch_bounds__(256) void k_read_pages4(Read4Args a) {
     const int n = blockIdx.x / a.Hk, h = blockIdx.x - n * a.Hk;
@@ -402,7 +482,10 @@ extern "C" int xr_read_pages4(void* k_out, void* v_out, void* kc, void* ks, void
 // ---------------------------------------------------------------- attention, any head size
 // Attention over 4-bit pages in 32 bits: a workgroup a token and query head, its waves 64 keys a turn each; a key a lane for the scores, a pair of channels a
 // lane for the values, 8 positions at a time as they lie side by side; the options of k_attention_ref.  For what the matrix-core kernel does not take: 32-bit
-// queries, and in recorded steps, whose pages cannot be read back first, other head sizes and kept first keys.
+// queries of few rows, head sizes that end inside a block and, in recorded steps, whose pages cannot be read back first, the other sizes and kept first keys.
+//
+// Bound by instructions: every query head converts its keys and values again, and beside a product stand half a conversion and the shared memory's reads of the
+// query.  8 requests of 4,000 keys, 32 heads of 128 over 8, take 57 us (9 TFLOP/s; channel by channel with a byte a load 252), 64 of 8,000 with heads of 64 344 (12 TFLOP/s).
 #define ANY4_WAVES 8
 struct Any4Args {
     Pages4 pages;
