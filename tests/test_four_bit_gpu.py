@@ -422,6 +422,13 @@ def test_other_head_sizes(ops, what, shape, mask, dt):
     attend(ops, (H, Hk, D, Dv, page, mask, [0, 6, 129, 61, 530], [1, 2, 9, 1, 1]), dt, 200 + D + len(what), **OPTIONS.get(what, {}))
 
 
+@pytest.mark.parametrize("what", ["", *OPTIONS])
+@pytest.mark.parametrize("D,mask", [(64, None), (128, 90), (40, Chunked(100))])
+def test_many_rows_in_32_bits(ops, what, D, mask):
+    """Steps of rows enough for pages that are read back."""
+    attend(ops, (16, 2, D, D, 32, mask, [37, 0, 300], [230, 40, 1]), "float32", 300 + D + len(what), **OPTIONS.get(what, {}))
+
+
 MANY = [
     # H, Hk, D, Dv, page, mask, starts, q_lens: more than 16 rows a key/value head
     (8, 2, 128, 128, 64, None, [0, 61, 700], [5, 33, 17]),

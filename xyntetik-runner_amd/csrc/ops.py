@@ -1227,12 +1227,13 @@ class Ops:
                         _ptr(plan.jobs), plan.n_jobs, ctx.cu_q.data_ptr(), ctx.starts_dev.data_ptr(), table.data_ptr(), table.stride(0), part_o, part_ml,
                         H, Hk, D, Dv, page_size, float(scale), window, chunk, _ptr(slopes), _ptr(sinks), float(softcap), *gating))
                 return out
-        # Pages are read back for what then runs on matrix cores: 16-bit queries, and 32-bit ones of more than 16 rows a request (8 requests of 4,000 keys, 32 heads
-        # over 8, codes and pages: 1 row 59 us and 441, 8 rows 282 and 540, 16 rows 517 and 540, 64 rows 1,904 and 1,002).  What is left for the kernel that takes a
+        # Pages are read back for what then runs on matrix cores: 16-bit queries, and 32-bit ones where the kernel that takes 32 rows of a request and head a
+        # workgroup, a key after the other, has rows enough for its rounds of 512 workgroups (32 heads over 8, codes and pages, us: 8 requests of 4,000 keys with 1 row 59 and 441, 8 rows 270 and
+        # 540, 16 rows 492 and 540, 64 rows 1,888 and 1,005; one of 2,000 with 64 rows, heads of 64, 77 and 158; of 512 with 512 rows 229 and 138).  What is left for the kernel that takes a
         # row and head at a time reads the codes itself (8 requests of 2,000 keys, heads of 72: 1 row 29 us and 769, 64 rows 834 and 15,227).
         cores = (self.attention_on_matrix_cores(dtype, D, Dv, page_size) and not (softcap and slopes is not None) and (D == Dv or not keep_first)
                  and ld_out % 4 == 0 and at % 8 == 0)
-        if knows and (cores or (dtype is torch.float32 and max(D, Dv) <= 128 and max(ctx.q_lens) > 16)):
+        if knows and (cores or (dtype is torch.float32 and max(D, Dv) <= 128 and T * H > 3500 * -(-sum(-(-n // 32) for n in ctx.q_lens) * H // 512))):
             k16, v16, table = self.read_pages(k_pages, v_pages, ctx, group, dtype, None, window, chunk, keep_first)
             return self.attention(q, k16, v16, _PagesOf(ctx, table), group, H, Hk, D, page_size, scale, window or None, slopes, chunk or None, keep_first, sinks, Dv,
                                      softcap, gate, out_scale, out)
