@@ -429,6 +429,31 @@ def test_many_rows_in_32_bits(ops, what, D, mask):
     attend(ops, (16, 2, D, D, 32, mask, [37, 0, 300], [230, 40, 1]), "float32", 300 + D + len(what), **OPTIONS.get(what, {}))
 
 
+@pytest.mark.parametrize("case", [(4, 2, 80, 48, 16, 50, [10, 130], [40, 1]), (16, 2, 64, 64, 32, None, [37, 300], [260, 1])])
+@pytest.mark.parametrize("dt", ["bfloat16", "float32"])
+def test_pages_too_many_to_be_read_back(ops, case, dt, monkeypatch):
+    monkeypatch.setattr(ops, "READ_BACK_BYTES", 1000)
+    monkeypatch.setattr(ops, "read_pages", None)
+    attend(ops, case, dt, 500, keep=3)
+
+
+@pytest.mark.parametrize("D", [64, 72])
+def test_a_page_that_the_cache_does_not_have(ops, D):
+    """A table's number past the pool's is no page, like -1."""
+    from xyntetik_runner_amd.csrc.ops import FourBitPages
+    rng, got = np.random.default_rng(5), []
+    ks, vs = ([F.random_sequence(rng, 200, 2, D)] for _ in range(2))
+    q = torch.tensor(rng.normal(size=(1, 4 * D)), device=DEV).bfloat16()
+    for bad in (-1, 7, 1 << 30):
+        tables = [[1, 2, bad, 3, 4, 5, 6]]
+        kp, vp = (on_gpu(*F.fill_pages(x, [[1, 2, 0, 3, 4, 5, 6]], 7, 32, values), D) for x, values in ((ks, False), (vs, True)))
+        ctx = step([199], [1], tables)
+        got.append([ops.attention(q, kp, vp, c, 0, 4, 2, D, 32, D ** -0.5).cpu() for c in (ctx, Recorded(ctx))])
+    for other in got[1:]:
+        for a, b in zip(got[0], other):
+            assert torch.isfinite(a).all() and torch.equal(a, b)
+
+
 MANY = [
     # H, Hk, D, Dv, page, mask, starts, q_lens: more than 16 rows a key/value head
     (8, 2, 128, 128, 64, None, [0, 61, 700], [5, 33, 17]),

@@ -149,3 +149,12 @@ def test_which_requests_are_read_back():
     assert four_row_requests([60000], [512], 4, None, 8) == [] and four_row_requests([60000], [512], 4, 1024, 8) == [0]      # a window leaves little to do
     assert four_row_requests([0], [FOUR_ROWS + 1], 1, None, 32) == [0]
     assert four_row_slots(1500, 8, 256) == 2 * four_row_slots(280, 8, 256) == 512 and four_row_slots(10 ** 6, 8, 512) == 256
+
+
+def test_pages_keep_their_tensors():
+    from xyntetik_runner_amd.csrc.ops import FourBitPages
+    pages = FourBitPages.zeros(2, 1, 16, 32, False, "cpu")
+    assert pages.pointers == (pages.codes.data_ptr(), pages.scales.data_ptr())
+    for name in ("codes", "scales"):
+        with pytest.raises(AttributeError):
+            setattr(pages, name, torch.zeros(1))

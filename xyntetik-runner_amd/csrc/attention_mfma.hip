@@ -86,6 +86,7 @@ struct AttnArgs {
     float out_scale;
     int ld_out;
     Pages4 four;            // the cache where it is held in 4 bits (kc and vc are not read then)
+    int n_pages;            // its pages: a table's other numbers are none
 };
 
 __device__ inline float row_factor(const float* gate, int ld_gate, float out_scale, int t, int h) {
@@ -1590,7 +1591,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES, FOUR_PER_CU) void k_attn_few4(AttnA
         const int pi = pages_base + lane;
         const bool in = ((long)pi << a.page_shift) < seq_len;
         my_page = bt[in ? pi : 0];
-        my_page = in ? my_page : -1;
+        my_page = in && (unsigned)my_page < (unsigned)a.n_pages ? my_page : -1;
     };
     look_up();
 
@@ -1949,7 +1950,7 @@ extern "C" int xr_attention_mfma(void* out, const void* q, const void* k_cache, 
 }
 
 // Requests of few rows over a cache held in 4 bits (``few_items`` as in xr_attention_mfma).
-extern "C" int xr_attention_few4(void* out, const void* q, const void* kc, const void* ks, const void* vc, const void* vs, const int* few_items, int n_few,
+extern "C" int xr_attention_few4(void* out, const void* q, const void* kc, const void* ks, const void* vc, const void* vs, int n_pages, const int* few_items, int n_few,
                                  int* counters, const int* block_table, int table_stride, float* part_o, float* part_ml, int H, int Hk, int D, int Dv,
                                  int page_size, float scale, int window, int chunk, const float* slopes, const float* sinks, float cap, const float* gate,
                                  int ld_gate, float out_scale, int ld_out, hipStream_t stream) {
@@ -1967,7 +1968,7 @@ extern "C" int xr_attention_few4(void* out, const void* q, const void* kc, const
     XR_REQUIRE((((uintptr_t)q | (uintptr_t)kc | (uintptr_t)vc) & 15) == 0 && (((uintptr_t)ks | (uintptr_t)vs) & 7) == 0, "attention: queries and codes must be 16-byte aligned, scales 8-byte");
     AttnArgs a = {};
     a.q = (const bf16_t*)q; a.out = (bf16_t*)out; a.few_items = few_items; a.n_few = n_few; a.counters = counters;
-    a.four = Pages4{(uint8_t*)kc, (uint8_t*)ks, (uint8_t*)vc, (uint8_t*)vs};
+    a.four = Pages4{(uint8_t*)kc, (uint8_t*)ks, (uint8_t*)vc, (uint8_t*)vs}; a.n_pages = n_pages;
     a.block_table = block_table; a.table_stride = table_stride; a.part_o = part_o; a.part_ml = part_ml; a.H = H; a.Hk = Hk;
     a.page_shift = shift; a.page_mask = page_size - 1; a.page_size = page_size; a.scale = scale; a.window = window; a.chunk = chunk;
     a.slopes = slopes; a.sinks = sinks; a.cap = cap; a.gate = gate; a.ld_gate = ld_gate; a.out_scale = out_scale; a.ld_out = ld_out;

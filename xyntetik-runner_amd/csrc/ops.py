@@ -186,7 +186,7 @@ class FourBitPages:
     BLOCK = 32
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, dim: int):
-        self.codes, self.scales, self.dim = codes, scales, int(dim)
+        self._codes, self._scales, self.dim = codes, scales, int(dim)
         self.values = codes.dim() == 5
         self.num_pages, self.heads = int(codes.shape[0]), int(codes.shape[1])
         self.page_size = int(codes.shape[2]) * (8 if self.values else 1)
@@ -197,9 +197,7 @@ class FourBitPages:
         if not codes.is_contiguous() or not scales.is_contiguous() or codes.data_ptr() % 16 or scales.data_ptr() % 8:
             raise KernelError("4-bit pages: codes and scales must be contiguous, 16 and 8 bytes aligned")
         self.device, self.is_cuda, self.index = codes.device, codes.is_cuda, codes.get_device()
-        # what a pair of keys and values has in common, and where the bytes are (the tensors are never replaced)
-        self.layout = (self.num_pages, self.heads, self.page_size, self.device)
-        self.pointers = (codes.data_ptr(), scales.data_ptr())
+        self.layout = (self.num_pages, self.heads, self.page_size, self.device)     # what a pair of keys and values has in common
 
     @staticmethod
     def shapes(pages: int, heads: int, page_size: int, dim: int, values: bool):
@@ -215,6 +213,18 @@ class FourBitPages:
     def zeros(cls, pages: int, heads: int, page_size: int, dim: int, values: bool, device) -> "FourBitPages":
         codes, scales = cls.shapes(pages, heads, page_size, dim, values)
         return cls(torch.zeros(codes, dtype=torch.uint8, device=device), torch.zeros(scales, dtype=torch.uint8, device=device), dim)
+
+    @property
+    def codes(self) -> torch.Tensor:        # (never replaced: the sizes above are theirs)
+        return self._codes
+
+    @property
+    def scales(self) -> torch.Tensor:
+        return self._scales
+
+    @property
+    def pointers(self):
+        return self._codes.data_ptr(), self._scales.data_ptr()
 
     def get_device(self) -> int:
         return self.index
@@ -512,6 +522,7 @@ class Ops:
     # With 4-bit pages up to here: a product whose ranges stay to be added up is one launch of one tile, which costs more rows more than the other kernel saves
     # (32 + 2 * 8 heads of 128, 8 of 64, 32 of 128, one kernel and two, us: 256 rows 32.8, 37.7; 19.8, 23.5; 49.1, 51.8; 300 37.7, 39.4; 22.7, 25.0; 58.1, 56.4; 450 44.7, 43.4; 26.4, 25.0; 72.6, 68.1).
     FOUR_FINISH_ROWS = 320
+    READ_BACK_BYTES = 2 << 30       # a step's 4-bit pages of a layer are read back whole up to here; beyond, rows are served from the codes, slower but in no memory of their own
 
     def _gemm_workspace(self, device):
         """Room for the sums of K ranges when a product with few rows is split (one buffer per process;
@@ -1029,7 +1040,7 @@ class Ops:
         if w.shape[0] != Q + 2 * KV:
             raise KernelError(f"projection has {w.shape[0]} rows, {H} query and 2 x {Hk} key/value heads of {D} need {Q + 2 * KV}")
         q = torch.empty((T, Q), dtype=rows.dtype, device=rows.device)
-        four = isinstance(k_cache, FourBitPages)
+        four = Hk > 0 and isinstance(k_cache, FourBitPages)
         if (self.fuse_rope and (T <= self.FINISH_ROWS or T >= self.ROPE_TILE_ROWS) and self._mfma_ok(rows, wt) and D % 16 == 0
                 and (T * w.shape[0] * 4 if T <= self.FINISH_ROWS else T * (rot // 2 + 1) * 8) <= self.GEMM_WORKSPACE_BYTES
                 and (Hk == 0 or (k_cache.dtype == torch.bfloat16 and v_cache.dtype == torch.bfloat16) or
@@ -1216,7 +1227,7 @@ class Ops:
                     part_ml = part_o + plan.n_slots * Hk * 32 * Dv * 4
                 if plan.n_few:
                     lib.check(lib.xr_attention_few4(
-                        at, q.data_ptr(), *pages[:4], plan.few.data_ptr(), plan.n_few, plan.counters.data_ptr(), block_table.data_ptr(),
+                        at, q.data_ptr(), *pages, plan.few.data_ptr(), plan.n_few, plan.counters.data_ptr(), block_table.data_ptr(),
                         block_table.stride(0), part_o, part_ml, H, Hk, D, Dv, page_size, float(scale), window, chunk, _ptr(slopes), _ptr(sinks),
                         float(softcap), *gating))
                 if rest:
@@ -1233,7 +1244,7 @@ class Ops:
         # row and head at a time reads the codes itself (8 requests of 2,000 keys, heads of 72: 1 row 29 us and 769, 64 rows 834 and 15,227).
         cores = (self.attention_on_matrix_cores(dtype, D, Dv, page_size) and not (softcap and slopes is not None) and (D == Dv or not keep_first)
                  and ld_out % 4 == 0 and at % 8 == 0)
-        if knows and (cores or (dtype is torch.float32 and max(D, Dv) <= 128 and T * H > 3500 * -(-sum(-(-n // 32) for n in ctx.q_lens) * H // 512))):
+        if knows and self._pages_back(ctx, page_size, window) * Hk * (D + Dv) * q.element_size() <= self.READ_BACK_BYTES and (cores or (dtype is torch.float32 and max(D, Dv) <= 128 and T * H > 3500 * -(-sum(-(-n // 32) for n in ctx.q_lens) * H // 512))):
             k16, v16, table = self.read_pages(k_pages, v_pages, ctx, group, dtype, None, window, chunk, keep_first)
             return self.attention(q, k16, v16, _PagesOf(ctx, table), group, H, Hk, D, page_size, scale, window or None, slopes, chunk or None, keep_first, sinks, Dv,
                                      softcap, gate, out_scale, out)
@@ -1241,6 +1252,11 @@ class Ops:
             at, q.data_ptr(), *pages, positions.data_ptr(), req_of_token.data_ptr(), block_table.data_ptr(), block_table.stride(0), T, H, Hk, D, Dv,
             page_size, float(scale), window, chunk, int(keep_first), dtype_code(dtype), _ptr(slopes), _ptr(sinks), float(softcap), *gating))
         return out
+
+    @staticmethod
+    def _pages_back(ctx, page_size: int, window: int) -> int:
+        """Positions of all pages that a step's rows read, at most."""
+        return sum((-(-(min(s, n + window) if window else s) // page_size) + 1) * page_size for s, n in zip(ctx.seq_lens, ctx.q_lens))
 
     def attention_on_matrix_cores(self, dtype: torch.dtype, D: int, Dv: int, page_size: int = 64) -> bool:
         """Whether keys of ``D`` and values of ``Dv`` channels have matrix-core attention kernels."""
@@ -1328,7 +1344,7 @@ class Ops:
             path = _build.find_built(unit) or _build.build_unit(unit)
             lib = _Lib(path, {"xr_attention_mfma": [_p, _p, _p, _p, _p, _i, _i, _p, _i, _p, _p, _i, _p, _p, _p, _i, _p, _p,
                                                     _i, _i, _i, _i, _i, _f, _i, _i, _p, _p, _f, _p, _i, _f, _i, _p],
-                              "xr_attention_few4": [_p] * 7 + [_i, _p, _p, _i, _p, _p] + [_i] * 5 + [_f, _i, _i, _p, _p, _f, _p, _i, _f, _i, _p]})
+                              "xr_attention_few4": [_p] * 6 + [_i, _p, _i, _p, _p, _i, _p, _p] + [_i] * 5 + [_f, _i, _i, _p, _p, _f, _p, _i, _f, _i, _p]})
             self._attn_libs[(D, Dv)] = lib
         return lib
 

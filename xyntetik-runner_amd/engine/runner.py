@@ -84,8 +84,9 @@ class ModelRunner:
             # what torch holds without having handed it out is as good as free
             free += torch.cuda.memory_reserved(self.device) - torch.cuda.memory_allocated(self.device)
             working = max(1 << 30, (max_step_tokens or 2048) << 20)     # a step's activations, generously
-            if four_bit and specs:      # and the longest request's pages of a layer, read back for the attention of a portion
-                working += max(page_bytes(s, 1, page_size, elt) for s in specs) * -(-(max_model_len or spec.max_position) // page_size)
+            if four_bit and specs:      # and pages of a layer that are read back: the longest request's for the attention of a portion, or a step's
+                working += max(self.ops.READ_BACK_BYTES,
+                               max(page_bytes(s, 1, page_size, elt) for s in specs) * -(-(max_model_len or spec.max_position) // page_size))
             sizes = size_pools(specs, owners, page_size, elt, max_requests, max_step_tokens,
                                budget_bytes=memory_budget(total, free, gpu_memory_fraction, working),
                                max_model_len=max_model_len or spec.max_position, four_bit=four_bit)
