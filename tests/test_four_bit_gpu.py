@@ -477,6 +477,20 @@ def test_attention_of_many_rows(ops, case, slots, what, monkeypatch):
     attend(ops, case, "bfloat16", 31 + case[2] + len(what), **OPTIONS.get(what, {}))
 
 
+@pytest.mark.parametrize("what", ["", "sinks", "cap and sinks", "slopes, sinks, gate"])
+@pytest.mark.parametrize("case", [(16, 1, 128, 128, 32, None, [3000, 40], [1, 1]), (8, 1, 256, 256, 64, None, [2500], [1]), (10, 1, 256, 224, 64, 900, [5000, 777, 3], [2, 1, 3]),
+                                  (34, 2, 128, 128, 64, Chunked(600), [599, 1100], [1, 1])])
+def test_ranges_added_up_apart(ops, case, what, monkeypatch):
+    """Blocks of many numbers in several key ranges, a request of one range among them."""
+    from xyntetik_runner_amd.engine import batch
+    monkeypatch.setattr(batch, "FEW_MANY", 1)
+    H, Hk, D, Dv, page, mask, starts, q_lens = case
+    ctx = step(starts, q_lens, scattered(np.random.default_rng(0), [s + n for s, n in zip(starts, q_lens)], page)[0])
+    plan = ctx.attention_plan(0, H // Hk, mask, Hk, page, few_rows=3, few_channels=D + Dv)
+    assert plan.merge_rows * Dv >= 2048
+    attend(ops, case, "bfloat16", 900 + D + len(what), **OPTIONS.get(what, {}))
+
+
 @pytest.mark.parametrize("case", MANY[:3])
 @pytest.mark.parametrize("rows", [0, 16, 70])
 def test_codes_beside_pages_read_back(ops, case, rows, monkeypatch):

@@ -35,17 +35,18 @@ def four(x):
 def models(tmp_path_factory):
     """name -> (folder, vocabulary, requests, prompt lengths, logits with a 4-bit cache, logits with a 64-bit one)."""
     out = {}
-    for name in ("A", "B", "D", "W", "G6", "G7"):
+    for name in ("A", "B", "D", "W", "X", "G6", "G7"):
         d = str(tmp_path_factory.mktemp("four" + name))
-        lens, extra = ([3, 40, 64, 90], 24) if name != "D" else ([2, 130, 300], 24)
+        lens, extra = ([3, 40, 64, 90], 24) if name not in "DX" else ([2, 130, 300], 24)
         if name.startswith("G"):
             girolorn_tiny.make_model(name, d)
             cfg, w = PL.load_folder(d)
             vocab, plain, place, attr = cfg["vocab"], lambda t: PG.forward(cfg, w, t), PG, "attend"
         else:
-            if name == "W":         # more heads over one key/value head than a block of rows holds
+            if name in "WX":        # more heads over one key/value head than a block of rows holds; blocks whose key ranges a kernel of its own adds up
                 from xyntetik_runner_amd.weights import write_random_model
-                write_random_model(dict(tiny.TINY_B, num_attention_heads=21, num_key_value_heads=1, head_dim=64), d, seed=7, std=0.05)
+                heads, dim = {"W": (21, 64), "X": (16, 128)}[name]
+                write_random_model(dict(tiny.TINY_B, num_attention_heads=heads, num_key_value_heads=1, head_dim=dim), d, seed=7, std=0.05)
             else:
                 tiny.make_model(name, d)
             cfg, w = PL.load_folder(d)
@@ -70,7 +71,7 @@ def error(got, want):
 
 @pytest.mark.parametrize("schedule", ["whole", "tail", "portions", "mixed"])
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
-@pytest.mark.parametrize("name,page", [("A", 16), ("B", 32), ("D", 64), ("W", 32), ("G6", 8), ("G7", 64)])
+@pytest.mark.parametrize("name,page", [("A", 16), ("B", 32), ("D", 64), ("W", 32), ("X", 32), ("G6", 8), ("G7", 64)])
 def test_every_way_of_cutting(models, tmp_path, name, page, dtype, schedule):
     from xyntetik_runner_amd.engine.runner import ModelRunner
     from xyntetik_runner_amd.trace import replay

@@ -87,6 +87,7 @@ struct AttnArgs {
     int ld_out;
     Pages4 four;            // the cache where it is held in 4 bits (kc and vc are not read then)
     int n_pages;            // its pages: a table's other numbers are none
+    int apart;              // 1: the key ranges of few rows are added up by a kernel of their own (k_few_merge), not by the last workgroup
 };
 
 __device__ inline float row_factor(const float* gate, int ld_gate, float out_scale, int t, int h) {
@@ -1111,6 +1112,45 @@ __device__ __forceinline__ float2 load_agent(const float* p) {
     return make_float2(__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32)));
 }
 
+// A pair of channels of a row: its `ns` ranges from slot s0 on weighed and added up, 16 at a time, and the result stored
+__device__ __forceinline__ void few_add_up(const AttnArgs& a, int s0, int ns, int kvh, int r, int d2, int row0, int q0, int G) {
+    const size_t ml_step = (size_t)a.Hk * ROWS * 2, po_step = (size_t)a.Hk * ROWS * HV;
+    const float* ml = a.part_ml + (((size_t)s0 * a.Hk + kvh) * ROWS + r) * 2;
+    const float* po = a.part_o + (((size_t)s0 * a.Hk + kvh) * ROWS + r) * HV + d2;
+    constexpr int U = 16;
+    float mx = -INFINITY, wsum = 0.f;
+    float2 acc = make_float2(0.f, 0.f);
+    for (int b = 0; b < ns; b += U) {
+        float2 mlv[U], pv[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int sc = b + u < ns ? b + u : b;
+            mlv[u] = load_agent(ml + sc * ml_step);
+            pv[u] = load_agent(po + sc * po_step);
+        }
+        __builtin_amdgcn_sched_barrier(0);           // (or the first numbers are waited for one by one: 2 us)
+        float cm = mx;
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (b + u < ns) cm = fmaxf(cm, mlv[u].x);
+        const float resc = mx == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mx - cm);
+        acc.x *= resc; acc.y *= resc;
+        wsum *= resc;
+        mx = cm;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const float w = (b + u < ns && mlv[u].y > 0.f) ? mlv[u].y * __builtin_amdgcn_exp2f(mlv[u].x - mx) : 0.f;
+            acc.x += w * pv[u].x; acc.y += w * pv[u].y;
+            wsum += w;
+        }
+    }
+    const int rr = row0 + r, tk = rr / G, hh = kvh * G + (rr - tk * G);
+    wsum = with_sink(a.sinks, hh, mx, wsum);
+    const float inv = (wsum > 0.f ? 1.0f / wsum : 0.f) * row_factor(a.gate, a.ld_gate, a.out_scale, q0 + tk, hh);
+    bf16_t* op = a.out + (size_t)(q0 + tk) * a.ld_out + hh * HV + d2;
+    *reinterpret_cast<uint32_t*>(op) = pack2(acc.x * inv, acc.y * inv);
+}
+
 // The end of a kernel for few rows: every wave has left its rows' unnormalised outputs in `mo`, their references and sums in `mml`; they are combined
 // here (sum_w 2^(m_w - max) O_w over sum_w 2^(m_w - max) l_w), and the row block's key ranges added up.
 constexpr int FEW_MS = HV + 4;                                // floats between rows of the combining buffer
@@ -1147,7 +1187,7 @@ template <int PB> __device__ __forceinline__ void few_finish(const AttnArgs& a, 
             if (d2 == 0) store_agent(a.part_ml + (((size_t)slot * a.Hk + kvh) * ROWS + r) * 2, mx, lsum);
         }
     }
-    if (slot < 0) return;
+    if (slot < 0 || a.apart) return;
 
     // ---- the last of a row block's workgroups adds the key ranges up.  Each has its partial result where all others read it
     // (the wait is for this wave's own stores) before it counts itself in; the counter is zero again afterwards.
@@ -1163,45 +1203,11 @@ template <int PB> __device__ __forceinline__ void few_finish(const AttnArgs& a, 
     __syncthreads();
     if (!*last_one) return;
     const int total = n_rows * (HV / 2);
-    const size_t ml_step = (size_t)a.Hk * ROWS * 2, po_step = (size_t)a.Hk * ROWS * HV;
     if (total <= 64 * FEW_WAVES) {
         // a pair of channels a thread, which weighs its row's ranges by itself, 16 at a time
         if (tid >= total) return;
         const int r = tid / (HV / 2), d2 = (tid - r * (HV / 2)) * 2;
-        const float* ml = a.part_ml + (((size_t)s0 * a.Hk + kvh) * ROWS + r) * 2;
-        const float* po = a.part_o + (((size_t)s0 * a.Hk + kvh) * ROWS + r) * HV + d2;
-        constexpr int U = 16;
-        float mx = -INFINITY, wsum = 0.f;
-        float2 acc = make_float2(0.f, 0.f);
-        for (int b = 0; b < ns; b += U) {
-            float2 mlv[U], pv[U];
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int sc = b + u < ns ? b + u : b;
-                mlv[u] = load_agent(ml + sc * ml_step);
-                pv[u] = load_agent(po + sc * po_step);
-            }
-            __builtin_amdgcn_sched_barrier(0);           // (or the first numbers are waited for one by one: 2 us)
-            float cm = mx;
-#pragma unroll
-            for (int u = 0; u < U; ++u)
-                if (b + u < ns) cm = fmaxf(cm, mlv[u].x);
-            const float resc = mx == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mx - cm);
-            acc.x *= resc; acc.y *= resc;
-            wsum *= resc;
-            mx = cm;
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const float w = (b + u < ns && mlv[u].y > 0.f) ? mlv[u].y * __builtin_amdgcn_exp2f(mlv[u].x - mx) : 0.f;
-                acc.x += w * pv[u].x; acc.y += w * pv[u].y;
-                wsum += w;
-            }
-        }
-        const int rr = row0 + r, tk = rr / G, hh = kvh * G + (rr - tk * G);
-        wsum = with_sink(a.sinks, hh, mx, wsum);
-        const float inv = (wsum > 0.f ? 1.0f / wsum : 0.f) * row_factor(a.gate, a.ld_gate, a.out_scale, q0 + tk, hh);
-        bf16_t* op = a.out + (size_t)(q0 + tk) * a.ld_out + hh * HV + d2;
-        *reinterpret_cast<uint32_t*>(op) = pack2(acc.x * inv, acc.y * inv);
+        few_add_up(a, s0, ns, kvh, r, d2, row0, q0, G);
         return;
     }
     // More: 16 lanes a row weigh its ranges, 64 of them a turn, while a thread's pairs of channels are on their way, up to 64 loads.  (As above, a pair after
@@ -1210,6 +1216,7 @@ template <int PB> __device__ __forceinline__ void few_finish(const AttnArgs& a, 
     float* const weight = mo;                            // [FEW_ROWS][FEW_TURN]
     float* const factor = mml;                           // [FEW_ROWS] what a turn's sums before it are multiplied by, then [FEW_ROWS] the results
     const int wr = tid >> 4, wj = tid & 15;
+    const size_t ml_step = (size_t)a.Hk * ROWS * 2, po_step = (size_t)a.Hk * ROWS * HV;
     const float* const ml = a.part_ml + (((size_t)s0 * a.Hk + kvh) * ROWS + (wr < n_rows ? wr : 0)) * 2;
     const float* const po = a.part_o + ((size_t)s0 * a.Hk + kvh) * ROWS * HV;      // (a row block's rows lie one after the other)
     constexpr int U = 16;
@@ -1519,6 +1526,11 @@ constexpr int KS4 = FKD % 4 == 0 ? FKD / 4 : 4 % FKD == 0 ? 1 : FKD;      // sca
 constexpr int VP4 = FDB >= 2 ? FDB / 2 : 1;                               // pairs of channels of a lane
 constexpr int VS4 = 32 % FDB == 0 ? 1 : VP4;                              // scales of its values: one, or pair by pair
 constexpr int FOUR_PER_CU = HD + HV <= 256 ? 3 : 2;
+// A kernel of its own adds the ranges up (k_few_merge) where they are many (the caller's `merge_rows`) and blocks have this many numbers: the last workgroup's trips to
+// memory, 64 KB on their way at a time (43 GB/s), then take longer than a launch.  In recorded steps, us, with it and without: 16 heads over one of 256 channels, one request
+// of 20,000 keys 18.1 and 26.6, 16 of 3,000 15.6 and 19.8; of 128 one of 500 8.1 and 9.3, 4 of 20,000 12.5 and 16.2; 8 over one of 256, 20,000 15.7 and 18.8; but 4 over one
+// of 256 (1,024 numbers) 16 of 3,000 19.3 and 17.8, 8 over one of 128, 131,072 keys 32.3 and 31.3, and five requests of 12 tokens, 60 blocks of 4 ranges, 21.8 and 21.1.
+constexpr int FEW_APART = 2048;
 constexpr int FOUR_PAIRS = FEW_PAIRS < 2 ? FEW_PAIRS : 2;
 typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
 
@@ -1793,6 +1805,17 @@ __global__ __launch_bounds__(64 * FEW_WAVES, FOUR_PER_CU) void k_attn_few4(AttnA
     }
 }
 
+// The key ranges of blocks of few rows, a pair of channels a thread, a workgroup (item's first range, key/value head, 256 of its pairs): see xr_attention_few4.
+__global__ __launch_bounds__(256) void k_few_merge(AttnArgs a) {
+    const int item_no = (int)(blockIdx.x / (unsigned)a.Hk), kvh = (int)blockIdx.x - item_no * a.Hk;
+    const int* it = a.few_items + (size_t)item_no * FEW_INTS;
+    if (it[3] <= it[2] || it[4] < 0 || it[4] != it[8]) return;       // (padding, a block with one range, ranges but the first)
+    const int G = a.H / a.Hk, row0 = it[1], q0 = it[5], q_len = it[6];
+    const int n_rows = q_len * G - row0 < FEW_ROWS ? q_len * G - row0 : FEW_ROWS;
+    const int idx = (int)blockIdx.y * 256 + threadIdx.x, r = idx / (HV / 2);
+    if (r < n_rows) few_add_up(a, it[8], it[9], kvh, r, (idx - r * (HV / 2)) * 2, row0, q0, G);
+}
+
 // One merge job: {req, row0, first_slot, n_slots, slot_stride, q0, q_len}.  Slot s holds the normalised output of
 // its keys with their maximum m_s (in units of log2) and sum l_s; the whole is
 // sum_s w_s O_s / sum_s w_s with w_s = l_s * 2^(m_s - max m).
@@ -1950,7 +1973,7 @@ extern "C" int xr_attention_mfma(void* out, const void* q, const void* k_cache, 
 }
 
 // Requests of few rows over a cache held in 4 bits (``few_items`` as in xr_attention_mfma).
-extern "C" int xr_attention_few4(void* out, const void* q, const void* kc, const void* ks, const void* vc, const void* vs, int n_pages, const int* few_items, int n_few,
+extern "C" int xr_attention_few4(void* out, const void* q, const void* kc, const void* ks, const void* vc, const void* vs, int n_pages, const int* few_items, int n_few, int merge_rows,
                                  int* counters, const int* block_table, int table_stride, float* part_o, float* part_ml, int H, int Hk, int D, int Dv,
                                  int page_size, float scale, int window, int chunk, const float* slopes, const float* sinks, float cap, const float* gate,
                                  int ld_gate, float out_scale, int ld_out, hipStream_t stream) {
@@ -1963,12 +1986,14 @@ extern "C" int xr_attention_few4(void* out, const void* q, const void* kc, const
     XR_REQUIRE(cap >= 0.f && !(cap > 0.f && slopes), "attention: a soft cap %g of the scores needs no slopes", (double)cap);
     XR_REQUIRE(ld_out >= H * HV && ld_out % 2 == 0 && ((uintptr_t)out % 4) == 0 && (!gate || ld_gate >= H), "attention: output rows %d apart (a gate's %d)", ld_out, ld_gate);
     XR_REQUIRE(n_few >= 0 && (long long)n_few * Hk < (1LL << 31), "attention: %d blocks of few rows of %d key/value heads", n_few, Hk);
+    XR_REQUIRE(merge_rows >= 0 && merge_rows <= FEW_ROWS, "attention: blocks of %d rows", merge_rows);
     if (n_few == 0) return XR_OK;
     XR_REQUIRE(out && q && kc && ks && vc && vs && few_items && counters && block_table, "attention: a null operand");
     XR_REQUIRE((((uintptr_t)q | (uintptr_t)kc | (uintptr_t)vc) & 15) == 0 && (((uintptr_t)ks | (uintptr_t)vs) & 7) == 0, "attention: queries and codes must be 16-byte aligned, scales 8-byte");
     AttnArgs a = {};
     a.q = (const bf16_t*)q; a.out = (bf16_t*)out; a.few_items = few_items; a.n_few = n_few; a.counters = counters;
     a.four = Pages4{(uint8_t*)kc, (uint8_t*)ks, (uint8_t*)vc, (uint8_t*)vs}; a.n_pages = n_pages;
+    a.apart = part_o && merge_rows * HV >= FEW_APART;
     a.block_table = block_table; a.table_stride = table_stride; a.part_o = part_o; a.part_ml = part_ml; a.H = H; a.Hk = Hk;
     a.page_shift = shift; a.page_mask = page_size - 1; a.page_size = page_size; a.scale = scale; a.window = window; a.chunk = chunk;
     a.slopes = slopes; a.sinks = sinks; a.cap = cap; a.gate = gate; a.ld_gate = ld_gate; a.out_scale = out_scale; a.ld_out = ld_out;
@@ -1977,5 +2002,9 @@ extern "C" int xr_attention_few4(void* out, const void* q, const void* kc, const
     else if (slopes) k_attn_few4<MODE_SLOPES><<<grid, 64 * FEW_WAVES, 0, stream>>>(a);
     else k_attn_few4<MODE_PLAIN><<<grid, 64 * FEW_WAVES, 0, stream>>>(a);
     XR_CHECK_LAUNCH("attention_few4");
+    if (a.apart) {
+        k_few_merge<<<dim3((unsigned)n_few * (unsigned)Hk, (unsigned)((merge_rows * (HV / 2) + 255) / 256)), 256, 0, stream>>>(a);
+        XR_CHECK_LAUNCH("few_merge");
+    }
     return XR_OK;
 }

@@ -1227,7 +1227,7 @@ class Ops:
                     part_ml = part_o + plan.n_slots * Hk * 32 * Dv * 4
                 if plan.n_few:
                     lib.check(lib.xr_attention_few4(
-                        at, q.data_ptr(), *pages, plan.few.data_ptr(), plan.n_few, plan.counters.data_ptr(), block_table.data_ptr(),
+                        at, q.data_ptr(), *pages, plan.few.data_ptr(), plan.n_few, plan.merge_rows, plan.counters.data_ptr(), block_table.data_ptr(),
                         block_table.stride(0), part_o, part_ml, H, Hk, D, Dv, page_size, float(scale), window, chunk, _ptr(slopes), _ptr(sinks),
                         float(softcap), *gating))
                 if rest:
@@ -1344,7 +1344,7 @@ class Ops:
             path = _build.find_built(unit) or _build.build_unit(unit)
             lib = _Lib(path, {"xr_attention_mfma": [_p, _p, _p, _p, _p, _i, _i, _p, _i, _p, _p, _i, _p, _p, _p, _i, _p, _p,
                                                     _i, _i, _i, _i, _i, _f, _i, _i, _p, _p, _f, _p, _i, _f, _i, _p],
-                              "xr_attention_few4": [_p] * 6 + [_i, _p, _i, _p, _p, _i, _p, _p] + [_i] * 5 + [_f, _i, _i, _p, _p, _f, _p, _i, _f, _i, _p]})
+                              "xr_attention_few4": [_p] * 6 + [_i, _p, _i, _i, _p, _p, _i, _p, _p] + [_i] * 5 + [_f, _i, _i, _p, _p, _f, _p, _i, _f, _i, _p]})
             self._attn_libs[(D, Dv)] = lib
         return lib
 

@@ -48,6 +48,7 @@ class AttentionPlan:
     n_few: int = 0
     counters: Optional[torch.Tensor] = None    # [row blocks of few rows x key/value heads], zero between launches
     rest: tuple = ()                           # the step's requests that are not among those of few rows
+    merge_rows: int = 0                        # rows of a block of few rows, at most, if blocks have many key ranges (``FEW_MANY``)
 
 
 def first_key(mask, pos: int) -> int:
@@ -81,6 +82,7 @@ FEW_PAGE = 32           # and the smallest page it takes
 FEW_INTS = 12           # numbers of such an item
 FEW_MIN_RANGE = 3       # tiles: its shortest key range
 FEW_FOUR = 3            # (a plan's ``few_rows``) the kernel for few rows over 4-bit pages
+FEW_MANY = 6            # key ranges of a row block that a kernel of its own may add up
 FOUR_ROWS = 400         # rows of a request that it always takes, 16 at a time
 FEW_SLOTS = 256         # workgroups of it that a step's requests are cut into: one a compute unit (twice as many cost more than they gain:
                         # 8 requests of 1,000 to 2,000 keys 15.0 us -> 15.9, 16 of 330 9.4 -> 10.6, 32 of 1,000 to 2,000 with heads of 64 22.6 -> 23.3)
@@ -427,6 +429,7 @@ class StepContext:
             extras = [tuple(x) for x in planned[4]] if extra_slot else []
             flat = [v for it in cta_items + items for v in it] + [v for j in jobs for v in j]
             n_few = n_count = 0
+            merge_rows = 0
             if few:
                 blocks = [(b, row0) for b in few for row0 in range(0, self.q_lens[b] * group_size, FEW_ROWS)]
                 of = [b for b, _ in blocks]
@@ -440,6 +443,7 @@ class StepContext:
                                                             row0s=[r for _, r in blocks] if len(blocks) > len(few) else None, group_size=group_size)
                 n_slots += more
                 n_few, n_count = len(few_items), len(blocks) * n_kv_heads
+                merge_rows = rows if more >= FEW_MANY * len(blocks) else 0
                 extras += few_extras.tolist()
             flat += [v for x in extras for v in x]
             if few:
@@ -453,7 +457,7 @@ class StepContext:
             plan = AttentionPlan(dev[:nw], ni, dev[nw:nx] if nj else None, nj, n_slots, nc,
                                  dev[nx:nf] if extras else None, len(extras),
                                  dev[nf:nf + n_few * FEW_INTS] if n_few else None, n_few, dev[nf + n_few * FEW_INTS:] if n_few else None,
-                                 tuple(b for b in range(len(self.q_lens)) if b not in few))
+                                 tuple(b for b in range(len(self.q_lens)) if b not in few), merge_rows)
             plan._host = host
             self._plans[key] = plan
         return plan

@@ -22,7 +22,7 @@ import numpy as np
 import torch
 
 from ..cache import NULL_PAGE
-from .batch import (ATTN_MIN_RANGE, ATTN_STREAM_SLOTS, ATTN_TILE, FEW_FOUR, FEW_INTS, FEW_MIN_RANGE, FEW_PAGE, FEW_ROWS, FEW_SLOTS, AttentionPlan,
+from .batch import (ATTN_MIN_RANGE, ATTN_STREAM_SLOTS, ATTN_TILE, FEW_FOUR, FEW_INTS, FEW_MANY, FEW_MIN_RANGE, FEW_PAGE, FEW_ROWS, FEW_SLOTS, AttentionPlan,
                     Chunked, StepEntry, few_row_items, few_row_least, four_row_slots, mask_reach)
 
 BUCKETS = (1, 2, 4, 8, 16, 32, 64, 128, 256, 512)
@@ -140,7 +140,7 @@ class StaticDecodeContext:
                 few, counters = d[base:base + n_items], d[base + n_items:base + n_items + n_count]
                 extras = d[base + n_items + n_count:base + n_items + n_count + n_extra] if n_extra else None
                 self._plans[k] = AttentionPlan(few[:0], 0, None, 0, S + (B if n_extra else 0) if S > B * few_blocks(k[0]) or n_extra else 0, 0,
-                                               extras, B if n_extra else 0, few, S, counters)
+                                               extras, B if n_extra else 0, few, S, counters, merge_rows=min(FEW_ROWS, k[0]) if S >= FEW_MANY * B * few_blocks(k[0]) else 0)
                 base += n_items + n_count + n_extra
                 continue
             items = d[base:base + B * S * 8]
