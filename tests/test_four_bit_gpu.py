@@ -564,6 +564,41 @@ def test_a_recorded_call(ops):
         assert torch.isfinite(got[0].float()).all()
 
 
+def test_a_recorded_projection(ops):
+    """A product of 40 decoded tokens, its ranges added up as they are rounded, and attention with ranges added up apart, recorded: as the eager calls give it."""
+    from xyntetik_runner_amd.csrc.ops import FourBitPages
+    H, Hk, D, page, B, K = 16, 1, 128, 32, 40, 1024
+    rng = np.random.default_rng(19)
+    lens = [1, 32, 33, 2000] + [int(n) for n in rng.integers(1, 900, B - 4)]
+    tables, n_pages = scattered(rng, lens, page)
+    ctx = step([n - 1 for n in lens], [1] * B, tables)
+    kp, vp = (FourBitPages.zeros(n_pages, Hk, page, D, values, DEV) for values in (False, True))
+    kp.codes.random_(0, 256)
+    vp.codes.random_(0, 256)
+    kp.scales.fill_(125)
+    vp.scales.fill_(127)
+    w = torch.tensor(rng.normal(size=((H + 2 * Hk) * D, K)) * K ** -0.5, device=DEV).bfloat16()
+    inv = torch.tensor(1e4 ** -(np.arange(D // 2) / (D // 2)), dtype=torch.float32, device=DEV)
+    h = torch.zeros((B, K), dtype=torch.bfloat16, device=DEV)
+
+    def call():
+        q = ops.project_rope_kv_write(h, w, None, kp, vp, ctx.positions, ctx.req_of_token, ctx.block_table(0), inv, H, Hk, D, D, False, 1.0, page, paired=True)
+        return ops.attention(q, kp, vp, ctx, 0, H, Hk, D, page, D ** -0.5), *ops.read_rows(kp, vp, ctx.positions, ctx.req_of_token, ctx.block_table(0), torch.float32)
+
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = call()
+    for i in range(4):
+        h.copy_(torch.tensor(rng.normal(size=h.shape) * (1 + i)))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in outs]
+        for a, b in zip(got, call()):
+            assert torch.isfinite(a.float()).all() and torch.equal(a, b)
+
+
 def test_on_another_stream(ops):
     """Calls on a stream of the caller's, behind its own work."""
     case = ATTEND[0]
