@@ -1517,7 +1517,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES, FEW_PER_CU) void k_attn_few(AttnArg
 // What bounds it: with one row block a request and head memory, 64 requests of 4,000 to 8,000 keys (8 heads of 128, 4 query heads each) take 65.6 us for 424 MB, 6.5
 // TB/s of the 7.05 that a kernel here reaches that only reads (pages read back first: 715); the 64 conversions and 32 exchanges of a tile, 4.65 cycles each, take
 // half of that time beside it.  Blocks of many rows are bound by instructions, 197 a tile of 32 keys (512 rows of 4 heads over 4,000 keys 64 us).  A lone request of 131,072
-// keys takes 31 us (143 MB, 4.5 TB/s): eight tiles a wave, then the sum over 64 ranges.
+// keys takes 31 us (143 MB, 4.5 TB/s): sixteen tiles a wave, then the sum over 64 ranges.
 // Three workgroups a compute unit with a tile on its way while one is multiplied, streaming loads (23 requests of 900 keys, 32 heads: 16 us; two workgroups and two
 // tiles 18; four do not fit the registers of heads of 128; ordinary loads 64 of 8,000 66 us -> 76).  32 rows a block would halve the conversions a row, but leaves two workgroups a unit (8 x 9 tokens of 4 heads over 3,000 keys 17 us -> 28).
 constexpr bool FOUR_OK = HD % 32 == 0 && HV % 32 == 0;
