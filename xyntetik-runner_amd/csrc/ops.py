@@ -522,7 +522,9 @@ class Ops:
     # With 4-bit pages up to here: a product whose ranges stay to be added up is one launch of one tile, which costs more rows more than the other kernel saves
     # (32 + 2 * 8 heads of 128, 8 of 64, 32 of 128, one kernel and two, us: 256 rows 32.8, 37.7; 19.8, 23.5; 49.1, 51.8; 300 37.7, 39.4; 22.7, 25.0; 58.1, 56.4; 450 44.7, 43.4; 26.4, 25.0; 72.6, 68.1).
     FOUR_FINISH_ROWS = 320
-    READ_BACK_BYTES = 2 << 30       # a step's 4-bit pages of a layer are read back whole up to here; beyond, rows are served from the codes, slower but in no memory of their own
+    # Of a step's 4-bit pages of a layer so many bytes are read back at most, or one request's that are more; other requests are served from the codes, slower but in
+    # no memory of their own.  (A runner that takes what the card leaves keeps that much free.)
+    READ_BACK_BYTES = 2 << 30
 
     def _gemm_workspace(self, device):
         """Room for the sums of K ranges when a product with few rows is split (one buffer per process;
@@ -1216,7 +1218,8 @@ class Ops:
         knows = getattr(ctx, "knows_lengths", False)
         if (dtype is torch.bfloat16 and self.use_mfma and D % 32 == 0 and Dv % 32 == 0 and page_size >= 32 and scale > 0.0 and not keep_first
                 and not (softcap and slopes is not None) and getattr(ctx, "plans_few_rows", False) and q.data_ptr() % 16 == 0 and ld_out % 4 == 0 and at % 8 == 0):
-            plan = ctx.attention_plan(group, H // Hk, Chunked(chunk) if chunk else window or None, Hk, page_size, few_rows=3, few_channels=D + Dv)   # (FEW_FOUR)
+            bound = {"read_back": self.READ_BACK_BYTES // (Hk * page_size * (D + Dv) * 2)} if knows else {}
+            plan = ctx.attention_plan(group, H // Hk, Chunked(chunk) if chunk else window or None, Hk, page_size, few_rows=3, few_channels=D + Dv, **bound)   # (FEW_FOUR)
             rest = plan.n_items or plan.n_cta_items
             if not rest or knows:
                 lib = self.attention_lib(D, Dv)

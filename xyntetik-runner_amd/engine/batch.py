@@ -252,6 +252,23 @@ def four_row_requests(starts, q_lens, group_size: int, mask, n_kv_heads: int):
     return list(range(len(rows)))
 
 
+def pages_read(start: int, end: int, page_size: int, mask, keep_first: int = 0):
+    """``(kept, first, last)``: rows at positions ``start`` to ``end - 1`` of a request read its pages 0 to ``kept - 1`` and ``first`` to ``last - 1``."""
+    first = first_key(mask, start) // page_size
+    return (min(-(-keep_first // page_size), first) if mask else 0), first, -(-end // page_size)
+
+
+def read_back_requests(requests, rows, pages, most: int):
+    """Of ``requests``, those whose 4-bit pages are read back: at most ``most`` of them together, or one request alone that has more.  Requests of many
+    ``rows`` first, whose products gain by it what ``pages`` cost."""
+    some, total = [], 0
+    for b in sorted(requests, key=lambda b: -rows[b]):
+        if not some or total + pages[b] <= most:
+            some.append(b)
+            total += pages[b]
+    return sorted(some)
+
+
 def few_row_items(req, starts, lens, q0s, mask, room: int, extra_slot: bool, first_slot: int = 0, pair_at: int = 0, least=None,
                   row0s=None, group_size: int = 1):
     """The work of the kernel for few rows: requests ``req`` of a step, each with one row block (its ``lens[i]`` tokens from row
@@ -411,16 +428,18 @@ class StepContext:
         self.shared = {}        # what parts make once a step and share between layers (a rotation's table)
 
     def attention_plan(self, group: int, group_size: int, window, n_kv_heads: int,
-                       page_size: int = 64, extra_slot: bool = False, few_rows: int = 0, few_channels: int = 256) -> AttentionPlan:
+                       page_size: int = 64, extra_slot: bool = False, few_rows: int = 0, few_channels: int = 256, read_back: int = 1 << 62) -> AttentionPlan:
         """The MFMA attention work list, made once per step and shared by all layers that can.  ``few_rows`` > 0:
         requests of up to 16 rows a key/value head go to the kernel for few rows (where the page size allows), of which a compute unit
-        holds so many workgroups; ``FEW_FOUR``: to the one over 4-bit pages, 16 rows a block (``four_row_requests``); ``few_channels``: those of a key and its
-        value together."""
-        key = (group_size, window, n_kv_heads, page_size, extra_slot, few_rows, few_channels)
+        holds so many workgroups; ``FEW_FOUR``: to the one over 4-bit pages, 16 rows a block (``four_row_requests``), as do requests whose pages would be more
+        than ``read_back`` together (``read_back_requests``); ``few_channels``: those of a key and its value together."""
+        key = (group_size, window, n_kv_heads, page_size, extra_slot, few_rows, few_channels, read_back)
         plan = self._plans.get(key)
         if plan is None:
             if few_rows == FEW_FOUR and page_size >= FEW_PAGE:
                 few = four_row_requests(self.starts, self.q_lens, group_size, window, n_kv_heads)
+                rest = read_back_requests([b for b in range(self.B) if b not in few], self.q_lens, self.pages_read(page_size, window), read_back)
+                few = [b for b in range(self.B) if b not in rest]
             else:
                 few = [b for b, n in enumerate(self.q_lens) if few_rows and page_size >= FEW_PAGE and n * group_size <= FEW_ROWS]
             planned = plan_attention(self.starts, self.q_lens, group_size, window, n_kv_heads, page_size,
@@ -462,6 +481,10 @@ class StepContext:
             self._plans[key] = plan
         return plan
 
+    def pages_read(self, page_size: int, mask, keep_first: int = 0) -> List[int]:
+        """How many pages the rows of each request read, at most (those that were given back are counted, too)."""
+        return [kept + last - first for kept, first, last in (pages_read(s, e, page_size, mask, keep_first) for s, e in zip(self.starts, self.seq_lens))]
+
     def page_list(self, group: int, page_size: int, requests, mask, keep_first: int = 0):
         """The pages that hold what the rows of ``requests`` (None: all) read, numbered from 0: ``(slots [n, 3], table, n)``, a slot's request,
         its place in the request's block table and how many of its positions are the request's; the table as ``block_table`` with these numbers.
@@ -469,10 +492,9 @@ class StepContext:
         slots, table = [], np.full((self.B, self.table_width[group]), -1, dtype=np.int32)
         for b in range(self.B) if requests is None else requests:
             end = self.seq_lens[b]
-            first = first_key(mask, self.starts[b]) // page_size
-            kept = -(-keep_first // page_size) if mask else 0
-            for i in range(-(-end // page_size)):
-                if (i >= first or i < kept) and self._held[group][b, i] >= 0:
+            kept, first, last = pages_read(self.starts[b], end, page_size, mask, keep_first)
+            for i in [*range(kept), *range(first, last)]:
+                if self._held[group][b, i] >= 0:
                     table[b, i] = len(slots)
                     slots.append((b, i, min(page_size, end - i * page_size)))
         n = len(slots)
