@@ -37,3 +37,21 @@ def test_what_is_read_back_beside_the_codes(ops, read, mask, pages, most, what, 
     assert read and max(read) <= most * page_bytes
     if not mask:
         assert max(read) == {0: 10, 16: 15, 26: 22, 27: 27, 1000: 27}[pages] * page_bytes
+
+
+@pytest.mark.parametrize("mask", [50, "chunk"])
+@pytest.mark.parametrize("pages", [40, 1000])
+def test_kept_pages_count_among_what_is_read_back(ops, read, mask, pages, monkeypatch):
+    """A window leaves few pages to read, the first keys that are kept beside it many."""
+    from xyntetik_runner_amd.engine.batch import Chunked
+    H, Hk, D, page = 4, 2, 80, 16
+    page_bytes = Hk * page * 2 * D * 2
+    monkeypatch.setattr(ops, "READ_BACK_BYTES", pages * page_bytes)
+    attend(ops, (H, Hk, D, D, page, Chunked(64) if mask == "chunk" else mask, [900, 700], [40, 1]), "bfloat16", 700, keep=500)
+    assert all(n <= pages * page_bytes for n in read) and bool(read) == (pages == 1000)
+
+
+def test_one_request_of_more_is_read_back(ops, read, monkeypatch):
+    monkeypatch.setattr(ops, "READ_BACK_BYTES", 1000)
+    attend(ops, (4, 2, 80, 80, 16, None, [100], [40]), "bfloat16", 710)
+    assert read and set(read) == {9 * 2 * 16 * 2 * 80 * 2}

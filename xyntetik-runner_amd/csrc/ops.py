@@ -1247,7 +1247,11 @@ class Ops:
         # row and head at a time reads the codes itself (8 requests of 2,000 keys, heads of 72: 1 row 29 us and 769, 64 rows 834 and 15,227).
         cores = (self.attention_on_matrix_cores(dtype, D, Dv, page_size) and not (softcap and slopes is not None) and (D == Dv or not keep_first)
                  and ld_out % 4 == 0 and at % 8 == 0)
-        if knows and self._pages_back(ctx, page_size, window) * Hk * (D + Dv) * q.element_size() <= self.READ_BACK_BYTES and (cores or (dtype is torch.float32 and max(D, Dv) <= 128 and T * H > 3500 * -(-sum(-(-n // 32) for n in ctx.q_lens) * H // 512))):
+        back = knows and (cores or (dtype is torch.float32 and max(D, Dv) <= 128 and T * H > 3500 * -(-sum(-(-n // 32) for n in ctx.q_lens) * H // 512)))
+        if back:
+            counts = ctx.pages_read(page_size, Chunked(chunk) if chunk else window or None, int(keep_first))
+            back = len(counts) == 1 or sum(counts) * Hk * page_size * (D + Dv) * q.element_size() <= self.READ_BACK_BYTES
+        if back:
             k16, v16, table = self.read_pages(k_pages, v_pages, ctx, group, dtype, None, window, chunk, keep_first)
             return self.attention(q, k16, v16, _PagesOf(ctx, table), group, H, Hk, D, page_size, scale, window or None, slopes, chunk or None, keep_first, sinks, Dv,
                                      softcap, gate, out_scale, out)
@@ -1255,11 +1259,6 @@ class Ops:
             at, q.data_ptr(), *pages, positions.data_ptr(), req_of_token.data_ptr(), block_table.data_ptr(), block_table.stride(0), T, H, Hk, D, Dv,
             page_size, float(scale), window, chunk, int(keep_first), dtype_code(dtype), _ptr(slopes), _ptr(sinks), float(softcap), *gating))
         return out
-
-    @staticmethod
-    def _pages_back(ctx, page_size: int, window: int) -> int:
-        """Positions of all pages that a step's rows read, at most."""
-        return sum((-(-(min(s, n + window) if window else s) // page_size) + 1) * page_size for s, n in zip(ctx.seq_lens, ctx.q_lens))
 
     def attention_on_matrix_cores(self, dtype: torch.dtype, D: int, Dv: int, page_size: int = 64) -> bool:
         """Whether keys of ``D`` and values of ``Dv`` channels have matrix-core attention kernels."""
