@@ -55,3 +55,59 @@ def test_one_request_of_more_is_read_back(ops, read, monkeypatch):
     monkeypatch.setattr(ops, "READ_BACK_BYTES", 1000)
     attend(ops, (4, 2, 80, 80, 16, None, [100], [40]), "bfloat16", 710)
     assert read and set(read) == {9 * 2 * 16 * 2 * 80 * 2}
+
+
+def ref_without(q, k, v, start, missing, Hk, scale, window, sinks):
+    """Rows of one request over the keys that exist."""
+    n, H, D = q.shape
+    out = np.zeros((n, H, v.shape[2]))
+    for i in range(n):
+        p = start + i
+        js = [j for j in range(max(0, p - window + 1) if window else 0, p + 1) if j not in missing]
+        for h in range(H):
+            s = k[js, h // (H // Hk)] @ q[i, h] * scale
+            top = max(s.max(initial=-np.inf), sinks[h] if sinks is not None else -np.inf)
+            if top == -np.inf:
+                continue
+            e = np.exp(s - top)
+            out[i, h] = e @ v[js, h // (H // Hk)] / (e.sum() + (np.exp(sinks[h] - top) if sinks is not None else 0.0))
+    return out
+
+
+@pytest.mark.parametrize("bad", [-1, 0, 1 << 30, "past the table"])
+@pytest.mark.parametrize("dt", ["bfloat16", "float32"])
+@pytest.mark.parametrize("path", ["codes", "read back", "recorded"])
+@pytest.mark.parametrize("H,Hk,D,window,q_lens", [(8, 2, 64, None, [1, 1, 1]), (4, 1, 128, None, [9, 5, 3]), (4, 2, 72, 90, [1, 2, 1]), (16, 2, 64, 150, [100, 130, 3]),
+                                                  (4, 2, 80, None, [40, 6, 2])])
+def test_pages_that_do_not_exist_are_left_out(ops, bad, dt, path, H, Hk, D, window, q_lens, monkeypatch):
+    """A page that a row's keys would lie in and that the cache does not have, some of a request's or all: its keys are in no row's sum, whichever kernel runs
+    and whatever page 0 holds (here blocks that read as NaN)."""
+    from xyntetik_runner_amd.engine import batch
+    monkeypatch.setattr(batch, "four_row_requests", lambda starts, *a: [] if path == "read back" else list(range(len(starts))))
+    rng, page, starts = np.random.default_rng(D + H), 32, [200, 150, 60]
+    lens = [s + n for s, n in zip(starts, q_lens)]
+    counts = [-(-n // page) for n in lens]
+    ids = (rng.permutation(sum(counts)) + 1).tolist()
+    full = [[ids.pop() for _ in range(c)] for c in counts]
+    n_pages = sum(counts) + 1
+    ks, vs = ([F.random_sequence(rng, n, Hk, D) for n in lens] for _ in range(2))
+    pages = []
+    for seqs, values in ((ks, False), (vs, True)):
+        codes, scales = F.fill_pages(seqs, full, n_pages, page, values, junk=rng)
+        scales[0] = 255
+        pages.append(on_gpu(codes, scales, D))
+    gone = [{2} if bad != "past the table" else {counts[0] - 1}, set(), set(range(counts[2]))]      # (the first request's table is the longest)
+    none = {0: n_pages, "past the table": -1}.get(bad, bad)
+    tables = [[none if i in g else p for i, p in enumerate(t)] for t, g in zip(full, gone)]
+    if bad == "past the table":
+        tables[0].pop()
+    ctx = step(starts, q_lens, tables)
+    scale, sinks = D ** -0.5, (rng.normal(size=H).astype(np.float32) if window else None)
+    q = [torch.tensor(rng.normal(size=(n, H, D)) * 1.5).to(DT[dt]) for n in q_lens]
+    got = ops.attention(torch.cat(q).reshape(-1, H * D).contiguous().to(DEV), *pages, Recorded(ctx) if path == "recorded" else ctx, 0, H, Hk, D, page, scale, window,
+                        sinks=torch.tensor(sinks, device=DEV) if window else None).cpu().double().numpy().reshape(-1, H, D)
+    want = np.concatenate([ref_without(q[b].double().numpy(), ks[b][2], vs[b][2], starts[b], {j for i in gone[b] for j in range(page * i, page * i + page)}, Hk, scale, window, sinks)
+                           for b in range(3)])
+    assert np.isfinite(got).all() and not got[q_lens[0] + q_lens[1]:].any()
+    # (bounds as in the tests of attention over pages that exist: two roundings to bfloat16, or sums in 32 bits)
+    assert np.abs(got - want).max() <= (1.2e-2 if dt == "bfloat16" else 2e-5) * np.abs(want).max()

@@ -1512,7 +1512,8 @@ __global__ __launch_bounds__(64 * FEW_WAVES, FEW_PER_CU) void k_attn_few(AttnArg
 // Values: operands want two positions side by side in a word, codes have two channels, and a scale belongs to a position.  A lane holds 8 positions of HV / 16
 // neighbouring channels; a pair of channels is converted position by position and two positions' words change halves (32 conversions and 32 exchanges of
 // halves for 32 keys x 128 channels).  Row m of output block d so stands for channel m * HV / 16 + d.
-// Scales past a request's end are taken as zeros' and codes there are any numbers: no operand has to be masked.
+// Scales past a request's end are taken as zeros' and codes there are any numbers: no operand has to be masked.  A page that does not exist (past the table, given
+// back, past the pool) is read as page 0 with such scales, and its keys are hidden.
 //
 // What bounds it: with one row block a request and head memory, 64 requests of 4,000 to 8,000 keys (8 heads of 128, 4 query heads each) take 65.6 us for 424 MB, 6.5
 // TB/s of the 7.05 that a kernel here reaches that only reads (pages read back first: 715); the 64 conversions and 32 exchanges of a tile, 4.65 cycles each, take
@@ -1599,9 +1600,10 @@ __global__ __launch_bounds__(64 * FEW_WAVES, FOUR_PER_CU) void k_attn_few4(AttnA
 
     int pages_base = kbeg >> a.page_shift;
     int my_page;
+    const int n_listed = min(((seq_len - 1) >> a.page_shift) + 1, a.table_stride);
     auto look_up = [&]() {
         const int pi = pages_base + lane;
-        const bool in = ((long)pi << a.page_shift) < seq_len;
+        const bool in = pi < n_listed;
         my_page = bt[in ? pi : 0];
         my_page = in && (unsigned)my_page < (unsigned)a.n_pages ? my_page : -1;
     };
@@ -1688,13 +1690,14 @@ __global__ __launch_bounds__(64 * FEW_WAVES, FOUR_PER_CU) void k_attn_few4(AttnA
 #pragma unroll
             for (int e = 0; e < 4; ++e) s[4 * b + e] = MODE == MODE_CAP ? cap.less(z[e], 0.f) : z[e];
         }
-        const bool whole = kt + 32 <= kend && kt + 31 <= pos_min && kt >= lo_max;
+        const int last = x.pg < 0 ? kt : kend;                   // (of a page that does not exist no key is seen)
+        const bool whole = kt + 32 <= last && kt + 31 <= pos_min && kt >= lo_max;
         if (!whole) {
             asm volatile("; hidden keys");      // (stays a branch: whole tiles, nearly all, skip the selection's 40 instructions)
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 const int key = kt + 8 * quad + e;
-                const bool ok = row_ok && key <= pos && key >= lo && key < kend;
+                const bool ok = row_ok && key <= pos && key >= lo && key < last;
                 s[e] = ok ? s[e] : -INFINITY;
             }
         }

@@ -917,7 +917,7 @@ class Ops:
         order, and the block table that names them: ``(k [n, heads, page_size, dim], v [n, heads, dim, page_size], table)``.  Positions behind a request's end
         are zeros.  ``requests``: the places in the step of those that are read (None: all); with a ``window`` or ``chunk`` the
         pages that none of the step's rows reads are left out (``keep_first``: except those of the first so many positions), as are
-        pages that were given back: -1 in the table.  A step that is being recorded has no lengths to go by and is refused."""
+        pages that were given back: -1 in the table; a number past the pool's reads as zeros.  A step that is being recorded has no lengths to go by and is refused."""
         pages = self._pages4("read_pages", k_pages, v_pages)
         if not getattr(ctx, "knows_lengths", False):
             raise KernelError("read_pages: the lengths of a recorded step's requests change from replay to replay")
@@ -1111,7 +1111,8 @@ class Ops:
         Caches that are ``FourBitPages``: requests of up to some hundred rows a key/value head are read from the codes by a matrix-core kernel of
         their own (bfloat16, sizes in whole blocks of 32, pages of at least 32 positions, no kept first keys).  The pages of others are read
         back first (``read_pages``) where matrix cores then have enough rows; what is left, and what a step that is being recorded cannot read back,
-        a 32-bit kernel serves from the codes.  Calls that share a step's context follow one another (they share its counters): on one stream, or
+        a 32-bit kernel serves from the codes.  Keys in pages that do not exist (given back, past the table or the pool) are in no row's sum, and a row
+        without keys and sink comes back as zeros.  Calls that share a step's context follow one another (they share its counters): on one stream, or
         behind an event.
         """
         if isinstance(k_cache, FourBitPages) or isinstance(v_cache, FourBitPages):
@@ -1216,10 +1217,16 @@ class Ops:
         window, chunk, ld_out, at = int(window or 0), int(chunk or 0), out.stride(0), out.data_ptr()
         gating = (_ptr(gate), gate.stride(0) if gate is not None else 0, float(out_scale), ld_out, _stream())
         knows = getattr(ctx, "knows_lengths", False)
+        mask = Chunked(chunk) if chunk else window or None
         if (dtype is torch.bfloat16 and self.use_mfma and D % 32 == 0 and Dv % 32 == 0 and page_size >= 32 and scale > 0.0 and not keep_first
                 and not (softcap and slopes is not None) and getattr(ctx, "plans_few_rows", False) and q.data_ptr() % 16 == 0 and ld_out % 4 == 0 and at % 8 == 0):
             bound = {"read_back": self.READ_BACK_BYTES // (Hk * page_size * (D + Dv) * 2)} if knows else {}
-            plan = ctx.attention_plan(group, H // Hk, Chunked(chunk) if chunk else window or None, Hk, page_size, few_rows=3, few_channels=D + Dv, **bound)   # (FEW_FOUR)
+            plan = ctx.attention_plan(group, H // Hk, mask, Hk, page_size, few_rows=3, few_channels=D + Dv, **bound)   # (FEW_FOUR)
+            if knows and plan.rest:
+                # (keys of pages that do not exist are left out where codes are read; pages read back would hold zeros in their place)
+                bad = ctx.without_pages(group, page_size, k_pages.num_pages, mask)
+                if bad:
+                    plan = ctx.attention_plan(group, H // Hk, mask, Hk, page_size, few_rows=3, few_channels=D + Dv, from_codes=bad, **bound)
             rest = plan.n_items or plan.n_cta_items
             if not rest or knows:
                 lib = self.attention_lib(D, Dv)
@@ -1249,8 +1256,9 @@ class Ops:
                  and ld_out % 4 == 0 and at % 8 == 0)
         back = knows and (cores or (dtype is torch.float32 and max(D, Dv) <= 128 and T * H > 3500 * -(-sum(-(-n // 32) for n in ctx.q_lens) * H // 512)))
         if back:
-            counts = ctx.pages_read(page_size, Chunked(chunk) if chunk else window or None, int(keep_first))
-            back = len(counts) == 1 or sum(counts) * Hk * page_size * (D + Dv) * q.element_size() <= self.READ_BACK_BYTES
+            counts = ctx.pages_read(page_size, mask, int(keep_first))
+            back = ((len(counts) == 1 or sum(counts) * Hk * page_size * (D + Dv) * q.element_size() <= self.READ_BACK_BYTES)
+                    and not ctx.without_pages(group, page_size, k_pages.num_pages, mask, int(keep_first)))
         if back:
             k16, v16, table = self.read_pages(k_pages, v_pages, ctx, group, dtype, None, window, chunk, keep_first)
             return self.attention(q, k16, v16, _PagesOf(ctx, table), group, H, Hk, D, page_size, scale, window or None, slopes, chunk or None, keep_first, sinks, Dv,

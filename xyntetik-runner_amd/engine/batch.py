@@ -428,17 +428,18 @@ class StepContext:
         self.shared = {}        # what parts make once a step and share between layers (a rotation's table)
 
     def attention_plan(self, group: int, group_size: int, window, n_kv_heads: int,
-                       page_size: int = 64, extra_slot: bool = False, few_rows: int = 0, few_channels: int = 256, read_back: int = 1 << 62) -> AttentionPlan:
+                       page_size: int = 64, extra_slot: bool = False, few_rows: int = 0, few_channels: int = 256, read_back: int = 1 << 62,
+                       from_codes: frozenset = frozenset()) -> AttentionPlan:
         """The MFMA attention work list, made once per step and shared by all layers that can.  ``few_rows`` > 0:
         requests of up to 16 rows a key/value head go to the kernel for few rows (where the page size allows), of which a compute unit
         holds so many workgroups; ``FEW_FOUR``: to the one over 4-bit pages, 16 rows a block (``four_row_requests``), as do requests whose pages would be more
-        than ``read_back`` together (``read_back_requests``); ``few_channels``: those of a key and its value together."""
-        key = (group_size, window, n_kv_heads, page_size, extra_slot, few_rows, few_channels, read_back)
+        than ``read_back`` together (``read_back_requests``) and those of ``from_codes``; ``few_channels``: those of a key and its value together."""
+        key = (group_size, window, n_kv_heads, page_size, extra_slot, few_rows, few_channels, read_back, from_codes)
         plan = self._plans.get(key)
         if plan is None:
             if few_rows == FEW_FOUR and page_size >= FEW_PAGE:
                 few = four_row_requests(self.starts, self.q_lens, group_size, window, n_kv_heads)
-                rest = read_back_requests([b for b in range(self.B) if b not in few], self.q_lens, self.pages_read(page_size, window), read_back)
+                rest = read_back_requests([b for b in range(self.B) if b not in few and b not in from_codes], self.q_lens, self.pages_read(page_size, window), read_back)
                 few = [b for b in range(self.B) if b not in rest]
             else:
                 few = [b for b, n in enumerate(self.q_lens) if few_rows and page_size >= FEW_PAGE and n * group_size <= FEW_ROWS]
@@ -484,6 +485,20 @@ class StepContext:
     def pages_read(self, page_size: int, mask, keep_first: int = 0) -> List[int]:
         """How many pages the rows of each request read, at most (those that were given back are counted, too)."""
         return [kept + last - first for kept, first, last in (pages_read(s, e, page_size, mask, keep_first) for s, e in zip(self.starts, self.seq_lens))]
+
+    def without_pages(self, group: int, page_size: int, n_pages: int, mask, keep_first: int = 0) -> frozenset:
+        """The requests whose rows read a page that a pool of ``n_pages`` does not have: given back, past the table or past the pool's end."""
+        key = ("without_pages", group, page_size, n_pages, mask, keep_first if mask else 0)
+        found = self.shared.get(key)
+        if found is None:
+            some = []
+            for b, held in enumerate(self._held[group]):
+                kept, first, last = pages_read(self.starts[b], self.seq_lens[b], page_size, mask, keep_first)
+                ids = np.concatenate([held[:kept], held[first:last]])
+                if len(ids) < kept + last - first or ids.min() < 0 or ids.max() >= n_pages:
+                    some.append(b)
+            found = self.shared[key] = frozenset(some)
+        return found
 
     def page_list(self, group: int, page_size: int, requests, mask, keep_first: int = 0):
         """The pages that hold what the rows of ``requests`` (None: all) read, numbered from 0: ``(slots [n, 3], table, n)``, a slot's request,
