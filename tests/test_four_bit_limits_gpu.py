@@ -111,3 +111,38 @@ def test_pages_that_do_not_exist_are_left_out(ops, bad, dt, path, H, Hk, D, wind
     assert np.isfinite(got).all() and not got[q_lens[0] + q_lens[1]:].any()
     # (bounds as in the tests of attention over pages that exist: two roundings to bfloat16, or sums in 32 bits)
     assert np.abs(got - want).max() <= (1.2e-2 if dt == "bfloat16" else 2e-5) * np.abs(want).max()
+
+
+@pytest.mark.parametrize("columns", ["fewer than the rows are apart", "shared by all requests"])
+def test_block_tables_that_are_views(ops, columns):
+    """A table of some columns of a wider one, or of one row that all requests read: a position past its columns has no page."""
+    from xyntetik_runner_amd.csrc.ops import FourBitPages
+    rng, page, Hk, D, B = np.random.default_rng(4), 16, 2, 32, 3
+    wide = torch.arange(1, 13, dtype=torch.int32, device=DEV).view(B, 4)
+    table = wide[:, :2] if columns.startswith("fewer") else wide[:1, :2].expand(B, 2)
+    assert not table.is_contiguous()
+    pos = [0, 15, 16, 31, 32, 33, 47, 48, 5, 21, 40, 63, 64, 2, 30, 35, 3, 36, 37, 38]
+    req = [0] * 8 + [1] * 5 + [2] * 7
+    p, r = (torch.tensor(x, dtype=torch.int32, device=DEV) for x in (pos, req))
+    x = torch.tensor(rng.normal(size=(len(pos), 2 * D)), dtype=torch.float32, device=DEV)
+    h = torch.tensor(rng.normal(size=(len(pos), 64)), device=DEV).bfloat16()
+    w = torch.tensor(rng.normal(size=(6 * D, 64)), device=DEV).bfloat16()
+    rows = []
+    for t in (table, table.contiguous()):
+        for fused in (False, True):
+            kp, vp = (FourBitPages.zeros(14, Hk, page, D, values, DEV) for values in (False, True))
+            if fused:                    # 20 rows: the kernel that adds the product's ranges up writes
+                ops.project_rope_kv_write(h, w, None, kp, vp, p, r, t, None, 2, Hk, D, 0, False, 1.0, page)
+            else:
+                ops.rope_kv_write(None, x, x, None, kp, vp, p, r, t, None, 0, Hk, D, 0, False, 1.0, page)
+            mine = torch.unique(table).tolist()
+            assert all(not pages.scales[i].any() for pages in (kp, vp) for i in range(14) if i not in mine)
+            k, v = ops.read_rows(kp, vp, p, r, t, torch.float32)
+            for got in (k, v):
+                there = torch.tensor([q < 2 * page for q in pos], device=DEV)
+                assert got[there].abs().amax(1).min() > 0 and not got[~there].any()
+            kp.scales.fill_(127)
+            kp.codes.fill_(0x22)
+            rows += [k, v, *ops.read_rows(kp, vp, p, r, t, torch.float32)]
+    for a, b in zip(rows[:8], rows[8:]):
+        assert torch.equal(a, b)

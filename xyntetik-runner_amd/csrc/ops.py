@@ -120,8 +120,8 @@ _PROTOS = {
     "xr_qkv_store": [_p, _p, _p, _p, _p, _p, _i, _p, _p, _p, _i, _i, _i, _i, _i, _i, _i, _i, _p],
     "xr_pool_blocks": [_p, _p, _p, _p, _p, _p, _p, _i, _p, _i, _i, _i, _i, _i, _i, _i, _i, _i, _p],
     "xr_attention_pool_partial": [_p, _p, _p, _p, _p, _p, _i, _p, _i, _i, _i, _i, _i, _i, _f, _i, _i, _i, _p],
-    "xr_rope_kv_write4": [_p, _p, _p, _i, _p] + [_p] * 4 + [_i] + [_p] * 3 + [_i, _i, _p] + [_i] * 7 + [_f, _i, _i, _i, _p],
-    "xr_read_rows4": [_p, _p] + [_p] * 4 + [_i] + [_p] * 3 + [_i] * 8 + [_p],
+    "xr_rope_kv_write4": [_p, _p, _p, _i, _p] + [_p] * 4 + [_i] + [_p] * 3 + [_i, _i, _i, _p] + [_i] * 7 + [_f, _i, _i, _i, _p],
+    "xr_read_rows4": [_p, _p] + [_p] * 4 + [_i] + [_p] * 3 + [_i] * 9 + [_p],
     "xr_read_pages4": [_p, _p] + [_p] * 4 + [_i, _p, _i, _p] + [_i] * 6 + [_p],
     "xr_attention_any4": [_p, _p] + [_p] * 4 + [_i] + [_p] * 3 + [_i] * 7 + [_f] + [_i] * 4 + [_p, _p, _f, _p, _i, _f, _i, _p],
     "xr_attention_pooled": [_p, _p, _p, _p, _p, _p, _p, _p, _p, _i, _p, _i, _i, _i, _i, _i, _i, _i, _f, _i, _i, _i, _p],
@@ -345,7 +345,7 @@ class _GemmRope(C.Structure):
 
 class _GemmPages4(C.Structure):
     """XrGemmPages4 of the library."""
-    _fields_ = [("kc", _p), ("ks", _p), ("vc", _p), ("vs", _p), ("n_pages", _i), ("n_requests", _i)]
+    _fields_ = [("kc", _p), ("ks", _p), ("vc", _p), ("vs", _p), ("n_pages", _i), ("n_requests", _i), ("table_width", _i)]
 
 
 def paired_order(D: int, rot: int) -> list:
@@ -891,7 +891,7 @@ class Ops:
             raise KernelError(f"rope_kv_write: {rot // 2} 32-bit frequencies are needed")
         self.lib.check(self.lib.xr_rope_kv_write4(
             _ptr(q_in), k_in.data_ptr(), v_in.data_ptr(), stride, _ptr(q_out), *pages, positions.data_ptr(), req_of_token.data_ptr(),
-            block_table.data_ptr(), block_table.stride(0), block_table.shape[0], _ptr(inv_freq) if rot else None, T, H, Hk, D, Dv, rot, 1 if interleaved else 0,
+            block_table.data_ptr(), block_table.stride(0), block_table.shape[1], block_table.shape[0], _ptr(inv_freq) if rot else None, T, H, Hk, D, Dv, rot, 1 if interleaved else 0,
             float(mscale), page_size, dtype_code(q_out.dtype) if q_out is not None else XR_F32, 1 if paired else 0, _stream()))
 
     def read_rows(self, k_pages: "FourBitPages", v_pages: "FourBitPages", positions: torch.Tensor, req_of_row: torch.Tensor,
@@ -907,7 +907,7 @@ class Ops:
         k = torch.empty((n, Hk * D), dtype=dtype, device=k_pages.device)
         v = torch.empty((n, Hk * Dv), dtype=dtype, device=k_pages.device)
         self.lib.check(self.lib.xr_read_rows4(k.data_ptr(), v.data_ptr(), *pages, positions.data_ptr(), req_of_row.data_ptr(),
-                                              block_table.data_ptr(), block_table.stride(0), block_table.shape[0], n, Hk, D, Dv, k_pages.page_size, dtype_code(dtype),
+                                              block_table.data_ptr(), block_table.stride(0), block_table.shape[1], block_table.shape[0], n, Hk, D, Dv, k_pages.page_size, dtype_code(dtype),
                                               _stream()))
         return k, v
 
@@ -1052,12 +1052,12 @@ class Ops:
             pages = None
             if four:
                 self._here("projection", rows, wt, bias, k_cache, v_cache, positions, req_of_token, block_table, inv_freq)
-                pages = _GemmPages4(*self._pages4("projection", k_cache, v_cache, Hk, D, page_size), 0)
+                pages = _GemmPages4(*self._pages4("projection", k_cache, v_cache, Hk, D, page_size), 0, 0)
                 if v_cache.dim != D or (rot and (inv_freq is None or inv_freq.dtype != torch.float32 or inv_freq.numel() != rot // 2 or not inv_freq.is_contiguous())):
                     raise KernelError(f"projection: values of {D} channels and {rot // 2} 32-bit frequencies are needed")
                 self._ints("projection", T, positions, req_of_token)
                 self._table("projection", block_table)
-                pages.n_requests = block_table.shape[0]
+                pages.n_requests, pages.table_width = block_table.shape
             else:
                 self._dev(rows, wt, bias, k_cache, v_cache, positions, req_of_token, block_table, inv_freq)
             self._contig(wt, "projection weight")

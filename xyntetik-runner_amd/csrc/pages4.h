@@ -33,7 +33,7 @@ struct Pages4 {
 // what a product's caller passes beside its rotation to have keys and values go to 4-bit pages
 struct XrGemmPages4 {
     void *kc, *ks, *vc, *vs;
-    int n_pages, n_requests;
+    int n_pages, n_requests, table_width;
 };
 
 struct Write4Sums {
@@ -44,7 +44,7 @@ struct Write4Sums {
     const int* positions;
     const int* req_of_token;
     const int* block_table;
-    int table_stride;
+    int table_stride;       // (from a request's row to the next's: a table may be a view of a wider one)
     const float* inv_freq;
     void* q_out;            // [T, H * D] bfloat16
     int T, H, Hk, D, rot, interleaved;     // (pairs that are not neighbours: in paired order)

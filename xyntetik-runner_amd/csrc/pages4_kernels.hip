@@ -23,8 +23,8 @@ struct Write4Args {
     Pages4 pages;
     const int* positions;   // [T]
     const int* req_of_token;
-    const int* block_table; // [B, table_stride]
-    int table_stride, n_requests, n_pages;
+    const int* block_table; // [n_requests, table_width], rows table_stride apart
+    int table_stride, table_width, n_requests, n_pages;
     const float* inv_freq;  // [rot / 2] or null
     int H, Hk, D, Dv, rot, interleaved, paired;
     float mscale;
@@ -137,7 +137,7 @@ __global__ __launch_bounds__(256) void k_rope_kv_write4(Write4Args a) {
         cs[j & 7][j >> 3] = make_float2(c * a.mscale, s * a.mscale);
     }
     const int bi = pos >> a.page_shift, off = pos & a.page_mask;
-    const int page = bi >= 0 && bi < a.table_stride && (unsigned)req < (unsigned)a.n_requests ? a.block_table[(size_t)req * a.table_stride + bi] : -1;
+    const int page = bi >= 0 && bi < a.table_width && (unsigned)req < (unsigned)a.n_requests ? a.block_table[(size_t)req * a.table_stride + bi] : -1;
     const bool there = (unsigned)page < (unsigned)a.n_pages;          // (what has no page is written nowhere)
     // the 8 positions of a page that this one belongs to: whole in this step, row by row?
     const int lead = t - (pos & 7);
@@ -294,7 +294,7 @@ int rope_kv_write4_sums(const Write4Sums& w, hipStream_t stream) {
     a.q_in = w.sums; a.k_in = w.sums + (size_t)w.H * w.D; a.v_in = a.k_in + (size_t)w.Hk * w.D; a.q_out = w.q_out;
     a.bias = w.bias; a.range_step = (size_t)w.T * a.in_stride; a.ranges = w.ranges;
     a.positions = w.positions; a.req_of_token = w.req_of_token; a.block_table = w.block_table; a.table_stride = w.table_stride;
-    a.n_requests = p.n_requests; a.n_pages = p.n_pages; a.inv_freq = w.inv_freq; a.H = w.H; a.Hk = w.Hk; a.D = a.Dv = w.D; a.rot = w.rot;
+    a.table_width = p.table_width; a.n_requests = p.n_requests; a.n_pages = p.n_pages; a.inv_freq = w.inv_freq; a.H = w.H; a.Hk = w.Hk; a.D = a.Dv = w.D; a.rot = w.rot;
     a.interleaved = w.interleaved; a.paired = !w.interleaved && w.rot > 0; a.mscale = w.mscale;
     a.page_shift = ilog2_exact(w.page_size); a.page_mask = w.page_size - 1; a.page_size = w.page_size;
     const dim3 grid = deal_units(a, w.T);
@@ -305,14 +305,14 @@ int rope_kv_write4_sums(const Write4Sums& w, hipStream_t stream) {
 
 extern "C" int xr_rope_kv_write4(const float* q_in, const float* k_in, const float* v_in, int in_stride, void* q_out,
                                  void* kc, void* ks, void* vc, void* vs, int n_pages, const int* positions, const int* req_of_token,
-                                 const int* block_table, int table_stride, int n_requests, const float* inv_freq, int T, int H, int Hk,
+                                 const int* block_table, int table_stride, int table_width, int n_requests, const float* inv_freq, int T, int H, int Hk,
                                  int D, int Dv, int rot, int interleaved, float mscale, int page_size, int q_dtype, int paired,
                                  hipStream_t stream) {
     Write4Args a;
     a.pages = Pages4{(uint8_t*)kc, (uint8_t*)ks, (uint8_t*)vc, (uint8_t*)vs};
     const int rc = check_pages4("rope_kv_write", a.pages, Hk, D, Dv, page_size, n_pages);
     if (rc != XR_OK) return rc;
-    XR_REQUIRE(T >= 0 && H >= 0 && H < (1 << 20) && Hk < (1 << 20) && table_stride > 0, "rope_kv_write: bad sizes T=%d H=%d, block tables of %d pages", T, H, table_stride);
+    XR_REQUIRE(T >= 0 && H >= 0 && H < (1 << 20) && Hk < (1 << 20) && table_stride >= 0 && table_width > 0, "rope_kv_write: bad sizes T=%d H=%d, block tables of %d pages", T, H, table_width);
     XR_REQUIRE(rot >= 0 && rot <= D && rot % 2 == 0, "rope_kv_write: rotary width %d must be even and at most head_dim %d", rot, D);
     XR_REQUIRE(rot == 0 || inv_freq, "rope_kv_write: rotary width %d without a frequency table", rot);
     XR_REQUIRE(q_dtype == XR_F32 || q_dtype == XR_BF16, "rope_kv_write: bad dtype %d", q_dtype);
@@ -321,7 +321,7 @@ extern "C" int xr_rope_kv_write4(const float* q_in, const float* k_in, const flo
     XR_REQUIRE(k_in && v_in && block_table && req_of_token && positions, "rope_kv_write: keys and values to cache but a null operand");
     XR_REQUIRE(H == 0 || (q_in && q_out && ((uintptr_t)q_out & 15) == 0), "rope_kv_write: queries but a null operand, or rows that are not 16-byte aligned");
     a.q_in = q_in; a.k_in = k_in; a.v_in = v_in; a.in_stride = in_stride; a.q_out = q_out; a.bias = nullptr; a.range_step = 0; a.ranges = 1;
-    a.positions = positions; a.req_of_token = req_of_token; a.block_table = block_table; a.table_stride = table_stride; a.n_requests = n_requests; a.n_pages = n_pages;
+    a.positions = positions; a.req_of_token = req_of_token; a.block_table = block_table; a.table_stride = table_stride; a.table_width = table_width; a.n_requests = n_requests; a.n_pages = n_pages;
     a.inv_freq = inv_freq; a.H = H; a.Hk = Hk; a.D = D; a.Dv = Dv; a.rot = rot; a.interleaved = interleaved; a.paired = paired ? 1 : 0;
     a.mscale = mscale; a.page_shift = ilog2_exact(page_size); a.page_mask = page_size - 1; a.page_size = page_size;
     const dim3 grid = deal_units(a, T);
@@ -362,7 +362,7 @@ struct Read4Args {
     const int* slots;           // pages: [n, 3] request, place in its table, positions of the page that are the request's
     void* k_out;                // rows: [n, Hk * D]; pages: [n, Hk, page_size, D]
     void* v_out;                // rows: [n, Hk * Dv]; pages: [n, Hk, Dv, page_size]
-    int table_stride, n_requests, n_pages, Hk, D, Dv, page_shift, page_size;
+    int table_stride, table_width, n_requests, n_pages, Hk, D, Dv, page_shift, page_size;
     size_t total;               // threads of all rows, keys' first
     size_t k_total;
 };
@@ -379,7 +379,7 @@ __global__ __launch_bounds__(256) void k_read_rows4(Read4Args a) {
         const int w = (int)(j - r * per), h = w / (D >> 3), c0 = (w - h * (D >> 3)) * 8;
         const int pos = a.positions[r], bi = pos >> a.page_shift, off = pos & (a.page_size - 1);
         const int req = a.req_of_row[r];
-        const int page = bi >= 0 && bi < a.table_stride && (unsigned)req < (unsigned)a.n_requests ? a.block_table[(size_t)req * a.table_stride + bi] : -1;
+        const int page = bi >= 0 && bi < a.table_width && (unsigned)req < (unsigned)a.n_requests ? a.block_table[(size_t)req * a.table_stride + bi] : -1;
         float x[8];
         if ((unsigned)page >= (unsigned)a.n_pages) {
 #pragma unroll
@@ -435,18 +435,18 @@ __global__ __launch_bounds__(256) void k_read_pages4(Read4Args a) {
 }
 
 extern "C" int xr_read_rows4(void* k_out, void* v_out, void* kc, void* ks, void* vc, void* vs, int n_pages, const int* positions,
-                             const int* req_of_row, const int* block_table, int table_stride, int n_requests, int n, int Hk, int D,
+                             const int* req_of_row, const int* block_table, int table_stride, int table_width, int n_requests, int n, int Hk, int D,
                              int Dv, int page_size, int dtype, hipStream_t stream) {
     Read4Args a;
     a.pages = Pages4{(uint8_t*)kc, (uint8_t*)ks, (uint8_t*)vc, (uint8_t*)vs};
     const int rc = check_pages4("read_rows", a.pages, Hk, D, Dv, page_size, n_pages);
     if (rc != XR_OK) return rc;
-    XR_REQUIRE(n >= 0 && table_stride > 0 && (dtype == XR_F32 || dtype == XR_BF16), "read_rows: bad sizes n=%d table=%d or dtype %d", n, table_stride, dtype);
+    XR_REQUIRE(n >= 0 && table_stride >= 0 && table_width > 0 && (dtype == XR_F32 || dtype == XR_BF16), "read_rows: bad sizes n=%d table=%d or dtype %d", n, table_width, dtype);
     if (n == 0) return XR_OK;
     XR_REQUIRE(k_out && v_out && positions && req_of_row && block_table, "read_rows: a null operand");
     XR_REQUIRE((((uintptr_t)k_out | (uintptr_t)v_out) & 15) == 0, "read_rows: outputs must be 16-byte aligned");
     a.positions = positions; a.req_of_row = req_of_row; a.block_table = block_table; a.slots = nullptr;
-    a.k_out = k_out; a.v_out = v_out; a.table_stride = table_stride; a.n_requests = n_requests; a.n_pages = n_pages; a.Hk = Hk; a.D = D; a.Dv = Dv;
+    a.k_out = k_out; a.v_out = v_out; a.table_stride = table_stride; a.table_width = table_width; a.n_requests = n_requests; a.n_pages = n_pages; a.Hk = Hk; a.D = D; a.Dv = Dv;
     a.page_shift = ilog2_exact(page_size); a.page_size = page_size;
     a.k_total = (size_t)n * Hk * (D >> 3);
     a.total = a.k_total + (size_t)n * Hk * (Dv >> 3);
@@ -470,7 +470,7 @@ extern "C" int xr_read_pages4(void* k_out, void* v_out, void* kc, void* ks, void
     XR_REQUIRE(k_out && v_out && slots && block_table, "read_pages: a null operand");
     XR_REQUIRE((((uintptr_t)k_out | (uintptr_t)v_out) & 15) == 0, "read_pages: outputs must be 16-byte aligned");
     a.positions = nullptr; a.req_of_row = nullptr; a.block_table = block_table; a.slots = slots;
-    a.k_out = k_out; a.v_out = v_out; a.table_stride = table_stride; a.n_requests = 0; a.n_pages = n_pages; a.Hk = Hk; a.D = D; a.Dv = Dv;
+    a.k_out = k_out; a.v_out = v_out; a.table_stride = table_stride; a.table_width = a.n_requests = 0; a.n_pages = n_pages; a.Hk = Hk; a.D = D; a.Dv = Dv;
     a.page_shift = ilog2_exact(page_size); a.page_size = page_size; a.total = a.k_total = 0;
     const unsigned grid = (unsigned)n * (unsigned)Hk;
     if (dtype == XR_F32) k_read_pages4<float><<<grid, 256, 0, stream>>>(a);
