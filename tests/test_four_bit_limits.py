@@ -46,3 +46,18 @@ def test_a_step_of_deep_portions_reads_back_no_more_than_the_bound(monkeypatch):
     items = plan.few.view(-1, batch.FEW_INTS)
     assert set(items[:, 0].tolist()) == set(range(20)) - set(plan.rest)
     assert ctx.attention_plan(0, group, None, heads, page, few_rows=batch.FEW_FOUR, few_channels=channels).rest == tuple(range(20))
+
+
+@pytest.mark.parametrize("requests", [(-1,), (0, 3), (2, -3), (1 << 40,)])
+def test_requests_that_a_step_does_not_have(requests, monkeypatch):
+    """(A place below 0 is one of Python's from the end, and would have been a row before the block table's first on the GPU.)"""
+    from xyntetik_runner_amd.csrc.ops import FourBitPages, KernelError, Ops
+    ctx = plain_step(monkeypatch, [20, 3, 40], [1, 1, 1], [[1, 2], [3], [4, 5, 6]])
+    ops = Ops.__new__(Ops)
+    made = []
+    monkeypatch.setattr(ctx, "page_list", lambda *a: made.append(a))
+    monkeypatch.setattr(Ops, "_here", staticmethod(lambda *a: None))
+    pages = [FourBitPages.zeros(8, 1, 16, 32, values, "cpu") for values in (False, True)]
+    with pytest.raises(KernelError, match="requests"):
+        ops.read_pages(*pages, ctx, 0, torch.bfloat16, requests=requests)
+    assert not made

@@ -923,13 +923,16 @@ class Ops:
             raise KernelError("read_pages: the lengths of a recorded step's requests change from replay to replay")
         if window and chunk:
             raise KernelError("read_pages: a layer reads a window or its chunk, not both")
+        requests = None if requests is None else tuple(requests)
+        if requests and not all(0 <= b < ctx.B for b in requests):
+            raise KernelError(f"read_pages: requests {requests} of a step of {ctx.B}")
         dtype_code(dtype)
         block_table = ctx.block_table(group)
         self._here("read_pages", k_pages, block_table)
         self._table("read_pages", block_table)
         Hk, D, Dv, P = k_pages.heads, k_pages.dim, v_pages.dim, k_pages.page_size
         mask = Chunked(int(chunk)) if chunk else window or None
-        key = ("read_pages", group, P, None if requests is None else tuple(requests), mask, keep_first if mask else 0)
+        key = ("read_pages", group, P, requests, mask, keep_first if mask else 0)
         made = ctx.shared.get(key)
         if made is None:
             made = ctx.shared[key] = ctx.page_list(group, P, requests, mask, keep_first)
