@@ -611,8 +611,8 @@ def main():
                 checks[f"{name}_row0_vs_alone"] = chk
                 log(f"{name}: the first request's logits against the same request alone: {chk}")
                 bound = 5e-3 * (max(layers, 2) / 32.0) ** 0.5
-                # (over a cache in 4 bits a key whose rounding falls the other way moves by a whole step: reported only)
-                if args.dtype == "bfloat16" and args.cache_dtype == "auto" and not (chk["mean"] <= bound and chk["max"] <= 10 * bound):
+                # (Over a cache in 4 bits a key whose rounding falls the other way moves by a whole step, but one of 2,048: 3.0e-3, 1.6e-2.)
+                if args.dtype == "bfloat16" and not (chk["mean"] <= bound and chk["max"] <= 10 * bound):
                     raise RuntimeError(f"{name}: a request's logits in the batch differ from the same request alone: {chk} "
                                        f"(allowed: mean {bound:.1e}, max {10 * bound:.1e} of the logit range)")
         for b in (1, 64):
