@@ -68,3 +68,24 @@ def test_write_of_aligned_rows(ops, case, dt, more):
             least, most = (np.array([[F.scale_byte(r[part]) for r in tok] for tok in t]) for t in (np.maximum(np.abs(ref) - off, 0), np.abs(ref) + off))
             assert ((least <= byte[..., block]) & (byte[..., block] <= most)).all()
         row += n
+
+
+@pytest.mark.parametrize("more", [0, 1])          # (an odd stride: the kernel that reads channel by channel)
+@pytest.mark.parametrize("start", [0, 60000, 130000])
+def test_cosines_and_sines_next_to_their_zeros(ops, start, more):
+    """Queries (1, 0) turn into the angle's cosine and sine.  Of each number: four steps for the function, as OpenCL's table of errors allows it, half a step each
+    for what is put back, the scale and the product, 6 * 2^-23 in all; and the angle itself, up to 21,000 turns that are rounded in 64 bits twice, 2^-52 of them each."""
+    from xyntetik_runner_amd.csrc.ops import FourBitPages
+    n, D, page = 700, 128, 64
+    ctx = step([start], [n], [[0] * (start // page) + list(range(1, 13))])
+    inv = (1.0 / 10000.0 ** (np.arange(0, D, 2) / D)).astype(np.float32)
+    x = torch.zeros((n, 3 * D + more), device=DEV)
+    x[:, :D // 2] = 1.0
+    q = torch.empty((n, D), device=DEV)
+    kp, vp = (FourBitPages.zeros(13, 1, page, D, values, DEV) for values in (False, True))
+    ops.rope_kv_write(x[:, :D], x[:, D:2 * D], x[:, 2 * D:3 * D], q, kp, vp, ctx.positions, ctx.req_of_token, ctx.block_table(0), torch.tensor(inv, device=DEV),
+                      1, 1, D, D, False, 1.0, page)
+    angle = np.arange(start, start + n)[:, None] * inv.astype(np.float64)
+    want = np.concatenate([np.cos(angle), np.sin(angle)], axis=1)
+    assert np.abs(want)[:, :-1].min() < 1e-4                # (some lie next to a zero)
+    assert (np.abs(q.cpu().double().numpy() - want) <= 6 * 2.0 ** -23 * np.abs(want) + 2 * np.abs(np.tile(angle, 2)) * 2.0 ** -52 + 2.0 ** -50).all()

@@ -132,9 +132,11 @@ __global__ __launch_bounds__(256) void k_rope_kv_write4(Write4Args a) {
     for (int j = threadIdx.x; j < half; j += 256) {
         double turns = (double)pos * (double)a.inv_freq[j] * 0.15915494309189533577;
         turns -= rint(turns);
+        // (what the angle loses as a 32-bit number is put back: cos(x + d) = cos x - d sin x, sin(x + d) = sin x + d cos x)
+        const float x = (float)(2.0 * turns), d = (float)((2.0 * turns - x) * 3.14159265358979323846);
         float s, c;
-        sincospif((float)(2.0 * turns), &s, &c);
-        cs[j & 7][j >> 3] = make_float2(c * a.mscale, s * a.mscale);
+        sincospif(x, &s, &c);
+        cs[j & 7][j >> 3] = make_float2(fmaf(-d, s, c) * a.mscale, fmaf(d, c, s) * a.mscale);
     }
     const int bi = pos >> a.page_shift, off = pos & a.page_mask;
     const int page = bi >= 0 && bi < a.table_width && (unsigned)req < (unsigned)a.n_requests ? a.block_table[(size_t)req * a.table_stride + bi] : -1;
