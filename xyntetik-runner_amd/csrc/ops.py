@@ -1115,7 +1115,8 @@ class Ops:
         their own (bfloat16, sizes in whole blocks of 32, pages of at least 32 positions, no kept first keys).  The pages of others are read
         back first (``read_pages``) where matrix cores then have enough rows; what is left, and what a step that is being recorded cannot read back,
         a 32-bit kernel serves from the codes.  Keys in pages that do not exist (given back, past the table or the pool) are in no row's sum, and a row
-        without keys and sink comes back as zeros.  Calls that share a step's context follow one another (they share its counters): on one stream, or
+        without keys and sink comes back as zeros.  A block that reads as NaN shows in the rows that see it; behind pages read back, a value's in other rows of the
+        request, too, as over 16-bit pages.  Calls that share a step's context follow one another (they share its counters): on one stream, or
         behind an event.
         """
         if isinstance(k_cache, FourBitPages) or isinstance(v_cache, FourBitPages):

@@ -370,7 +370,8 @@ struct Read4Args {
 };
 
 // Rows of a list of (request, position): a thread 8 channels of a head, whose codes are one word (of a value: 4 bytes 8 apart, in lines that the row's neighbours
-// share).  Rows without a page read as zeros.  Bound by what it writes: 2,048 rows of 8 heads of 128, 16 bits, take 7.2 us (8.4 MB out; the neighbours' lines come from L2), one 2.5.
+// share).  Rows without a page read as zeros.  2,048 rows of 8 heads of 128, 16 bits, take 7.2 us for 9.5 MB, 1.3 TB/s of the 5.06 of a large copy: not memory, but three trips that wait for one
+// another (position, page, codes: one row takes 2.5) and a value's codes byte by byte.
 template <typename T>
 __global__ __launch_bounds__(256) void k_read_rows4(Read4Args a) {
     for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < a.total; i += (size_t)gridDim.x * 256) {
@@ -396,7 +397,7 @@ __global__ __launch_bounds__(256) void k_read_rows4(Read4Args a) {
 }
 
 // Whole pages in the layout of 16- and 32-bit caches (values transposed), a workgroup a page and head.  What lies behind a request's
-// end becomes zero, so that readers may multiply it.  Bound by memory: 32,768 positions of 8 heads of 128 (36 MB in, 134 MB out, 16 bits) take 27.4 us, 6.2 TB/s;
+// end becomes zero, so that readers may multiply it.  Bound by memory: 32,768 positions of 8 heads of 128 (36 MB in, 134 MB out, 16 bits) take 37 us, 4.6 TB/s, and 27.4 where the results of a call before lie in the last cache;
 // 13,300 of 8 heads of 64 in 32 bits (7 MB in, 55 MB out) 13.5, 4.6 TB/s.
 template <typename T>
 __global__ __launch_bounds__(256) void k_read_pages4(Read4Args a) {
@@ -486,7 +487,7 @@ extern "C" int xr_read_pages4(void* k_out, void* v_out, void* kc, void* ks, void
 // lane for the values, 8 positions at a time as they lie side by side; the options of k_attention_ref.  For what the matrix-core kernel does not take: 32-bit
 // queries of few rows, head sizes that end inside a block and, in recorded steps, whose pages cannot be read back first, the other sizes and kept first keys.
 //
-// Bound by instructions: every query head converts its keys and values again, and beside a product stand half a conversion and the shared memory's reads of the
+// Bound by instructions as the work is shared out: every query head converts its keys and values again (and a request's keys are not cut into ranges: few requests leave compute units idle), and beside a product stand half a conversion and the shared memory's reads of the
 // query.  8 requests of 4,000 keys, 32 heads of 128 over 8, take 57 us (9 TFLOP/s; channel by channel with a byte a load 252), 64 of 8,000 with heads of 64 344 (12 TFLOP/s).
 #define ANY4_WAVES 8
 struct Any4Args {
